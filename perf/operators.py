@@ -115,14 +115,15 @@ def _randn(g, *shape):
 
 
 def _quantized(x, q, rows=1):
-    """fp8 codes and scales of random data, in the layout the product takes."""
+    """fp8 codes and scales of random data. Scales of rows are stored block by block, as the framework's quantized outputs
+    hold them."""
     m, k = x.shape
     mb, kb = -(-m // rows), -(-k // BLOCK)
     padded = torch.zeros(mb * rows, kb * BLOCK, device=DEVICE)
     padded[:m, :k] = x
     scale = padded.view(mb, rows, kb, BLOCK).abs().amax((1, 3)) / LARGEST[q]
     codes = x / scale.repeat_interleave(rows, 0)[:m].repeat_interleave(BLOCK, 1)[:, :k]
-    return codes.to(DTYPES[q]), scale
+    return codes.to(DTYPES[q]), scale.t().contiguous().t() if rows == 1 else scale
 
 
 def _weight(g, n, k, q, by_row=False):

@@ -1,0 +1,240 @@
+// What the operators with one scale for each block of 128 values share (include/feather_block_ops.h): 8-value pieces of
+// rows, and the quantization of blocks.
+//
+// A row is handled in pieces of 8 consecutive values, one per lane and step, so a block of 128 is the 16 lanes of one DPP
+// row: its largest value takes four row rotations and no LDS. Rows whose start or stride is not 16-byte aligned, and a
+// row's last piece where it is short, go value by value.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "feather_block_ops.h"
+
+namespace feather {
+
+constexpr int kBlock = 128;           // values per scale
+constexpr int kPiece = 8;             // values per lane and step
+constexpr uint32_t kLeastBits = 27u << 23;  // 2^-100: the least a block's largest value counts as
+
+using u32x4v = uint32_t __attribute__((ext_vector_type(4)));
+using u32x2v = uint32_t __attribute__((ext_vector_type(2)));
+
+// Bytes of one value of `type`.
+__host__ __device__ constexpr int type_bytes(int type) { return type == FEATHER_FP32 ? 4 : 2; }
+
+template <int kType>
+__device__ __forceinline__ float to_float(uint32_t bits) {
+    if constexpr (kType == FEATHER_BF16) return __builtin_bit_cast(float, bits << 16);
+    if constexpr (kType == FEATHER_FP16)
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+    return __builtin_bit_cast(float, bits);
+}
+
+// v rounded to the type (nearest even; subnormals and NaN kept), as its bits.
+template <int kType>
+__device__ __forceinline__ uint32_t to_bits(float v) {
+    if constexpr (kType == FEATHER_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
+    if constexpr (kType == FEATHER_FP16) return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// Two values rounded to a 16-bit type and packed, the first one lowest.
+template <int kType>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    using f32x2 = float __attribute__((ext_vector_type(2)));
+    if constexpr (kType == FEATHER_BF16) {
+        using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+    } else {
+        using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), f16x2));
+    }
+}
+
+// v[0..7] = the 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are
+// zero. kVec: the row and `at` are such that whole pieces are 16-byte aligned.
+template <int kType, bool kVec>
+__device__ __forceinline__ void load_piece(const void* row, int at, int valid, float (&v)[kPiece]) {
+    if (kVec && valid >= kPiece) {
+        if constexpr (kType == FEATHER_FP32) {
+            const auto* p = reinterpret_cast<const u32x4v*>(static_cast<const float*>(row) + at);
+            const u32x4v a = p[0], b = p[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x = a[i], y = b[i];
+                v[i] = __builtin_bit_cast(float, x);
+                v[4 + i] = __builtin_bit_cast(float, y);
+            }
+        } else {
+            const u32x4v a = *reinterpret_cast<const u32x4v*>(static_cast<const uint16_t*>(row) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x = a[i];
+                v[2 * i] = to_float<kType>(x & 0xffffu);
+                v[2 * i + 1] = to_float<kType>(x >> 16);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+        uint32_t bits = 0;
+        if (i < valid) {
+            if constexpr (kType == FEATHER_FP32) bits = static_cast<const uint32_t*>(row)[at + i];
+            else bits = static_cast<const uint16_t*>(row)[at + i];
+        }
+        v[i] = to_float<kType>(bits);
+    }
+}
+
+template <int kType, bool kVec>
+__device__ __forceinline__ void store_piece(void* row, int at, int valid, const float (&v)[kPiece]) {
+    if (kVec && valid >= kPiece) {
+        if constexpr (kType == FEATHER_FP32) {
+            auto* p = reinterpret_cast<u32x4v*>(static_cast<float*>(row) + at);
+            p[0] = u32x4v{to_bits<kType>(v[0]), to_bits<kType>(v[1]), to_bits<kType>(v[2]), to_bits<kType>(v[3])};
+            p[1] = u32x4v{to_bits<kType>(v[4]), to_bits<kType>(v[5]), to_bits<kType>(v[6]), to_bits<kType>(v[7])};
+        } else {
+            *reinterpret_cast<u32x4v*>(static_cast<uint16_t*>(row) + at) =
+                u32x4v{pack2<kType>(v[0], v[1]), pack2<kType>(v[2], v[3]), pack2<kType>(v[4], v[5]),
+                       pack2<kType>(v[6], v[7])};
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+        if (i < valid) {
+            if constexpr (kType == FEATHER_FP32) static_cast<uint32_t*>(row)[at + i] = to_bits<kType>(v[i]);
+            else static_cast<uint16_t*>(row)[at + i] = static_cast<uint16_t>(to_bits<kType>(v[i]));
+        }
+    }
+}
+
+// A norm's weight: of the activations' type or fp32 (kVec: 16-byte aligned).
+template <int kType, bool kVec>
+__device__ __forceinline__ void load_weight(const void* w, bool fp32, int at, int valid, float (&v)[kPiece]) {
+    if (kType != FEATHER_FP32 && fp32) load_piece<FEATHER_FP32, kVec>(w, at, valid, v);
+    else load_piece<kType, kVec>(w, at, valid, v);
+}
+
+// ---- reductions without LDS -------------------------------------------------------------------------------
+
+template <int kRotate>
+__device__ __forceinline__ uint32_t row_ror(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x120 + kRotate, 0xf, 0xf, true));
+}
+
+// The largest of 16 lanes' values, in each of them.
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    v = max(v, row_ror<8>(v));
+    v = max(v, row_ror<4>(v));
+    v = max(v, row_ror<2>(v));
+    return max(v, row_ror<1>(v));
+}
+
+__device__ __forceinline__ float add_ror(float v, uint32_t r) { return v + __builtin_bit_cast(float, r); }
+
+// The wave's sum, in every lane.
+__device__ __forceinline__ float sum64(float v) {
+    v = add_ror(v, row_ror<8>(__builtin_bit_cast(uint32_t, v)));
+    v = add_ror(v, row_ror<4>(__builtin_bit_cast(uint32_t, v)));
+    v = add_ror(v, row_ror<2>(__builtin_bit_cast(uint32_t, v)));
+    v = add_ror(v, row_ror<1>(__builtin_bit_cast(uint32_t, v)));
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// ---- quantization -------------------------------------------------------------------------------------------
+
+// |v| as bits: ordered like the values, infinity above them and NaN above infinity, so an unsigned maximum keeps NaN.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t max_bits(const float (&v)[kPiece]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) m = max(m, abs_bits(v[i]));
+    return m;
+}
+
+// A block's scale and the factor that takes its values to codes. A product with L / amax in place of the quotient by
+// amax / L: one division a block instead of one a value. The product of the largest value is at most L (1 + 2^-22), which
+// rounds to L, so codes need no clamp.
+__device__ __forceinline__ float block_scale(uint32_t amax_bits, bool e5m2, float& factor) {
+    const float amax = __builtin_bit_cast(float, max(amax_bits, kLeastBits));
+    const float largest = e5m2 ? 57344.0f : 448.0f;
+    factor = largest / amax;
+    return amax / largest;
+}
+
+// Four values times factor -> four codes, the first one lowest.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float factor, bool e5m2) {
+    int out = 0;
+    if (e5m2) {
+        out = __builtin_amdgcn_cvt_pk_bf8_f32(a * factor, b * factor, out, false);
+        out = __builtin_amdgcn_cvt_pk_bf8_f32(c * factor, d * factor, out, true);
+    } else {
+        out = __builtin_amdgcn_cvt_pk_fp8_f32(a * factor, b * factor, out, false);
+        out = __builtin_amdgcn_cvt_pk_fp8_f32(c * factor, d * factor, out, true);
+    }
+    return static_cast<uint32_t>(out);
+}
+
+// Where the quantized form of a matrix goes: rows of codes and block scales.
+struct Quantized {
+    uint8_t* codes;
+    float* scale;
+    int64_t ld_codes, scale_row, scale_block;
+    int e5m2;
+};
+
+// One piece of a row quantized with its block's 16 lanes, all of which call this together (with valid <= 0 past the row's
+// end): writes its codes, and the block's first lane the scale. kVec: ld_codes and codes are multiples of 8.
+template <bool kVec>
+__device__ __forceinline__ void quantize_piece(const Quantized& q, int64_t row, int at, int valid,
+                                               const float (&v)[kPiece]) {
+    float factor;
+    const float scale = block_scale(max16(max_bits(v)), q.e5m2, factor);
+    if (valid <= 0) return;
+    const u32x2v codes{codes4(v[0], v[1], v[2], v[3], factor, q.e5m2), codes4(v[4], v[5], v[6], v[7], factor, q.e5m2)};
+    uint8_t* out = q.codes + row * q.ld_codes + at;
+    if (kVec && valid >= kPiece) {
+        *reinterpret_cast<u32x2v*>(out) = codes;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) {
+            const uint32_t word = codes[i / 4];
+            if (i < valid) out[i] = static_cast<uint8_t>(word >> (8 * (i % 4)));
+        }
+    }
+    if (at % kBlock == 0) q.scale[row * q.scale_row + (at / kBlock) * q.scale_block] = scale;
+}
+
+// ---- host-side checks ---------------------------------------------------------------------------------------
+
+inline bool on_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Whether rows of `type` with stride ld start on 16-byte boundaries.
+inline bool rows_on_16(const void* p, int64_t ld, int type) { return on_16(p) && ld * type_bytes(type) % 16 == 0; }
+
+constexpr int64_t kMaxSize = (int64_t{1} << 31) - 1;
+
+// A matrix that the kernels can walk: sizes under 2^31 and rows under 2 GiB, no stride under the row's length.
+inline bool matrix_ok(const void* p, int64_t ld, int64_t rows, int64_t cols) {
+    return p != nullptr && rows >= 1 && rows <= kMaxSize && cols >= 1 && cols <= kMaxSize / 4 && ld >= cols &&
+           ld <= kMaxSize / 4;
+}
+
+inline bool type_ok(int type) { return type == FEATHER_BF16 || type == FEATHER_FP16 || type == FEATHER_FP32; }
+
+inline bool aligned_to_type(const void* p, int type) {
+    return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(type_bytes(type) - 1)) == 0;
+}
+
+// Codes and scales to write, or neither.
+inline bool quantized_ok(const uint8_t* codes, int64_t ld_codes, const float* scale, int64_t rows, int64_t cols) {
+    return matrix_ok(codes, ld_codes, rows, cols) && scale != nullptr && aligned_to_type(scale, FEATHER_FP32);
+}
+
+}  // namespace feather

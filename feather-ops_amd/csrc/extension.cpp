@@ -8,21 +8,16 @@
 #include <torch/csrc/stable/library.h>
 #include <torch/csrc/stable/tensor.h>
 
-#include <hip/hip_runtime_api.h>
-
 #include <cstdint>
 #include <optional>
 
+#include "extension_common.h"
 #include "feather_internal.h"
 
 namespace {
 
 using torch::stable::Tensor;
 using ST = torch::headeronly::ScalarType;
-
-bool is_aligned(const void* p, uintptr_t bytes) {
-    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
-}
 
 // What the C ABI needs of one validated scaled_mm call.
 struct Operands {
@@ -115,18 +110,6 @@ Operands check_operands(const Tensor& a, const Tensor& b_prepacked, const std::o
     }
     return Operands{M, N, K, scale_mode, b_type == ST::Float8_e5m2, a_type == ST::BFloat16,
                     c.scalar_type() == ST::BFloat16, device_index};
-}
-
-hipStream_t current_stream(int32_t device_index) {
-    void* raw_stream = nullptr;
-    TORCH_ERROR_CODE_CHECK(aoti_torch_get_current_cuda_stream(device_index, &raw_stream));
-    return static_cast<hipStream_t>(raw_stream);
-}
-
-void check_launch(bool launched, const char* what) {
-    STD_TORCH_CHECK(launched, "Unsupported config");
-    const hipError_t err = hipGetLastError();
-    STD_TORCH_CHECK(err == hipSuccess, what, " kernel launch failed: ", hipGetErrorString(err));
 }
 
 // feather_ops::scaled_mm (csrc/hip_kernel.cu:716-823 of the reference).

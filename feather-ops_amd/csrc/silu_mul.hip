@@ -1,0 +1,141 @@
+// Gated activation silu(gate) * up with 16-bit, fp32 or block-scaled fp8 output, its backward, and the quantization of
+// rows to blocks of 128 (include/feather_block_ops.h).
+//
+//   s = 1 / (1 + exp(-g))     y = g s u     grad_u = grad_y g s     grad_g = grad_y u s (1 + g (1 - s))
+//
+// Streams through memory: a lane takes one piece of 8 values at a time, the 16 lanes of a block together. Pieces are
+// counted over all rows, whole blocks to a row, so that short rows fill the waves too.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "block_common.h"
+
+namespace feather {
+namespace {
+
+constexpr int kThreads = 256;
+
+enum class Op { kQuantize, kSiluMul, kSiluMulBackward };
+
+struct RowsParams {
+    const void* x;          // the values; gate and up side by side
+    const void* grad_y;
+    void* y;                // null: q; grad_x of the backward
+    Quantized q;
+    int64_t ldx, ld_grad_y, ldy, rows;
+    int32_t cols, pieces;   // of a row: a multiple of 16
+};
+
+template <int kType>
+__device__ __forceinline__ const void* row_at(const void* p, int64_t row, int64_t ld) {
+    return static_cast<const uint8_t*>(p) + row * ld * type_bytes(kType);
+}
+
+// 1 / (1 + exp(-g)): exp overflows to infinity for g < -88, and the quotient is then zero.
+__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + __expf(-g)); }
+
+template <Op kOp, int kType, bool kVec>
+__global__ __launch_bounds__(kThreads) void rows_kernel(const RowsParams p) {
+    // The workgroup's first piece as (row, piece of it), then this lane's from there in 32 bits.
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
+    const int64_t first_row = first / p.pieces;
+    const uint32_t piece0 = static_cast<uint32_t>(first - first_row * p.pieces) + threadIdx.x;
+    const uint32_t more = piece0 / static_cast<uint32_t>(p.pieces);
+    const int64_t row = first_row + more;
+    if (row >= p.rows) return;   // whole blocks of lanes: a row's pieces are a multiple of 16
+    const int at = static_cast<int>(piece0 - more * static_cast<uint32_t>(p.pieces)) * kPiece;
+    const int valid = p.cols - at;
+    float v[kPiece];
+    const void* x = row_at<kType>(p.x, row, p.ldx);
+    load_piece<kType, kVec>(x, at, valid, v);
+    if constexpr (kOp != Op::kQuantize) {
+        float up[kPiece];
+        load_piece<kType, kVec>(x, p.cols + at, valid, up);
+        if constexpr (kOp == Op::kSiluMul) {
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i) v[i] = v[i] * sigmoid(v[i]) * up[i];
+        } else {
+            float g[kPiece];
+            load_piece<kType, kVec>(row_at<kType>(p.grad_y, row, p.ld_grad_y), at, valid, g);
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i) {
+                const float s = sigmoid(v[i]);
+                const float grad_up = g[i] * v[i] * s;
+                v[i] = g[i] * up[i] * s * (1.0f + v[i] * (1.0f - s));
+                up[i] = grad_up;
+            }
+            void* out = static_cast<uint8_t*>(p.y) + row * p.ldy * type_bytes(kType);
+            store_piece<kType, kVec>(out, at, valid, v);
+            store_piece<kType, kVec>(out, p.cols + at, valid, up);
+            return;
+        }
+        if (p.y) {
+            store_piece<kType, kVec>(static_cast<uint8_t*>(p.y) + row * p.ldy * type_bytes(kType), at, valid, v);
+            return;
+        }
+    }
+    quantize_piece<kVec>(p.q, row, at, valid, v);
+}
+
+template <Op kOp>
+bool launch(const RowsParams& p, int type, bool vec, hipStream_t stream) {
+    const int64_t groups = (p.rows * p.pieces + kThreads - 1) / kThreads;
+    if (groups > kMaxSize) return false;
+    const auto go = [&](auto t) {
+        if (vec) rows_kernel<kOp, t(), true><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(p);
+        else rows_kernel<kOp, t(), false><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(p);
+    };
+    if (type == FEATHER_BF16) go(std::integral_constant<int, FEATHER_BF16>{});
+    else if (type == FEATHER_FP16) go(std::integral_constant<int, FEATHER_FP16>{});
+    else go(std::integral_constant<int, FEATHER_FP32>{});
+    return true;
+}
+
+int32_t pieces_of(int64_t cols) { return static_cast<int32_t>((cols + kBlock - 1) / kBlock * (kBlock / kPiece)); }
+
+}  // namespace
+}  // namespace feather
+
+using namespace feather;
+
+extern "C" bool feather_quantize_blocks(const void* x, int type, int64_t ldx, uint8_t* codes, int64_t ld_codes,
+                                        float* scale, int64_t scale_row, int64_t scale_block, bool e5m2, int64_t rows,
+                                        int64_t cols, hipStream_t stream) {
+    if (!type_ok(type) || !matrix_ok(x, ldx, rows, cols) || !aligned_to_type(x, type) ||
+        !quantized_ok(codes, ld_codes, scale, rows, cols))
+        return false;
+    const RowsParams p{x, nullptr, nullptr, {codes, scale, ld_codes, scale_row, scale_block, e5m2}, ldx, 0, 0, rows,
+                       static_cast<int32_t>(cols), pieces_of(cols)};
+    return launch<Op::kQuantize>(p, type, rows_on_16(x, ldx, type) && on_16(codes) && ld_codes % 8 == 0, stream);
+}
+
+extern "C" bool feather_silu_mul(const void* x, int64_t ldx, int type, void* y, int64_t ldy, uint8_t* codes,
+                                 int64_t ld_codes, float* scale, int64_t scale_row, int64_t scale_block, bool e5m2,
+                                 int64_t rows, int64_t cols, hipStream_t stream) {
+    if (!type_ok(type) || !matrix_ok(x, ldx, rows, cols) || ldx < 2 * cols || !aligned_to_type(x, type)) return false;
+    if (y ? codes || scale || !matrix_ok(y, ldy, rows, cols) || !aligned_to_type(y, type)
+          : !quantized_ok(codes, ld_codes, scale, rows, cols))
+        return false;
+    const RowsParams p{x, nullptr, y, {codes, scale, ld_codes, scale_row, scale_block, e5m2}, ldx, 0, ldy, rows,
+                       static_cast<int32_t>(cols), pieces_of(cols)};
+    // up starts at column cols: on a 16-byte boundary too
+    const bool vec = rows_on_16(x, ldx, type) && cols * type_bytes(type) % 16 == 0 &&
+                     (y ? rows_on_16(y, ldy, type) : (on_16(codes) && ld_codes % 8 == 0));
+    return launch<Op::kSiluMul>(p, type, vec, stream);
+}
+
+extern "C" bool feather_silu_mul_backward(const void* grad_y, int64_t ld_grad_y, const void* x, int64_t ldx, int type,
+                                          void* grad_x, int64_t ld_grad_x, int64_t rows, int64_t cols,
+                                          hipStream_t stream) {
+    if (!type_ok(type) || !matrix_ok(x, ldx, rows, cols) || ldx < 2 * cols || !matrix_ok(grad_y, ld_grad_y, rows, cols) ||
+        !matrix_ok(grad_x, ld_grad_x, rows, cols) || ld_grad_x < 2 * cols || !aligned_to_type(x, type) ||
+        !aligned_to_type(grad_y, type) || !aligned_to_type(grad_x, type))
+        return false;
+    const RowsParams p{x, grad_y, grad_x, {}, ldx, ld_grad_y, ld_grad_x, rows, static_cast<int32_t>(cols),
+                       pieces_of(cols)};
+    const bool vec = rows_on_16(x, ldx, type) && cols * type_bytes(type) % 16 == 0 &&
+                     rows_on_16(grad_y, ld_grad_y, type) && rows_on_16(grad_x, ld_grad_x, type);
+    return launch<Op::kSiluMulBackward>(p, type, vec, stream);
+}

@@ -139,6 +139,9 @@ Tensor block_scaled_mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, 
                     "b_scale must be [", blocks_of(N), ", ", kb, "], one scale for each 128 x 128 block of b, or [", N,
                     ", ", kb, "], one for each row and block of 128 columns");
     const bool by_row = b_scale.size(0) != blocks_of(N);
+    const int64_t as_row = a_scale.size(0) > 1 ? a_scale.stride(0) : 0;
+    const int64_t bs_row = b_scale.size(0) > 1 ? b_scale.stride(0) : 0;
+    STD_TORCH_CHECK(as_row <= (1 << 20) && bs_row <= (1 << 20), "the scales' rows are too far apart");
     STD_TORCH_CHECK(out_type >= 0 && out_type <= 2, "the output must be bfloat16, float16 or float32");
     const int type = static_cast<int>(out_type);
     if (bias.has_value()) {
@@ -160,9 +163,9 @@ Tensor block_scaled_mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, 
     }
     torch::stable::accelerator::DeviceGuard guard(device_index);
     check_launch(feather_block_scaled_mm(
-                     static_cast<const uint8_t*>(a.const_data_ptr()), lda, a_e5m2, floats(a_scale), a_scale.stride(0),
-                     a_scale.stride(1), static_cast<const uint8_t*>(b.const_data_ptr()), ldb, b_e5m2, floats(b_scale),
-                     b_scale.stride(0), b_scale.stride(1), by_row, bias.has_value() ? bias->const_data_ptr() : nullptr,
+                     static_cast<const uint8_t*>(a.const_data_ptr()), lda, a_e5m2, floats(a_scale), as_row,
+                     a_scale.stride(1), static_cast<const uint8_t*>(b.const_data_ptr()), ldb, b_e5m2, floats(b_scale), bs_row,
+                     b_scale.stride(1), by_row, bias.has_value() ? bias->const_data_ptr() : nullptr,
                      c.mutable_data_ptr(), N, type, M, N, K, need > 0 ? workspace->mutable_data_ptr() : nullptr,
                      need > 0 ? workspace->numel() : 0, current_stream(device_index)),
                  "block_scaled_mm");

@@ -35,7 +35,7 @@ struct BlockMmParams {
     void* c;
     int64_t ldc;
     int32_t out_type;
-    int32_t store4;         // four neighbouring outputs are one aligned store
+    int32_t store4, store8; // four and eight neighbouring outputs (and biases) are aligned stores
     uint32_t* split_ctr;
     uint8_t* split_part;
 };

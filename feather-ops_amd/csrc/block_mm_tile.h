@@ -1,0 +1,271 @@
+// The tile kernel of the block-scaled fp8 product: a workgroup owns BM x BN outputs, its WM x WN waves split them, and K
+// streams through an LDS ring of one-block (128-deep) stages that direct global-to-LDS loads fill.
+#pragma once
+
+#include "block_mm_common.h"
+
+namespace feather {
+
+template <int BM_, int BN_, int WM_, int WN_, int kSlots_>
+struct BlockTile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kSlots = kSlots_;
+    static constexpr int kWaves = WM * WN;
+    static constexpr int kThreads = 64 * kWaves;
+    static constexpr int RM = BM / WM / 16;             // 16-row fragments of a per wave
+    static constexpr int RN = BN / WN / 16;             // and of b
+    static constexpr int kABytes = BM * kBlock;         // a stage: rows of 128 bytes, 16-byte pieces XOR-swizzled
+    static constexpr int kBBytes = BN * kBlock;
+    static constexpr int kScaleBytes = (BM + BN) * 4;   // each row's scale of the block
+    static constexpr int kStageBytes = kABytes + kBBytes + kScaleBytes;
+    static constexpr int kLdsBytes = kSlots * kStageBytes;
+    static constexpr int kALoads = kABytes / 1024 / kWaves;
+    static constexpr int kBLoads = kBBytes / 1024 / kWaves;
+    static constexpr int kScaleLoads = (BM + BN) / 64;  // of the workgroup, one a wave (some twice)
+    static constexpr int kLoads = kALoads + kBLoads + 1;
+    static_assert(kABytes % (1024 * kWaves) == 0 && kBBytes % (1024 * kWaves) == 0, "whole loads");
+    static_assert(kScaleLoads <= kWaves, "one scale load a wave");
+    static_assert(RM % 2 == 0 && RM >= 2, "fragments of a go through two registers");
+    static_assert(kBlock % (BN / WN) == 0, "a wave's columns have one square scale");
+    static_assert((kSlots - 1) * kLoads < 64, "vmcnt range");
+};
+
+// 4 bytes per lane straight into LDS.
+__device__ __forceinline__ void dma4(rsrc_t r, const uint8_t* lds_dst, uint32_t voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        r, (__attribute__((address_space(3))) void*)(reinterpret_cast<uintptr_t>(lds_dst)), 4, static_cast<int>(voff), 0,
+        0, 0);
+}
+
+// The epilogue: a wave's 16 RN-column outputs, 16 rows at a time through LDS of its own, so that a row leaves as whole
+// pieces of 8 outputs on neighbouring lanes, or, where rows are not aligned, value by value on neighbouring lanes.
+template <int RN>
+struct OutRow {
+    static constexpr int kCols = 16 * RN;
+    static constexpr int kPitch = kCols + 4;    // floats: the 16 rows' writes of a column fall on different banks
+};
+
+template <int kType, bool kVec, int RM, int RN>
+__device__ __forceinline__ void store_typed(const BlockMmParams& p, const f32x4 (&acc)[RM][RN], int row0, int col0,
+                                            int lane, float* own) {
+    using O = OutRow<RN>;
+    constexpr int kLanes = kVec ? O::kCols / 8 : O::kCols;   // of a row
+    const int r16 = lane % 16;
+    const int g = lane / 16;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+#pragma unroll
+        for (int j = 0; j < RN; ++j) *reinterpret_cast<f32x4*>(own + r16 * O::kPitch + 16 * j + 4 * g) = acc[i][j];
+        __builtin_amdgcn_s_waitcnt(kLgkm0Imm);   // a wave's LDS operations are done in order
+#pragma unroll
+        for (int at = 0; at < 16 * kLanes; at += 64) {
+            const int r = (at + lane) / kLanes;
+            const int c = (at + lane) % kLanes * (kVec ? 8 : 1);
+            const int m = row0 + 16 * i + r;
+            const int n = col0 + c;
+            if (m >= p.M || n >= p.N || r >= 16) continue;
+            const float* from = own + r * O::kPitch + c;
+            if constexpr (kVec) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = from[e];
+                if (p.bias) {
+                    float add[8];
+                    load_piece<kType, true>(p.bias, n, 8, add);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += add[e];
+                }
+                uint8_t* out = static_cast<uint8_t*>(p.c) + static_cast<int64_t>(m) * p.ldc * type_bytes(kType);
+                store_piece<kType, true>(out, n, 8, v);
+            } else {
+                float v = *from;
+                const int64_t to = static_cast<int64_t>(m) * p.ldc + n;
+                if constexpr (kType == FEATHER_FP32) {
+                    if (p.bias) v += static_cast<const float*>(p.bias)[n];
+                    static_cast<float*>(p.c)[to] = v;
+                } else {
+                    if (p.bias) v += to_float<kType>(static_cast<const uint16_t*>(p.bias)[n]);
+                    static_cast<uint16_t*>(p.c)[to] = static_cast<uint16_t>(to_bits<kType>(v));
+                }
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
+    }
+}
+
+template <int RM, int RN>
+__device__ __forceinline__ void store_tile(const BlockMmParams& p, const f32x4 (&acc)[RM][RN], int row0, int col0, int lane,
+                                           float* own) {
+    const auto go = [&](auto type) {
+        if (p.store8) store_typed<type(), true>(p, acc, row0, col0, lane, own);
+        else store_typed<type(), false>(p, acc, row0, col0, lane, own);
+    };
+    if (p.out_type == FEATHER_BF16) go(std::integral_constant<int, FEATHER_BF16>{});
+    else if (p.out_type == FEATHER_FP16) go(std::integral_constant<int, FEATHER_FP16>{});
+    else go(std::integral_constant<int, FEATHER_FP32>{});
+}
+
+template <typename T, bool kAE5M2, bool kBE5M2, bool kByRow>
+__global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmParams p) {
+    constexpr int RM = T::RM, RN = T::RN;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLdsBytes];
+    const int tid = threadIdx.x;
+    const int lane = tid % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wave_m = wave / T::WN;
+    const int wave_n = wave % T::WN;
+    const int tiles_m = (p.M + T::BM - 1) / T::BM;
+    const int tiles_n = (p.N + T::BN - 1) / T::BN;
+    int tm, tn;
+    tile_of_block(static_cast<int>(blockIdx.x), tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * T::BM;
+    const int n0 = tn * T::BN;
+    const int stages = (p.K + kBlock - 1) / kBlock;
+
+    // Direct loads: each fills 8 rows of 8 pieces; lane l's place is piece l % 8 of row l / 8, which holds the row's piece
+    // (l % 8) ^ (row % 8), so that 8 rows' reads of one piece fall on 8 different places.
+    const rsrc_t a_rsrc = rows_rsrc(p.a, p.lda, m0, p.M, T::BM, p.K);
+    const rsrc_t b_rsrc = rows_rsrc(p.b, p.ldb, n0, p.N, T::BN, p.K);
+    const rsrc_t null_rsrc = make_rsrc(p.a, 0u);
+    const int piece_at = ((lane % 8) ^ (lane / 8)) * 16;
+    const uint32_t a_off = static_cast<uint32_t>(wave * 8 + lane / 8) * static_cast<uint32_t>(p.lda) + piece_at;
+    const uint32_t b_off = static_cast<uint32_t>(wave * 8 + lane / 8) * static_cast<uint32_t>(p.ldb) + piece_at;
+    const uint32_t a_step = 8u * T::kWaves * static_cast<uint32_t>(p.lda);
+    const uint32_t b_step = 8u * T::kWaves * static_cast<uint32_t>(p.ldb);
+    // This wave's 64 scales of a stage.
+    const int scale_load = wave % T::kScaleLoads;
+    const bool scale_a = scale_load < T::BM / 64;
+    const int scale_row = scale_load * 64 + lane - (scale_a ? 0 : T::BM);
+    uint32_t scale_off;
+    {
+        const int row = scale_a ? m0 + scale_row : n0 + scale_row;
+        const int64_t first = scale_a ? m0 : kByRow ? n0 : n0 / kBlock;
+        const int64_t index = scale_a || kByRow ? row : row / kBlock;
+        const bool there = row < (scale_a ? p.M : p.N);
+        scale_off = there ? static_cast<uint32_t>((index - first) * (scale_a ? p.as_row : p.bs_row)) * 4u : kOob;
+    }
+    const float* scale_base = scale_a ? p.a_scale + m0 * p.as_row
+                                      : p.b_scale + (kByRow ? static_cast<int64_t>(n0) : n0 / kBlock) * p.bs_row;
+    const int64_t scale_block = scale_a ? p.as_block : p.bs_block;
+
+    // Load d of stage kb (past the last: nothing, into a slot nobody reads).
+    const auto load = [&](int d, int kb, uint32_t slot) {
+        const bool live = kb < stages;
+        uint8_t* const stage = lds + slot;
+        if (d < T::kALoads + T::kBLoads) {
+            const bool is_a = d < T::kALoads;
+            const int i = is_a ? d : d - T::kALoads;
+            const uint32_t off = is_a ? a_off + i * a_step : b_off + i * b_step;
+            const bool there = piece_at < p.K - kb * kBlock;
+            dma16(live ? (is_a ? a_rsrc : b_rsrc) : null_rsrc, stage + (is_a ? 0 : T::kABytes) + (wave + i * T::kWaves) * 1024,
+                  there ? off : kOob, static_cast<uint32_t>(kb) * kBlock);
+        } else {
+            dma4(make_rsrc(scale_base + kb * scale_block, live ? 0x7fffffffu : 0u),
+                 stage + T::kABytes + T::kBBytes + scale_load * 256, scale_off);
+        }
+    };
+    // The last stage's bytes past K (K % 16 != 0: inside a 16-byte piece) become zero.
+    const auto clear_tail = [&](uint32_t slot) {
+        const int piece = p.K % kBlock / 16;
+        for (int r = tid; r < T::BM + T::BN; r += T::kThreads) {
+            auto* at = reinterpret_cast<u32x4*>(lds + slot + r * kBlock + ((piece ^ (r % 8)) << 4));
+            *at = keep_bytes(*at, p.K % 16);
+        }
+        __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
+        barrier_only();
+    };
+
+    const int g = lane / 16;
+    const int r16 = lane % 16;
+    const uint32_t a_rd = static_cast<uint32_t>((wave_m * 16 * RM + r16) * kBlock + ((g ^ (r16 % 8)) << 4));
+    const uint32_t b_rd = static_cast<uint32_t>(T::kABytes + (wave_n * 16 * RN + r16) * kBlock + ((g ^ (r16 % 8)) << 4));
+    const uint32_t sa_rd = static_cast<uint32_t>(T::kABytes + T::kBBytes + (wave_m * 16 * RM + r16) * 4);
+    const uint32_t sb_rd = static_cast<uint32_t>(T::kABytes + T::kBBytes + (T::BM + wave_n * 16 * RN) * 4);
+    // Fragment i of a row block: pieces g and g + 4, whose places differ in one bit.
+    const auto read_fragment = [&](uint32_t slot, uint32_t rd, int i) {
+        return join16(*reinterpret_cast<const u32x4*>(lds + slot + rd + i * 2048),
+                      *reinterpret_cast<const u32x4*>(lds + slot + (rd ^ 64u) + i * 2048));
+    };
+    using ScaleB = std::conditional_t<kByRow, f32x4, float>;
+    constexpr int kScalesB = kByRow ? RN : 1;
+    static_assert(T::kWaves * 16 * OutRow<RN>::kPitch * 4 <= T::kLdsBytes, "the epilogue's rows fit");
+
+    f32x4 acc[RM][RN], t[RN];
+    i32x8 fa[2], fb[RN];
+    float sa[RM];
+    ScaleB sb[kScalesB];
+#pragma unroll
+    for (int j = 0; j < RN; ++j) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        t[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    sa[RM - 1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kScalesB; ++j) sb[j] = ScaleB{};
+
+#pragma unroll
+    for (int s = 0; s < T::kSlots; ++s)
+#pragma unroll
+        for (int d = 0; d < T::kLoads; ++d) load(d, s, s * T::kStageBytes);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 1) * T::kLoads));
+    barrier_only();
+    if (p.K % 16 != 0 && stages == 1) clear_tail(0);
+#pragma unroll
+    for (int j = 0; j < RN; ++j) fb[j] = read_fragment(0, b_rd, j);
+    fa[0] = read_fragment(0, a_rd, 0);
+    fa[1] = read_fragment(0, a_rd, 1);
+
+    uint32_t cur = 0;
+    const auto stage = [&](int kb, auto tail) {
+        const uint32_t nxt = cur + T::kStageBytes == T::kLdsBytes ? 0 : cur + T::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < RM; ++i) {
+            if (i == RM - 2) {
+                // All of this stage's operands are read and the next stage has landed, for every wave past the barrier.
+                __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads));
+                barrier_only();
+                if (tail() && kb + 2 == stages) clear_tail(nxt);
+#pragma unroll
+                for (int d = 0; d < T::kLoads; ++d) load(d, kb + T::kSlots, cur);
+            }
+#pragma unroll
+            for (int j = 0; j < RN; ++j) {
+                // The products of the row before (at the first row: of the stage before, with its scales), RN MFMAs ago,
+                // leave their registers to this row's. The empty asm keeps the compiler from gathering the
+                // multiply-adds behind the stage's MFMAs, where nothing hides them.
+                f32x4& sum = acc[(i + RM - 1) % RM][j];
+                add_scaled(sum, t[j], sa[(i + RM - 1) % RM] * sb[kByRow ? j : 0]);
+                asm volatile("" : "+v"(sum));
+                t[j] = mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i % 2]);
+                if (i == RM - 1) fb[j] = read_fragment(nxt, b_rd, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (i == 0) {
+#pragma unroll
+                for (int r = 0; r < RM; ++r) sa[r] = *reinterpret_cast<const float*>(lds + cur + sa_rd + r * 64);
+#pragma unroll
+                for (int j = 0; j < kScalesB; ++j) {
+                    if constexpr (kByRow) sb[j] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + j * 64 + g * 16);
+                    else sb[j] = *reinterpret_cast<const float*>(lds + cur + sb_rd);
+                }
+            }
+            fa[i % 2] = i + 2 < RM ? read_fragment(cur, a_rd, i + 2) : read_fragment(nxt, a_rd, i + 2 - RM);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        cur = nxt;
+    };
+    const int plain = p.K % 16 == 0 ? stages : stages < 2 ? 0 : stages - 2;
+    int kb = 0;
+    for (; kb < plain; ++kb) stage(kb, std::false_type{});
+    for (; kb < stages; ++kb) stage(kb, std::true_type{});
+#pragma unroll
+    for (int j = 0; j < RN; ++j) add_scaled(acc[RM - 1][j], t[j], sa[RM - 1] * sb[kByRow ? j : 0]);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // the last loads write LDS
+    __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
+    barrier_only();
+    store_tile<RM, RN>(p, acc, m0 + wave_m * 16 * RM, n0 + wave_n * 16 * RN, lane,
+                       reinterpret_cast<float*>(lds + wave * (16 * OutRow<RN>::kPitch * 4)));
+}
+
+}  // namespace feather

@@ -4,6 +4,7 @@
 #include <cstdint>
 
 #include "block_mm_common.h"
+#include "block_mm_tile.h"
 
 namespace feather {
 namespace {
@@ -98,7 +99,22 @@ void launch_stream(const BlockMmParams& p, bool a_e5m2, bool b_e5m2, bool by_row
     else go(std::false_type{}, std::false_type{});
 }
 
-constexpr int64_t kMaxLd = int64_t{4} << 20;   // 256 rows of a tile stay within 31-bit offsets
+template <typename T>
+void launch_tile(const BlockMmParams& p, bool a_e5m2, bool b_e5m2, bool by_row, hipStream_t stream) {
+    const auto grid = static_cast<uint32_t>((p.M + T::BM - 1) / T::BM) * static_cast<uint32_t>((p.N + T::BN - 1) / T::BN);
+    const auto go = [&](auto ae, auto be) {
+        if (by_row) block_tile_kernel<T, ae(), be(), true><<<grid, T::kThreads, 0, stream>>>(p);
+        else block_tile_kernel<T, ae(), be(), false><<<grid, T::kThreads, 0, stream>>>(p);
+    };
+    if (a_e5m2 && b_e5m2) go(std::true_type{}, std::true_type{});
+    else if (a_e5m2) go(std::true_type{}, std::false_type{});
+    else if (b_e5m2) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
+}
+
+// 256 rows of a tile stay within 31-bit offsets, of codes and of scales.
+constexpr int64_t kMaxLd = int64_t{4} << 20;
+constexpr int64_t kMaxScaleStride = int64_t{1} << 20;
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
     return M >= 1 && M <= kMaxSize / 4 && N >= 1 && N <= kMaxSize / 4 && K >= 0 && K <= kMaxLd &&
@@ -125,18 +141,22 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0))
         return false;
     if (K > 0 && (!a || !b || !a_scale || !b_scale || !on_16(a) || !on_16(b) || lda < K || ldb < K || lda % 16 != 0 ||
-                  ldb % 16 != 0 || lda > kMaxLd || ldb > kMaxLd || !aligned_to_type(a_scale, FEATHER_FP32) ||
+                  ldb % 16 != 0 || lda > kMaxLd || ldb > kMaxLd || a_scale_row < 0 || a_scale_row > kMaxScaleStride ||
+                  b_scale_row < 0 || b_scale_row > kMaxScaleStride || a_scale_block < 0 || b_scale_block < 0 || !aligned_to_type(a_scale, FEATHER_FP32) ||
                   !aligned_to_type(b_scale, FEATHER_FP32)))
         return false;
     if (!c || ldc < N || ldc > kMaxSize || !aligned_to_type(c, out_type) || (bias && !aligned_to_type(bias, out_type)))
         return false;
     const int bytes = type_bytes(out_type);
     const bool store4 = (reinterpret_cast<uintptr_t>(c) & (4 * bytes - 1)) == 0 && ldc % 4 == 0;
+    const bool store8 = rows_on_16(c, ldc, out_type) && N % 8 == 0 && on_16(bias);
     const BlockMmParams p{a, b, a_scale, b_scale, lda, ldb, a_scale_row, a_scale_block, b_scale_row, b_scale_block,
                           static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), 1, bias, c, ldc,
-                          out_type, store4, nullptr, nullptr};
+                          out_type, store4, store8, nullptr, nullptr};
     if (M <= 16) launch_stream<1, 1>(p, a_e5m2, b_e5m2, b_by_row, stream);
     else if (M <= 32) launch_stream<2, 1>(p, a_e5m2, b_e5m2, b_by_row, stream);
-    else launch_stream<4, 2>(p, a_e5m2, b_e5m2, b_by_row, stream);
+    else if (M <= 64) launch_stream<4, 2>(p, a_e5m2, b_e5m2, b_by_row, stream);
+    else if (M <= 512) launch_tile<BlockTile<128, 128, 2, 2, 2>>(p, a_e5m2, b_e5m2, b_by_row, stream);
+    else launch_tile<BlockTile<256, 256, 2, 4, 2>>(p, a_e5m2, b_e5m2, b_by_row, stream);
     return true;
 }

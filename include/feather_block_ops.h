@@ -40,10 +40,11 @@ enum { FEATHER_BF16 = 0, FEATHER_FP16 = 1, FEATHER_FP32 = 2 };
  * instructions align 8 neighbouring products to the largest of them and cut each off 13 bits below it before they are added
  * in fp32, which costs about 1.5e-5 of a result (2-norm, random operands); whole numbers within those bits are exact.
  *
- *   a, b      [M, K] and [N, K] fp8 codes, each of its own format; row strides lda and ldb, multiples of 16; 16-byte
- *             aligned. Bytes between K and the next row are not used (up to 3 of them are read where K % 4 != 0).
+ *   a, b      [M, K] and [N, K] fp8 codes, each of its own format; row strides lda and ldb, multiples of 16 up to 2^22;
+ *             16-byte aligned. Bytes between K and the next row are not used (up to 3 of them are read where K % 4 != 0).
  *   a_scale   fp32 [M, ceil(K / 128)]: element (m, k) at m * a_scale_row + k * a_scale_block. Block-major (a_scale_row = 1,
- *             what the functions below write) is the layout that reads fastest.
+ *             what the functions below write) is the layout that reads fastest. Strides from row to row (for b: from
+ *             square to square) are 0 .. 2^20, those from block to block not negative.
  *   b_scale   fp32, the same for b: one per 128 x 128 block (b_by_row = false: element (n / 128, k)) or per row of b
  *             (b_by_row = true: element (n, k)).
  *   bias      N values of out_type, or null.

@@ -152,7 +152,7 @@ Tensor block_scaled_mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, 
     }
     Tensor c = new_matrix(a, M, N, torch_dtype(type));
     if (M == 0 || N == 0) return c;
-    const int64_t need = feather_block_scaled_mm_workspace_bytes(M, N, K, by_row);
+    const int64_t need = feather_block_scaled_mm_workspace_bytes(M, N, K);
     STD_TORCH_CHECK(need >= 0, "block_scaled_mm: sizes are out of range");
     if (need > 0) {
         STD_TORCH_CHECK(workspace.has_value() && workspace->is_cuda() && workspace->get_device_index() == device_index &&

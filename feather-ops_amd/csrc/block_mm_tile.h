@@ -6,7 +6,7 @@
 
 namespace feather {
 
-template <int BM_, int BN_, int WM_, int WN_, int kSlots_>
+template <int BM_, int BN_, int WM_, int WN_, int kSlots_, int kSpread = 5>
 struct BlockTile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kSlots = kSlots_;
     static constexpr int kWaves = WM * WN;
@@ -20,11 +20,29 @@ struct BlockTile {
     static constexpr int kLdsBytes = kSlots * kStageBytes;
     static constexpr int kALoads = kABytes / 1024 / kWaves;
     static constexpr int kBLoads = kBBytes / 1024 / kWaves;
-    static constexpr int kScaleLoads = (BM + BN) / 64;  // of the workgroup, one a wave (some twice)
-    static constexpr int kLoads = kALoads + kBLoads + 1;
+    static constexpr int kScaleGroups = (BM + BN) / 64; // of 64 scales
+    static constexpr int kScaleLoads = (kScaleGroups + kWaves - 1) / kWaves;   // of a wave (some groups twice)
+    static constexpr int kLoads = kALoads + kBLoads + kScaleLoads;
+    // A stage's MFMAs go by pairs of rows, the two rows of each column one after the other, to and fro, so that one operand
+    // changes from each to the next: MFMA n is row(n), col(n). Its product is added kLag MFMAs later.
+    static constexpr int kMfmas = RM * RN;
+    static constexpr int kPair = 2 * RN;
+    static constexpr int kLag = 4;
+    static constexpr int row(int n) { return n / kPair * 2 + (n + n / 2) % 2; }
+    static constexpr int col(int n) { return n % kPair / 2; }
+    // The barrier that hands a slot over comes before the last pair. The refill's loads follow it, spread over kSpread / 8 of
+    // a stage's MFMAs: load d after MFMA at(d), from kMfmas on in the next stage.
+    static constexpr int kBarrier = kMfmas - kPair;
+    static constexpr int at(int d) { return kBarrier + 1 + d * (kMfmas * kSpread / 8) / kLoads; }
+    static constexpr int kEarly = [] {
+        int n = 0;
+        while (n < kLoads && at(n) < kMfmas) ++n;
+        return n;
+    }();
+    static_assert(at(kLoads - 1) - kMfmas < kBarrier, "a stage's loads are issued before the next barrier");
+    static_assert(kMfmas >= 2 * kPair && kPair >= kLag, "two pairs of rows at least");
     static_assert(kABytes % (1024 * kWaves) == 0 && kBBytes % (1024 * kWaves) == 0, "whole loads");
-    static_assert(kScaleLoads <= kWaves, "one scale load a wave");
-    static_assert(RM % 2 == 0 && RM >= 2, "fragments of a go through two registers");
+    static_assert(RM % 4 == 0, "pairs of rows go through two sets of registers");
     static_assert(kBlock % (BN / WN) == 0, "a wave's columns have one square scale");
     static_assert((kSlots - 1) * kLoads < 64, "vmcnt range");
 };
@@ -115,11 +133,18 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     const int wave_n = wave % T::WN;
     const int tiles_m = (p.M + T::BM - 1) / T::BM;
     const int tiles_n = (p.N + T::BN - 1) / T::BN;
+    // Workgroup -> (K range, tile), ranges of one tile a whole round of tiles apart.
+    const int tiles = tiles_m * tiles_n;
+    const int split = p.splits > 1 ? static_cast<int>(blockIdx.x) / tiles : 0;
+    const int tile = static_cast<int>(blockIdx.x) - split * tiles;
     int tm, tn;
-    tile_of_block(static_cast<int>(blockIdx.x), tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+    tile_of_block(tile, tiles, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * T::BM;
     const int n0 = tn * T::BN;
-    const int stages = (p.K + kBlock - 1) / kBlock;
+    const int blocks = (p.K + kBlock - 1) / kBlock;
+    const int first = static_cast<int>(static_cast<int64_t>(split) * blocks / p.splits);
+    const int stages = static_cast<int>(static_cast<int64_t>(split + 1) * blocks / p.splits) - first;
+    const bool tail = p.K % 16 != 0 && first + stages == blocks;   // the last block ends inside a 16-byte piece
 
     // Direct loads: each fills 8 rows of 8 pieces; lane l's place is piece l % 8 of row l / 8, which holds the row's piece
     // (l % 8) ^ (row % 8), so that 8 rows' reads of one piece fall on 8 different places.
@@ -131,25 +156,29 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     const uint32_t b_off = static_cast<uint32_t>(wave * 8 + lane / 8) * static_cast<uint32_t>(p.ldb) + piece_at;
     const uint32_t a_step = 8u * T::kWaves * static_cast<uint32_t>(p.lda);
     const uint32_t b_step = 8u * T::kWaves * static_cast<uint32_t>(p.ldb);
-    // This wave's 64 scales of a stage.
-    const int scale_load = wave % T::kScaleLoads;
-    const bool scale_a = scale_load < T::BM / 64;
-    const int scale_row = scale_load * 64 + lane - (scale_a ? 0 : T::BM);
-    uint32_t scale_off;
-    {
-        const int row = scale_a ? m0 + scale_row : n0 + scale_row;
-        const int64_t first = scale_a ? m0 : kByRow ? n0 : n0 / kBlock;
-        const int64_t index = scale_a || kByRow ? row : row / kBlock;
-        const bool there = row < (scale_a ? p.M : p.N);
-        scale_off = there ? static_cast<uint32_t>((index - first) * (scale_a ? p.as_row : p.bs_row)) * 4u : kOob;
+    // This wave's groups of 64 scales of a stage.
+    uint32_t scale_off[T::kScaleLoads];
+    const float* scale_base[T::kScaleLoads];
+    int64_t scale_step[T::kScaleLoads];
+    int scale_group[T::kScaleLoads];
+#pragma unroll
+    for (int s = 0; s < T::kScaleLoads; ++s) {
+        const int group = (wave + s * T::kWaves) % T::kScaleGroups;
+        const bool of_a = group < T::BM / 64;
+        const int row = (of_a ? m0 : n0 - T::BM) + group * 64 + lane;
+        const int64_t base = of_a ? m0 : kByRow ? n0 : n0 / kBlock;
+        const int64_t index = of_a || kByRow ? row : row / kBlock;
+        const int64_t pitch = of_a ? p.as_row : p.bs_row;
+        scale_group[s] = group;
+        scale_off[s] = row < (of_a ? p.M : p.N) ? static_cast<uint32_t>((index - base) * pitch) * 4u : kOob;
+        scale_base[s] = (of_a ? p.a_scale : p.b_scale) + base * pitch;
+        scale_step[s] = of_a ? p.as_block : p.bs_block;
     }
-    const float* scale_base = scale_a ? p.a_scale + m0 * p.as_row
-                                      : p.b_scale + (kByRow ? static_cast<int64_t>(n0) : n0 / kBlock) * p.bs_row;
-    const int64_t scale_block = scale_a ? p.as_block : p.bs_block;
 
-    // Load d of stage kb (past the last: nothing, into a slot nobody reads).
-    const auto load = [&](int d, int kb, uint32_t slot) {
-        const bool live = kb < stages;
+    // Load d of stage `at` (past the last: nothing, into a slot nobody reads).
+    const auto load = [&](int d, int at, uint32_t slot) {
+        const bool live = at < stages;
+        const int kb = first + at;
         uint8_t* const stage = lds + slot;
         if (d < T::kALoads + T::kBLoads) {
             const bool is_a = d < T::kALoads;
@@ -159,8 +188,9 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
             dma16(live ? (is_a ? a_rsrc : b_rsrc) : null_rsrc, stage + (is_a ? 0 : T::kABytes) + (wave + i * T::kWaves) * 1024,
                   there ? off : kOob, static_cast<uint32_t>(kb) * kBlock);
         } else {
-            dma4(make_rsrc(scale_base + kb * scale_block, live ? 0x7fffffffu : 0u),
-                 stage + T::kABytes + T::kBBytes + scale_load * 256, scale_off);
+            const int i = d - T::kALoads - T::kBLoads;
+            dma4(make_rsrc(scale_base[i] + kb * scale_step[i], live ? 0x7fffffffu : 0u),
+                 stage + T::kABytes + T::kBBytes + scale_group[i] * 256, scale_off[i]);
         }
     };
     // The last stage's bytes past K (K % 16 != 0: inside a 16-byte piece) become zero.
@@ -189,81 +219,110 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     constexpr int kScalesB = kByRow ? RN : 1;
     static_assert(T::kWaves * 16 * OutRow<RN>::kPitch * 4 <= T::kLdsBytes, "the epilogue's rows fit");
 
-    f32x4 acc[RM][RN], t[RN];
-    i32x8 fa[2], fb[RN];
+    f32x4 acc[RM][RN], t[T::kLag];
+    i32x8 fa[2][2], fb[RN];     // two pairs of rows of a
     float sa[RM];
     ScaleB sb[kScalesB];
 #pragma unroll
-    for (int j = 0; j < RN; ++j) {
+    for (int j = 0; j < RN; ++j)
 #pragma unroll
         for (int i = 0; i < RM; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        t[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    sa[RM - 1] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < T::kLag; ++n) t[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < RM; ++i) sa[i] = 0.0f;
 #pragma unroll
     for (int j = 0; j < kScalesB; ++j) sb[j] = ScaleB{};
 
 #pragma unroll
     for (int s = 0; s < T::kSlots; ++s)
 #pragma unroll
-        for (int d = 0; d < T::kLoads; ++d) load(d, s, s * T::kStageBytes);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 1) * T::kLoads));
+        for (int d = 0; d < (s + 1 < T::kSlots ? T::kLoads : T::kEarly); ++d) load(d, s, s * T::kStageBytes);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads + T::kEarly));
     barrier_only();
-    if (p.K % 16 != 0 && stages == 1) clear_tail(0);
+    if (tail && stages == 1) clear_tail(0);
 #pragma unroll
     for (int j = 0; j < RN; ++j) fb[j] = read_fragment(0, b_rd, j);
-    fa[0] = read_fragment(0, a_rd, 0);
-    fa[1] = read_fragment(0, a_rd, 1);
+    fa[0][0] = read_fragment(0, a_rd, 0);
+    fa[0][1] = read_fragment(0, a_rd, 1);
 
+    float sa_next[2], sb_next = 0.0f;
+    const auto read_first_scales = [&](uint32_t slot) {
+        sa_next[0] = *reinterpret_cast<const float*>(lds + slot + sa_rd);
+        sa_next[1] = *reinterpret_cast<const float*>(lds + slot + sa_rd + 64);
+        if constexpr (!kByRow) sb_next = *reinterpret_cast<const float*>(lds + slot + sb_rd);
+    };
+    read_first_scales(0);
     uint32_t cur = 0;
-    const auto stage = [&](int kb, auto tail) {
+    uint32_t prv = (T::kSlots - 1) * T::kStageBytes;
+    const auto stage = [&](int kb, auto may_end) {
         const uint32_t nxt = cur + T::kStageBytes == T::kLdsBytes ? 0 : cur + T::kStageBytes;
 #pragma unroll
-        for (int i = 0; i < RM; ++i) {
-            if (i == RM - 2) {
+        for (int n = 0; n < T::kMfmas; ++n) {
+            const int i = T::row(n), j = T::col(n);
+            {
+                // The product of kLag MFMAs ago (at first: of the stage before, with its scales) leaves its registers to this
+                // one's. The empty asm keeps the compiler from gathering the multiply-adds behind the stage's MFMAs, where
+                // nothing hides them.
+                const int before = (n + T::kMfmas - T::kLag) % T::kMfmas;
+                const int bi = T::row(before), bj = T::col(before);
+                f32x4& sum = acc[bi][bj];
+                add_scaled(sum, t[n % T::kLag], sa[bi] * sb[kByRow ? bj : 0]);
+                asm volatile("" : "+v"(sum));
+            }
+            if (n == T::kBarrier) {
                 // All of this stage's operands are read and the next stage has landed, for every wave past the barrier.
                 __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads));
                 barrier_only();
-                if (tail() && kb + 2 == stages) clear_tail(nxt);
-#pragma unroll
-                for (int d = 0; d < T::kLoads; ++d) load(d, kb + T::kSlots, cur);
+                if (may_end() && kb + 2 == stages) clear_tail(nxt);
             }
-#pragma unroll
-            for (int j = 0; j < RN; ++j) {
-                // The products of the row before (at the first row: of the stage before, with its scales), RN MFMAs ago,
-                // leave their registers to this row's. The empty asm keeps the compiler from gathering the
-                // multiply-adds behind the stage's MFMAs, where nothing hides them.
-                f32x4& sum = acc[(i + RM - 1) % RM][j];
-                add_scaled(sum, t[j], sa[(i + RM - 1) % RM] * sb[kByRow ? j : 0]);
-                asm volatile("" : "+v"(sum));
-                t[j] = mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i % 2]);
-                if (i == RM - 1) fb[j] = read_fragment(nxt, b_rd, j);
-                __builtin_amdgcn_sched_barrier(0);
+            t[n % T::kLag] = mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i / 2 % 2][i % 2]);
+            // Operands: a pair of rows during the pair before, a column of b after its last use.
+            const int q = n % T::kPair;
+            const int next_row = n / T::kPair * 2 + 2;
+            if (q < 2) {
+                fa[next_row / 2 % 2][q] = next_row < RM ? read_fragment(cur, a_rd, next_row + q) : read_fragment(nxt, a_rd, q);
             }
-            if (i == 0) {
+            if (n >= T::kBarrier && n % 2 == 1) fb[j] = read_fragment(nxt, b_rd, j);
+            // Scales: those of the first pair with the operands, the others once the stage before is done with them.
+            if (n == T::kBarrier + 2) read_first_scales(nxt);
+            if (n == T::kLag - 1) {
+                sa[0] = sa_next[0];
+                sa[1] = sa_next[1];
 #pragma unroll
-                for (int r = 0; r < RM; ++r) sa[r] = *reinterpret_cast<const float*>(lds + cur + sa_rd + r * 64);
+                for (int r = 2; r < RM; ++r) sa[r] = *reinterpret_cast<const float*>(lds + cur + sa_rd + r * 64);
+                if constexpr (kByRow) {
 #pragma unroll
-                for (int j = 0; j < kScalesB; ++j) {
-                    if constexpr (kByRow) sb[j] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + j * 64 + g * 16);
-                    else sb[j] = *reinterpret_cast<const float*>(lds + cur + sb_rd);
+                    for (int c = 0; c < RN; ++c) sb[c] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + c * 64 + g * 16);
+                } else {
+                    sb[0] = sb_next;
                 }
             }
-            fa[i % 2] = i + 2 < RM ? read_fragment(cur, a_rd, i + 2) : read_fragment(nxt, a_rd, i + 2 - RM);
+#pragma unroll
+            for (int d = 0; d < T::kLoads; ++d) {
+                if (T::at(d) == n) load(d, kb + T::kSlots, cur);
+                if (T::at(d) - T::kMfmas == n) load(d, kb + T::kSlots - 1, prv);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
+        prv = cur;
         cur = nxt;
     };
-    const int plain = p.K % 16 == 0 ? stages : stages < 2 ? 0 : stages - 2;
+    const int plain = !tail ? stages : stages < 2 ? 0 : stages - 2;
     int kb = 0;
     for (; kb < plain; ++kb) stage(kb, std::false_type{});
     for (; kb < stages; ++kb) stage(kb, std::true_type{});
 #pragma unroll
-    for (int j = 0; j < RN; ++j) add_scaled(acc[RM - 1][j], t[j], sa[RM - 1] * sb[kByRow ? j : 0]);
+    for (int n = 0; n < T::kLag; ++n) {
+        constexpr int kFirst = T::kMfmas - T::kLag;
+        const int i = T::row(kFirst + n), j = T::col(kFirst + n);
+        add_scaled(acc[i][j], t[(kFirst + n) % T::kLag], sa[i] * sb[kByRow ? j : 0]);
+    }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // the last loads write LDS
     __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
     barrier_only();
+    if (p.splits > 1 && !join_split<T::kWaves, RM, RN>(p, acc, tile, split, wave, lane)) return;
     store_tile<RM, RN>(p, acc, m0 + wave_m * 16 * RM, n0 + wave_n * 16 * RN, lane,
                        reinterpret_cast<float*>(lds + wave * (16 * OutRow<RN>::kPitch * 4)));
 }

@@ -1,115 +1,106 @@
-// The block-scaled fp8 product's host side and its streaming kernel (include/feather_block_ops.h, block_mm_common.h).
+// The block-scaled fp8 product's host side (include/feather_block_ops.h): the choice of a kernel, the contract's checks and
+// the C ABI.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "block_mm_common.h"
-#include "block_mm_tile.h"
+#include "block_mm_launch.h"
 
 namespace feather {
 namespace {
 
-constexpr int kStreamWaves = 8;
+constexpr int64_t kCUs = 256;
+constexpr int64_t kCtrBytes = 64 * 1024;                // the workspace's arrival counters, as the other split launches'
+constexpr int64_t kMaxCounters = kCtrBytes / 4;
+constexpr int64_t kMaxPartBytes = kMaxSize - kCtrBytes;
 
-// Streaming kernel: a workgroup owns 16 RM x 16 RN outputs and its 8 waves take every eighth block of K each, reading both
-// operands from memory straight into registers; their fp32 sums meet in LDS, added in wave order.
-template <bool kAE5M2, bool kBE5M2, bool kByRow, int RM, int RN>
-__global__ __launch_bounds__(kStreamWaves * 64) void block_stream_kernel(const BlockMmParams p) {
-    __shared__ f32x4 join[kStreamWaves][RM * RN][64];
-    const int lane = threadIdx.x % 64;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int tiles_n = (p.N + 16 * RN - 1) / (16 * RN);
-    const int m0 = static_cast<int>(blockIdx.x) / tiles_n * 16 * RM;
-    const int n0 = static_cast<int>(blockIdx.x) % tiles_n * 16 * RN;
-    const int r16 = lane % 16;
-    const int g = lane / 16;
-    const rsrc_t a_rsrc = rows_rsrc(p.a, p.lda, m0, p.M, 16 * RM, p.K);
-    const rsrc_t b_rsrc = rows_rsrc(p.b, p.ldb, n0, p.N, 16 * RN, p.K);
-    const int blocks = (p.K + kBlock - 1) / kBlock;
+int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
 
-    f32x4 acc[RM][RN];
-#pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < RN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+bool splits_fit(const BlockMmPlan& plan) {
+    return plan.tiles * plan.slots <= kMaxCounters && plan.tiles * plan.splits * plan.tile_bytes <= kMaxPartBytes;
+}
 
-    for (int kb = wave; kb < blocks; kb += kStreamWaves) {
-        i32x8 fa[RM], fb[RN];
-        const auto fetch = [&](rsrc_t r, int row, int64_t ld) {
-            u32x4 half[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = kb * kBlock + h * 64 + g * 16;
-                half[h] = buf_load16(r, at < p.K ? static_cast<uint32_t>(row) * static_cast<uint32_t>(ld) + at : kOob);
-                if (p.K % 16 != 0) half[h] = keep_bytes(half[h], p.K - at);
+BlockMmPlan stream_plan(BlockMmKernel kernel, int rm, int rn, int64_t M, int64_t N, int splits) {
+    BlockMmPlan plan{kernel, splits, ceil_div(M, 16 * rm) * ceil_div(N, 16 * rn), rm * rn, int64_t{1024} * rm * rn};
+    if (!splits_fit(plan)) plan.splits = 1;
+    return plan;
+}
+
+// At most 64 rows. Measured (us, e4m3fn, weights from HBM; RM x RN is a workgroup's fragments, "/s" its K splits):
+//   RN. A workgroup reads all rows of a beside its own rows of b, from L2: with 9 rows and more, 16 columns a workgroup read
+//     as much of a as of b. 16 x 14336 x 4096: 1 x 4 14.6, 1 x 1 16.6; 16 x 4096 x 14336: 1 x 4/4 15.2, 1 x 1 16.5; 24 x
+//     4096 x 14336: 2 x 4/4 16.4, 2 x 1 20.4. With one row, 1 x 1 is faster: 4096 x 14336 12.4 against 1 x 4/4 14.3; 8192 x
+//     8192 14.1 against 15.7. Few columns have too few workgroups: 16 x 1024 x 4096 1 x 1/2 5.7, 1 x 4 over 7.
+//   Waves. 16 take 32 blocks in flight at once, which pays where that is half of K to all of it: 1 x 4096 x 4096 5.8 against
+//     6.3, 1 x 14336 x 4096 14.1 against 15.8; 1 x 4096 x 14336 13.8 against 12.4, 1 x 12288 x 2048 7.3 against 6.5.
+//   Splits. Up to 256 workgroups of at least 16 blocks (8 with 17 rows and more): 1 x 1024 x 16384 /4 7.8, /2 9.0, /1 over
+//     10; 1 x 1024 x 4096 /1 4.7, /2 5.1; 32 x 1024 x 4096 /4 6.4, /2 6.6.
+BlockMmPlan few_rows_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t blocks = ceil_div(K, kBlock);
+    const auto splits = [&](int64_t tiles, int64_t target, int64_t least) {
+        int s = 1;
+        while (s < 4 && tiles * s * 2 <= target && blocks / (s * 2) >= least) s *= 2;
+        return s;
+    };
+    if (M > 32) return stream_plan(kStream4x1, 4, 1, M, N, splits(ceil_div(N, 16), 256, 8));
+    const bool wide = M > 8 && (N >= 8192 || (N >= 4096 && blocks >= 64));
+    if (wide) {
+        const int64_t tiles = ceil_div(N, 64);
+        const int s = tiles >= 192 ? 1 : splits(tiles, 512, 16);
+        return M > 16 ? stream_plan(kStream2x4, 2, 4, M, N, s) : stream_plan(kStream1x4, 1, 4, M, N, s);
+    }
+    const int64_t tiles = ceil_div(N, 16);
+    if (M > 16) return stream_plan(kStream2x1, 2, 1, M, N, splits(tiles, 256, 8));
+    const BlockMmKernel kernel = blocks >= 32 && blocks <= 64 && tiles >= 256 ? kStream1x1Wide : kStream1x1;
+    return stream_plan(kernel, 1, 1, M, N, splits(tiles, 256, 16));
+}
+
+// A tile of the ring kernel: workgroups that share a CU's LDS, and microseconds fitted to 3300 timings of 115 shapes (33 to
+// 12288 rows, N and K 256 to 16384): a workgroup's start and end, and a stage with the CU full of workgroups and with one. The
+// tile and splits with the least estimate took at most 1.10 of the best pair's time on any of them, 1.009 in geometric mean.
+struct TileCost {
+    BlockMmKernel kernel;
+    int bm, bn, waves, per_cu;
+    float fixed, full, alone;
+};
+constexpr TileCost kTiles[] = {
+    {kTile64x64, 64, 64, 2, 4, 2.60f, 1.058f, 0.350f},     {kTile64x128, 64, 128, 4, 2, 1.37f, 0.944f, 0.659f},
+    {kTile128x128, 128, 128, 8, 1, 1.69f, 0.662f, 0.662f}, {kTile256x128, 256, 128, 8, 1, 5.10f, 0.905f, 0.905f},
+    {kTile128x256, 128, 256, 8, 1, 2.55f, 1.103f, 1.103f}, {kTile256x256, 256, 256, 8, 1, 5.36f, 1.695f, 1.695f},
+};
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+
+BlockMmPlan tile_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t blocks = std::max<int64_t>(1, ceil_div(K, kBlock));
+    const float memory = static_cast<float>(N + M) * static_cast<float>(K) / 5.0e6f;   // us at 5 TB/s
+    BlockMmPlan best{};
+    float least = 0.0f;
+    for (const TileCost& t : kTiles) {
+        const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
+        for (const int splits : kSplits) {
+            const BlockMmPlan plan{t.kernel, splits, tiles, t.waves, int64_t{4} * t.bm * t.bn};
+            if (splits > 1 && (splits > blocks || tiles * splits > 6 * kCUs || !splits_fit(plan))) break;
+            const auto stages = static_cast<float>(ceil_div(blocks, splits));
+            const int64_t groups = tiles * splits;
+            const int64_t rounds = groups / (kCUs * t.per_cu);
+            const int64_t rest = groups - rounds * kCUs * t.per_cu;
+            float cost = static_cast<float>(rounds) * (stages * t.full + t.fixed);
+            if (rest > 0) {
+                const float more = t.per_cu > 1 ? static_cast<float>(ceil_div(rest, kCUs) - 1) / (t.per_cu - 1) : 0.0f;
+                cost += stages * (t.alone + (t.full - t.alone) * more) + t.fixed;
             }
-            return join16(half[0], half[1]);
-        };
-        float sa[RM];
-#pragma unroll
-        for (int i = 0; i < RM; ++i) {
-            fa[i] = fetch(a_rsrc, 16 * i + r16, p.lda);
-            const int m = m0 + 16 * i + r16;
-            sa[i] = m < p.M ? p.a_scale[m * p.as_row + kb * p.as_block] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < RN; ++j) {
-            fb[j] = fetch(b_rsrc, 16 * j + r16, p.ldb);
-            const int n = n0 + 16 * j;
-            if constexpr (kByRow) {
-                f32x4 sb;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int col = n + 4 * g + e;
-                    sb[e] = col < p.N ? p.b_scale[col * p.bs_row + kb * p.bs_block] : 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < RM; ++i) add_scaled(acc[i][j], mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i]), sa[i] * sb);
-            } else {
-                const float sb = n < p.N ? p.b_scale[n / kBlock * p.bs_row + kb * p.bs_block] : 0.0f;
-#pragma unroll
-                for (int i = 0; i < RM; ++i) add_scaled(acc[i][j], mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i]), sa[i] * sb);
+            cost = std::max(cost, memory);
+            // the last of a tile's workgroups reads all of its sums back
+            if (splits > 1) cost += 1.56f + 1.14f / 65536.0f * static_cast<float>(splits * plan.tile_bytes);
+            if (least == 0.0f || cost < least) {
+                least = cost;
+                best = plan;
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < RN; ++j) join[wave][i * RN + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int f = wave; f < RM * RN; f += kStreamWaves) {
-        f32x4 sum = join[0][f][lane];
-#pragma unroll
-        for (int w = 1; w < kStreamWaves; ++w) sum += join[w][f][lane];
-        store_out(p, m0 + f / RN * 16 + r16, n0 + f % RN * 16 + 4 * g, sum);
-    }
-}
-
-template <int RM, int RN>
-void launch_stream(const BlockMmParams& p, bool a_e5m2, bool b_e5m2, bool by_row, hipStream_t stream) {
-    const auto grid = static_cast<uint32_t>((p.M + 16 * RM - 1) / (16 * RM)) *
-                      static_cast<uint32_t>((p.N + 16 * RN - 1) / (16 * RN));
-    const auto go = [&](auto ae, auto be) {
-        if (by_row) block_stream_kernel<ae(), be(), true, RM, RN><<<grid, kStreamWaves * 64, 0, stream>>>(p);
-        else block_stream_kernel<ae(), be(), false, RM, RN><<<grid, kStreamWaves * 64, 0, stream>>>(p);
-    };
-    if (a_e5m2 && b_e5m2) go(std::true_type{}, std::true_type{});
-    else if (a_e5m2) go(std::true_type{}, std::false_type{});
-    else if (b_e5m2) go(std::false_type{}, std::true_type{});
-    else go(std::false_type{}, std::false_type{});
-}
-
-template <typename T>
-void launch_tile(const BlockMmParams& p, bool a_e5m2, bool b_e5m2, bool by_row, hipStream_t stream) {
-    const auto grid = static_cast<uint32_t>((p.M + T::BM - 1) / T::BM) * static_cast<uint32_t>((p.N + T::BN - 1) / T::BN);
-    const auto go = [&](auto ae, auto be) {
-        if (by_row) block_tile_kernel<T, ae(), be(), true><<<grid, T::kThreads, 0, stream>>>(p);
-        else block_tile_kernel<T, ae(), be(), false><<<grid, T::kThreads, 0, stream>>>(p);
-    };
-    if (a_e5m2 && b_e5m2) go(std::true_type{}, std::true_type{});
-    else if (a_e5m2) go(std::true_type{}, std::false_type{});
-    else if (b_e5m2) go(std::false_type{}, std::true_type{});
-    else go(std::false_type{}, std::false_type{});
+    return best;
 }
 
 // 256 rows of a tile stay within 31-bit offsets, of codes and of scales.
@@ -118,16 +109,25 @@ constexpr int64_t kMaxScaleStride = int64_t{1} << 20;
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
     return M >= 1 && M <= kMaxSize / 4 && N >= 1 && N <= kMaxSize / 4 && K >= 0 && K <= kMaxLd &&
-           ((M + 15) / 16) * ((N + 15) / 16) <= kMaxSize;
+           ceil_div(M, 64) * ceil_div(N, 16) <= kMaxSize / 16;
 }
 
 }  // namespace
+
+BlockMmPlan block_mm_plan(int64_t M, int64_t N, int64_t K) {
+    // 33 to 64 rows stream only beside few columns: 64 x 2048 x 2048 6.5 us against 64 x 64 tiles' 7.7 and more, 64 x 4096 x
+    // 4096 over 11 against 10.8.
+    return M <= 32 || (M <= 64 && N <= 2048) ? few_rows_plan(M, N, K) : tile_plan(M, N, K);
+}
+
 }  // namespace feather
 
 using namespace feather;
 
-extern "C" int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, bool) {
-    return sizes_ok(M, N, K) ? 0 : -1;
+extern "C" int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (!sizes_ok(M, N, K)) return -1;
+    const BlockMmPlan plan = block_mm_plan(M, N, K);
+    return plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
 }
 
 extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5m2, const float* a_scale,
@@ -137,13 +137,14 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
                                         int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                                         hipStream_t stream) {
     if (!sizes_ok(M, N, K) || !type_ok(out_type)) return false;
-    const int64_t need = feather_block_scaled_mm_workspace_bytes(M, N, K, b_by_row);
+    const BlockMmPlan plan = block_mm_plan(M, N, K);
+    const int64_t need = plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0))
         return false;
     if (K > 0 && (!a || !b || !a_scale || !b_scale || !on_16(a) || !on_16(b) || lda < K || ldb < K || lda % 16 != 0 ||
                   ldb % 16 != 0 || lda > kMaxLd || ldb > kMaxLd || a_scale_row < 0 || a_scale_row > kMaxScaleStride ||
-                  b_scale_row < 0 || b_scale_row > kMaxScaleStride || a_scale_block < 0 || b_scale_block < 0 || !aligned_to_type(a_scale, FEATHER_FP32) ||
-                  !aligned_to_type(b_scale, FEATHER_FP32)))
+                  b_scale_row < 0 || b_scale_row > kMaxScaleStride || a_scale_block < 0 || b_scale_block < 0 ||
+                  !aligned_to_type(a_scale, FEATHER_FP32) || !aligned_to_type(b_scale, FEATHER_FP32)))
         return false;
     if (!c || ldc < N || ldc > kMaxSize || !aligned_to_type(c, out_type) || (bias && !aligned_to_type(bias, out_type)))
         return false;
@@ -151,12 +152,10 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
     const bool store4 = (reinterpret_cast<uintptr_t>(c) & (4 * bytes - 1)) == 0 && ldc % 4 == 0;
     const bool store8 = rows_on_16(c, ldc, out_type) && N % 8 == 0 && on_16(bias);
     const BlockMmParams p{a, b, a_scale, b_scale, lda, ldb, a_scale_row, a_scale_block, b_scale_row, b_scale_block,
-                          static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), 1, bias, c, ldc,
-                          out_type, store4, store8, nullptr, nullptr};
-    if (M <= 16) launch_stream<1, 1>(p, a_e5m2, b_e5m2, b_by_row, stream);
-    else if (M <= 32) launch_stream<2, 1>(p, a_e5m2, b_e5m2, b_by_row, stream);
-    else if (M <= 64) launch_stream<4, 2>(p, a_e5m2, b_e5m2, b_by_row, stream);
-    else if (M <= 512) launch_tile<BlockTile<128, 128, 2, 2, 2>>(p, a_e5m2, b_e5m2, b_by_row, stream);
-    else launch_tile<BlockTile<256, 256, 2, 4, 2>>(p, a_e5m2, b_e5m2, b_by_row, stream);
+                          static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), plan.splits, bias, c,
+                          ldc, out_type, store4, store8, static_cast<uint32_t*>(workspace),
+                          need > 0 ? static_cast<uint8_t*>(workspace) + kCtrBytes : nullptr};
+    (a_e5m2 ? (b_e5m2 ? block_mm_launch_11 : block_mm_launch_10) : (b_e5m2 ? block_mm_launch_01 : block_mm_launch_00))(
+        p, plan, b_by_row, stream);
     return true;
 }

@@ -47,7 +47,7 @@ def c_library() -> ctypes.CDLL:
         lib.feather_linear_backward_split_bytes.argtypes = ([ctypes.c_int64] * 3 + [ctypes.c_bool] + [ctypes.c_int] * 5 +
                                                             [ctypes.c_bool, ctypes.c_int])
         lib.feather_block_scaled_mm_workspace_bytes.restype = ctypes.c_int64
-        lib.feather_block_scaled_mm_workspace_bytes.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_bool]
+        lib.feather_block_scaled_mm_workspace_bytes.argtypes = [ctypes.c_int64] * 3
         _c_library = lib
     return _c_library
 

@@ -81,8 +81,8 @@ def _square_shape(shape: torch.Size) -> tuple[int, int]:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(M: int, N: int, K: int, by_row: bool) -> int:
-    return max(0, _lib.c_library().feather_block_scaled_mm_workspace_bytes(M, N, K, by_row))
+def _workspace_bytes(M: int, N: int, K: int) -> int:
+    return max(0, _lib.c_library().feather_block_scaled_mm_workspace_bytes(M, N, K))
 
 
 def _codes(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -109,7 +109,7 @@ def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_s
     a, b = _codes(a, "a"), _codes(b, "b")
     m, k = a.shape
     n = b.shape[0]
-    need = _workspace_bytes(m, n, k, b_scale.shape[:1] != (-(-n // BLOCK),))
+    need = _workspace_bytes(m, n, k)
     return torch.ops.feather_ops.block_scaled_mm.default(a, a_scale, b, b_scale, bias, out_type,
                                                          _workspace_for(a, need) if need else None)
 

@@ -49,7 +49,7 @@ enum { FEATHER_BF16 = 0, FEATHER_FP16 = 1, FEATHER_FP32 = 2 };
  *             (b_by_row = true: element (n, k)).
  *   bias      N values of out_type, or null.
  *   c         [M, N] of out_type, row stride ldc >= N.
- *   workspace feather_block_scaled_mm_workspace_bytes(M, N, K, b_by_row) bytes, 256-byte aligned; may be null where that
+ *   workspace feather_block_scaled_mm_workspace_bytes(M, N, K) bytes, 256-byte aligned; may be null where that
  *             is 0. As feather_scaled_mm_splitk's: its first 64 KiB all zero before its first use, left zero by every call;
  *             calls that share it must be ordered.
  *
@@ -62,7 +62,7 @@ bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5m2, const f
                              int64_t workspace_bytes, hipStream_t stream);
 
 /* Workspace bytes of feather_block_scaled_mm for this shape (host only): 0 where it needs none, -1 outside its contract. */
-int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, bool b_by_row);
+int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /*
  * Blocks of 128 along each row of x [rows, cols] (row stride ldx): codes [rows, cols] with row stride ld_codes, scale

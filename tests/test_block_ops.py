@@ -36,7 +36,7 @@ def lib():
         getattr(handle, name).restype = BOOL
         getattr(handle, name).argtypes = args
     handle.feather_block_scaled_mm_workspace_bytes.restype = I64
-    handle.feather_block_scaled_mm_workspace_bytes.argtypes = [I64, I64, I64, BOOL]
+    handle.feather_block_scaled_mm_workspace_bytes.argtypes = [I64, I64, I64]
     handle.feather_rms_norm_backward_parts.restype = I64
     handle.feather_rms_norm_backward_parts.argtypes = [I64, I64]
     return handle
@@ -67,14 +67,17 @@ def test_product_refuses(lib, bad):
 
 def test_workspace_bytes(lib):
     need = lib.feather_block_scaled_mm_workspace_bytes
-    assert need(0, 5, 128, False) == -1 and need(5, 5, -1, False) == -1 and need(1, 1 << 31, 128, True) == -1
-    for m, n, k in [(1, 4096, 4096), (64, 1024, 16384), (512, 512, 8192), (4096, 4096, 4096), (128, 300, 16000)]:
-        for by_row in (False, True):
-            nbytes = need(m, n, k, by_row)
-            assert 0 <= nbytes < 1 << 31
-            if nbytes:   # a short, missing or unaligned one is refused
-                for ws, size in ((None, nbytes), (W, nbytes - 1), (W + 16, nbytes)):
-                    assert not _mm(lib, lda=k, ldb=k, ldc=n, M=m, N=n, K=k, ws=ws, ws_bytes=size)
+    assert need(0, 5, 128) == -1 and need(5, 5, -1) == -1 and need(1, 1 << 31, 128) == -1
+    seen = set()
+    for m, n, k in [(1, 4096, 4096), (64, 1024, 16384), (512, 512, 8192), (4096, 4096, 4096), (128, 300, 16000),
+                    (1, 128, 16384), (24, 4096, 14336), (1, 1 << 20, 128), (1 << 20, 1 << 14, 1 << 14), (300, 300, 4 << 20)]:
+        nbytes = need(m, n, k)
+        assert 0 <= nbytes < 1 << 31
+        seen.add(nbytes > 0)
+        if nbytes:   # a short, missing or unaligned one is refused
+            for ws, size in ((None, nbytes), (W, nbytes - 1), (W + 16, nbytes)):
+                assert not _mm(lib, lda=k, ldb=k, ldc=n, M=m, N=n, K=k, ws=ws, ws_bytes=size)
+    assert seen == {False, True}
 
 
 def _norm(lib, x=X, ldx=64, res=None, h=None, ldh=64, w=W, type=0, y=Y, ldy=64, codes=None, ldq=64, s=None, rows=4, cols=64):

@@ -53,40 +53,58 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     }
 }
 
-// v[0..7] = the 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are
-// zero. kVec: the row and `at` are such that whole pieces are 16-byte aligned.
+// A piece's bits as they are in memory: a value that is loaded well before it is used holds half the registers of its 8
+// floats, and its conversion does not wait for it early.
+template <int kType>
+struct RawPiece {
+    static constexpr int kWords = kType == FEATHER_FP32 ? 8 : 4;
+    uint32_t w[kWords];
+};
+
+// The 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are zero. kVec:
+// whole pieces are 16-byte aligned and rows are whole pieces (valid <= 0 or >= 8); then no load is a branch, so that all of a
+// lane's loads are in flight together: a lane past the end reads the row's first piece and drops it. (Behind branches each
+// waited for the one before: the norm of one row of 14336, 7 pieces a lane, took 10.7 us.)
 template <int kType, bool kVec>
-__device__ __forceinline__ void load_piece(const void* row, int at, int valid, float (&v)[kPiece]) {
-    if (kVec && valid >= kPiece) {
-        if constexpr (kType == FEATHER_FP32) {
-            const auto* p = reinterpret_cast<const u32x4v*>(static_cast<const float*>(row) + at);
-            const u32x4v a = p[0], b = p[1];
+__device__ __forceinline__ RawPiece<kType> load_raw(const void* row, int at, int valid) {
+    RawPiece<kType> raw;
+    if constexpr (kVec) {
+        const bool there = valid > 0;
+        const auto* p = reinterpret_cast<const u32x4v*>(static_cast<const uint8_t*>(row) + (there ? at : 0) * type_bytes(kType));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t x = a[i], y = b[i];
-                v[i] = __builtin_bit_cast(float, x);
-                v[4 + i] = __builtin_bit_cast(float, y);
-            }
-        } else {
-            const u32x4v a = *reinterpret_cast<const u32x4v*>(static_cast<const uint16_t*>(row) + at);
+        for (int h = 0; h < RawPiece<kType>::kWords / 4; ++h) {
+            const u32x4v v = p[h];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t x = a[i];
-                v[2 * i] = to_float<kType>(x & 0xffffu);
-                v[2 * i + 1] = to_float<kType>(x >> 16);
-            }
+            for (int i = 0; i < 4; ++i) raw.w[4 * h + i] = there ? v[i] : 0u;
         }
-        return;
+        return raw;
     }
+#pragma unroll
+    for (int i = 0; i < RawPiece<kType>::kWords; ++i) raw.w[i] = 0;
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
-        uint32_t bits = 0;
         if (i < valid) {
-            if constexpr (kType == FEATHER_FP32) bits = static_cast<const uint32_t*>(row)[at + i];
-            else bits = static_cast<const uint16_t*>(row)[at + i];
+            if constexpr (kType == FEATHER_FP32) raw.w[i] = static_cast<const uint32_t*>(row)[at + i];
+            else raw.w[i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[at + i]) << (16 * (i % 2));
         }
-        v[i] = to_float<kType>(bits);
     }
+    return raw;
+}
+
+template <int kType>
+__device__ __forceinline__ void unpack(const RawPiece<kType>& raw, float (&v)[kPiece]) {
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+        if constexpr (kType == FEATHER_FP32) v[i] = __builtin_bit_cast(float, raw.w[i]);
+        else if constexpr (kType == FEATHER_BF16)
+            v[i] = __builtin_bit_cast(float, i % 2 ? raw.w[i / 2] & 0xffff0000u : raw.w[i / 2] << 16);
+        else v[i] = to_float<kType>(i % 2 ? raw.w[i / 2] >> 16 : raw.w[i / 2] & 0xffffu);
+    }
+}
+
+template <int kType, bool kVec>
+__device__ __forceinline__ void load_piece(const void* row, int at, int valid, float (&v)[kPiece]) {
+    unpack(load_raw<kType, kVec>(row, at, valid), v);
 }
 
 template <int kType, bool kVec>
@@ -110,13 +128,6 @@ __device__ __forceinline__ void store_piece(void* row, int at, int valid, const 
             else static_cast<uint16_t*>(row)[at + i] = static_cast<uint16_t>(to_bits<kType>(v[i]));
         }
     }
-}
-
-// A norm's weight: of the activations' type or fp32 (kVec: 16-byte aligned).
-template <int kType, bool kVec>
-__device__ __forceinline__ void load_weight(const void* w, bool fp32, int at, int valid, float (&v)[kPiece]) {
-    if (kType != FEATHER_FP32 && fp32) load_piece<FEATHER_FP32, kVec>(w, at, valid, v);
-    else load_piece<kType, kVec>(w, at, valid, v);
 }
 
 // ---- reductions without LDS -------------------------------------------------------------------------------
@@ -189,14 +200,10 @@ struct Quantized {
     int e5m2;
 };
 
-// One piece of a row quantized with its block's 16 lanes, all of which call this together (with valid <= 0 past the row's
-// end): writes its codes, and the block's first lane the scale. kVec: ld_codes and codes are multiples of 8.
+// One piece's codes. kVec: ld_codes and codes are multiples of 8, and valid is <= 0 or >= 8.
 template <bool kVec>
-__device__ __forceinline__ void quantize_piece(const Quantized& q, int64_t row, int at, int valid,
-                                               const float (&v)[kPiece]) {
-    float factor;
-    const float scale = block_scale(max16(max_bits(v)), q.e5m2, factor);
-    if (valid <= 0) return;
+__device__ __forceinline__ void write_codes(const Quantized& q, int64_t row, int at, int valid, const float (&v)[kPiece],
+                                            float factor) {
     const u32x2v codes{codes4(v[0], v[1], v[2], v[3], factor, q.e5m2), codes4(v[4], v[5], v[6], v[7], factor, q.e5m2)};
     uint8_t* out = q.codes + row * q.ld_codes + at;
     if (kVec && valid >= kPiece) {
@@ -208,6 +215,17 @@ __device__ __forceinline__ void quantize_piece(const Quantized& q, int64_t row, 
             if (i < valid) out[i] = static_cast<uint8_t>(word >> (8 * (i % 4)));
         }
     }
+}
+
+// One piece of a row quantized with its block's 16 lanes, all of which call this together (with valid <= 0 past the row's
+// end): writes its codes, and the block's first lane the scale.
+template <bool kVec>
+__device__ __forceinline__ void quantize_piece(const Quantized& q, int64_t row, int at, int valid,
+                                               const float (&v)[kPiece]) {
+    float factor;
+    const float scale = block_scale(max16(max_bits(v)), q.e5m2, factor);
+    if (valid <= 0) return;
+    write_codes<kVec>(q, row, at, valid, v, factor);
     if (at % kBlock == 0) q.scale[row * q.scale_row + (at / kBlock) * q.scale_block] = scale;
 }
 
@@ -215,7 +233,7 @@ __device__ __forceinline__ void quantize_piece(const Quantized& q, int64_t row, 
 
 inline bool on_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Whether rows of `type` with stride ld start on 16-byte boundaries.
+// Whether rows of `type` with stride ld start on 16-byte boundaries (kVec also needs whole pieces: cols % 8 == 0).
 inline bool rows_on_16(const void* p, int64_t ld, int type) { return on_16(p) && ld * type_bytes(type) % 16 == 0; }
 
 constexpr int64_t kMaxSize = (int64_t{1} << 31) - 1;

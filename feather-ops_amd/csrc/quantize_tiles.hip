@@ -4,7 +4,8 @@
 //
 // A workgroup takes one 128 x 128 tile: 16 lanes to a row's block as everywhere, and each value's bits into LDS, where a
 // lane then walks two neighbouring columns over 32 rows (one LDS word a row, lanes on consecutive words: no conflicts).
-// The four waves' quarters of a column meet in LDS for its largest value and its sum, in wave order.
+// The four waves' quarters of a column meet in LDS for its largest value and its sum, in wave order; its codes pass through
+// LDS once more to leave as whole lines.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -30,8 +31,9 @@ struct TilesParams {
 
 template <int kType, bool kVec, bool kSquare>
 __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
-    using Word = std::conditional_t<kType == FEATHER_FP32, u32x2v, uint32_t>;   // two neighbouring values
-    __shared__ __attribute__((aligned(16))) Word values[kBlock][kBlock / 2];
+    using Raw = RawPiece<kType>;
+    constexpr int kWord = kType == FEATHER_FP32 ? 2 : 1;   // dwords of two neighbouring values
+    __shared__ __attribute__((aligned(16))) uint32_t values[kBlock][kBlock / 2 * kWord];
     __shared__ uint32_t joint_max[4][kBlock];
     __shared__ float joint_sum[4][kBlock];
     const int tid = threadIdx.x;
@@ -45,32 +47,31 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
     const int at = col0 + tid % 16 * kPiece;
     const bool walk = p.t.codes || p.sums;
 
-    float v[kSteps][kPiece];
+    Raw raw[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int r = s * 16 + tid / 16;   // past the last row: nothing of the last row
+        const int64_t row = row0 + (r < rows ? r : rows - 1);
+        raw[s] = load_raw<kType, kVec>(static_cast<const uint8_t*>(p.x) + row * p.ldx * type_bytes(kType), at,
+                                       r < rows ? p.cols - at : 0);
+    }
     uint32_t most = 0;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         const int r = s * 16 + tid / 16;
-        const int valid = r < rows ? p.cols - at : 0;
-        load_piece<kType, kVec>(static_cast<const uint8_t*>(p.x) + (row0 + r) * p.ldx * type_bytes(kType), at, valid, v[s]);
-        if constexpr (kSquare) most = max(most, max_bits(v[s]));
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int r = s * 16 + tid / 16;
         if (walk) {
-            auto* to = &values[r][tid % 16 * (kPiece / 2)];
+            auto* to = reinterpret_cast<u32x4v*>(&values[r][tid % 16 * (kPiece / 2) * kWord]);
 #pragma unroll
-            for (int i = 0; i < kPiece / 2; ++i) {
-                if constexpr (kType == FEATHER_FP32) {
-                    to[i] = u32x2v{to_bits<kType>(v[s][2 * i]), to_bits<kType>(v[s][2 * i + 1])};
-                } else {
-                    to[i] = pack2<kType>(v[s][2 * i], v[s][2 * i + 1]);
-                }
-            }
+            for (int h = 0; h < Raw::kWords / 4; ++h)
+                to[h] = u32x4v{raw[s].w[4 * h], raw[s].w[4 * h + 1], raw[s].w[4 * h + 2], raw[s].w[4 * h + 3]};
         }
-        if constexpr (!kSquare) {
+        float v[kPiece];
+        unpack(raw[s], v);
+        if constexpr (kSquare) {
+            most = max(most, max_bits(v));
+        } else {
             // valid <= 0 past the last row: quantize_piece writes nothing there
-            if (p.q.codes) quantize_piece<kVec>(p.q, row0 + r, at, r < rows ? p.cols - at : 0, v[s]);
+            if (p.q.codes) quantize_piece<kVec>(p.q, row0 + r, at, r < rows ? p.cols - at : 0, v);
         }
     }
     float factor = 0.0f, scale = 0.0f;
@@ -92,19 +93,9 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 const int r = s * 16 + tid / 16;
-                const int valid = r < rows ? p.cols - at : 0;
-                uint8_t* out = p.q.codes + (row0 + r) * p.q.ld_codes + at;
-                const u32x2v codes{codes4(v[s][0], v[s][1], v[s][2], v[s][3], factor, p.q.e5m2),
-                                   codes4(v[s][4], v[s][5], v[s][6], v[s][7], factor, p.q.e5m2)};
-                if (kVec && valid >= kPiece) {
-                    *reinterpret_cast<u32x2v*>(out) = codes;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kPiece; ++i) {
-                        const uint32_t word = codes[i / 4];
-                        if (i < valid) out[i] = static_cast<uint8_t>(word >> (8 * (i % 4)));
-                    }
-                }
+                float v[kPiece];
+                unpack(raw[s], v);
+                write_codes<kVec>(p.q, row0 + r, at, r < rows ? p.cols - at : 0, v, factor);
             }
         }
     }
@@ -115,14 +106,13 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
     uint32_t col_most[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < kWalk; ++i) {
-        const Word word = values[wave * kWalk + i][lane];
+        const uint32_t* word = &values[wave * kWalk + i][lane * kWord];
         if constexpr (kType == FEATHER_FP32) {
-            const uint32_t x0 = word[0], x1 = word[1];
-            w[0][i] = __builtin_bit_cast(float, x0);
-            w[1][i] = __builtin_bit_cast(float, x1);
+            w[0][i] = __builtin_bit_cast(float, word[0]);
+            w[1][i] = __builtin_bit_cast(float, word[1]);
         } else {
-            w[0][i] = to_float<kType>(word & 0xffffu);
-            w[1][i] = to_float<kType>(word >> 16);
+            w[0][i] = to_float<kType>(word[0] & 0xffffu);
+            w[1][i] = to_float<kType>(word[0] >> 16);
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -130,41 +120,56 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
             sum[c] += w[c][i];
         }
     }
-    __syncthreads();   // joint_max[.][0] of the square's largest value has been read
+    __syncthreads();   // joint_max[.][0] of the square's largest value, and the values, have been read
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         joint_max[wave][2 * lane + c] = col_most[c];
         joint_sum[wave][2 * lane + c] = sum[c];
     }
     __syncthreads();
+    // The transposed codes go to LDS, over the values: a column's 128 bytes as 8 pieces of 16, XOR-swizzled by the column, so
+    // that they leave as whole lines, 8 lanes to a column.
+    auto* staged = reinterpret_cast<u32x4v*>(&values[0][0]);
+    static_assert(sizeof(values) >= kBlock * kBlock, "a tile's codes fit over its values");
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         const int j = 2 * lane + c;
         const int col = col0 + j;
-        if (col >= p.cols) continue;
-        if (p.sums && wave == 0)
+        if (p.sums && wave == 0 && col < p.cols)
             p.sums[tile_m * p.cols + col] = (joint_sum[0][j] + joint_sum[1][j]) + (joint_sum[2][j] + joint_sum[3][j]);
         if (!p.t.codes) continue;
         if constexpr (!kSquare) {
             scale = block_scale(max(max(joint_max[0][j], joint_max[1][j]), max(joint_max[2][j], joint_max[3][j])),
                                 p.t.e5m2, factor);
-            if (wave == 0) p.t.scale[col * p.t.scale_row + tile_m * p.t.scale_block] = scale;
+            if (wave == 0 && col < p.cols) p.t.scale[col * p.t.scale_row + tile_m * p.t.scale_block] = scale;
         }
-        uint32_t codes[kWalk / 4];
 #pragma unroll
-        for (int i = 0; i < kWalk / 4; ++i)
-            codes[i] = codes4(w[c][4 * i], w[c][4 * i + 1], w[c][4 * i + 2], w[c][4 * i + 3], factor, p.t.e5m2);
-        const int valid = rows - wave * kWalk;
-        uint8_t* out = p.t.codes + col * p.t.ld_codes + row0 + wave * kWalk;
-        if (p.t_on_16 && valid >= kWalk) {
+        for (int h = 0; h < kWalk / 16; ++h) {
+            const float* x = &w[c][16 * h];
+            staged[j * 8 + ((wave * (kWalk / 16) + h) ^ (j / 2 % 8))] =
+                u32x4v{codes4(x[0], x[1], x[2], x[3], factor, p.t.e5m2), codes4(x[4], x[5], x[6], x[7], factor, p.t.e5m2),
+                       codes4(x[8], x[9], x[10], x[11], factor, p.t.e5m2),
+                       codes4(x[12], x[13], x[14], x[15], factor, p.t.e5m2)};
+        }
+    }
+    if (!p.t.codes) return;
+    __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kWalk / 16; ++i)
-                reinterpret_cast<u32x4v*>(out)[i] =
-                    u32x4v{codes[4 * i], codes[4 * i + 1], codes[4 * i + 2], codes[4 * i + 3]};
+    for (int s = 0; s < kBlock * kBlock / 16 / kThreads; ++s) {
+        const int j = (s * kThreads + tid) / 8;
+        const int piece = tid % 8;
+        const int valid = rows - 16 * piece;
+        if (col0 + j >= p.cols || valid <= 0) continue;
+        const u32x4v codes = staged[j * 8 + (piece ^ (j / 2 % 8))];
+        uint8_t* out = p.t.codes + (col0 + j) * p.t.ld_codes + row0 + 16 * piece;
+        if (p.t_on_16 && valid >= 16) {
+            *reinterpret_cast<u32x4v*>(out) = codes;
         } else {
 #pragma unroll
-            for (int i = 0; i < kWalk; ++i)
-                if (i < valid) out[i] = static_cast<uint8_t>(codes[i / 4] >> (8 * (i % 4)));
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t word = codes[i / 4];
+                if (i < valid) out[i] = static_cast<uint8_t>(word >> (8 * (i % 4)));
+            }
         }
     }
 }
@@ -190,7 +195,7 @@ extern "C" bool feather_quantize_tiles(const void* x, int type, int64_t ldx, boo
     const TilesParams p{x, {codes, scale, ld_codes, scale_row, scale_block, e5m2},
                         {codes_t, scale_t, ld_codes_t, scale_t_row, scale_t_block, e5m2}, sums, ldx, rows,
                         static_cast<int32_t>(cols), static_cast<int32_t>(tiles_n), on_16(codes_t) && ld_codes_t % 16 == 0};
-    const bool vec = rows_on_16(x, ldx, type) && (!codes || (on_16(codes) && ld_codes % 8 == 0));
+    const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) && (!codes || (on_16(codes) && ld_codes % 8 == 0));
     const auto grid = static_cast<uint32_t>(tiles);
     const auto go = [&](auto t, auto v) {
         if (square) tiles_kernel<t(), v(), true><<<grid, kThreads, 0, stream>>>(p);

@@ -6,8 +6,9 @@
 //
 // Both directions are streams through memory: a row is read once into registers (pieces of 8 values a lane), its sums
 // are taken there, and what is written follows from the registers. Rows of up to 2048 values belong to one wave (sums
-// by DPP, no barrier), longer ones to the four waves of a workgroup (one LDS exchange), and those past 16384 are read
-// twice by one workgroup, the second time h as it was just written.
+// by DPP, no barrier), longer ones to the four waves of a workgroup (one LDS exchange; sixteen waves where there are no more
+// rows than CUs: one row of 14336 9.6 -> 5.6 us), and those past 16384 are read twice by one workgroup, the second time h as
+// it was just written.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -56,59 +57,94 @@ __device__ __forceinline__ void* row_at(void* p, int64_t row, int64_t ld) {
     return static_cast<uint8_t*>(p) + row * ld * type_bytes(kType);
 }
 
+// Threads of a workgroup whose rows have kRowWaves waves each.
+constexpr int threads_of(int row_waves) { return row_waves > kWaves ? 64 * row_waves : kThreads; }
+
 // The sum over the kRowWaves waves that share a row, in all of their lanes.
 template <int kRowWaves>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
     v = sum64(v);
     if constexpr (kRowWaves > 1) {
-        static_assert(kRowWaves == kWaves, "a row has one wave or the whole workgroup");
+        static_assert(64 * kRowWaves == threads_of(kRowWaves), "a row has one wave or the whole workgroup");
         __syncthreads();   // the last exchange's values have been read
         if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
         __syncthreads();
-        v = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWaves; w += 2) v += lds[w] + lds[w + 1];
     }
     return v;
 }
 
 // x + residual rounded to the type, kept as h (or x alone).
 template <int kType, bool kVec>
-__device__ __forceinline__ void stream_piece(const NormParams& p, int64_t row, int at, int valid, float (&v)[kPiece]) {
-    load_piece<kType, kVec>(row_at<kType>(p.x, row, p.ldx), at, valid, v);
+__device__ __forceinline__ void stream_piece(const NormParams& p, int64_t row, int at, int valid, const RawPiece<kType>& x,
+                                             const RawPiece<kType>& residual, float (&v)[kPiece]) {
+    unpack(x, v);
     if (p.residual) {
         float res[kPiece];
-        load_piece<kType, kVec>(row_at<kType>(p.residual, row, p.ld_residual), at, valid, res);
+        unpack(residual, res);
 #pragma unroll
         for (int i = 0; i < kPiece; ++i) v[i] = to_float<kType>(to_bits<kType>(v[i] + res[i]));
-        store_piece<kType, kVec>(row_at<kType>(p.h, row, p.ldh), at, valid, v);
+        if (valid > 0) store_piece<kType, kVec>(row_at<kType>(p.h, row, p.ldh), at, valid, v);
+    }
+}
+
+// y = v r w, and where it goes. raw_w: the weight's piece where it has the activations' type.
+template <int kType, bool kVec>
+__device__ __forceinline__ void write_piece(const NormParams& p, int64_t row, int at, int valid, float r,
+                                            float (&v)[kPiece], const RawPiece<kType>& raw_w) {
+    float w[kPiece];
+    if (p.weight_fp32) load_piece<FEATHER_FP32, kVec>(p.weight, at, valid, w);
+    else unpack(raw_w, w);
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) v[i] = v[i] * r * w[i];
+    if (p.y) {
+        if (valid > 0) store_piece<kType, kVec>(row_at<kType>(p.y, row, p.ldy), at, valid, v);
+    } else {
+        quantize_piece<kVec>(p.q, row, at, valid, v);
     }
 }
 
 template <int kType, bool kVec>
-__device__ __forceinline__ void write_piece(const NormParams& p, int64_t row, int at, int valid, float r,
-                                            float (&v)[kPiece]) {
-    float w[kPiece];
-    load_weight<kType, kVec>(p.weight, p.weight_fp32, at, valid, w);
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) v[i] = v[i] * r * w[i];
-    if (p.y) store_piece<kType, kVec>(row_at<kType>(p.y, row, p.ldy), at, valid, v);
-    else quantize_piece<kVec>(p.q, row, at, valid, v);
+__device__ __forceinline__ RawPiece<kType> weight_piece(const void* weight, bool fp32, int at, int valid) {
+    return fp32 ? RawPiece<kType>{} : load_raw<kType, kVec>(weight, at, valid);
 }
 
 // kPieces: pieces per lane, all of the row's in registers (0: a row of any length, read twice).
 template <int kType, bool kVec, int kRowWaves, int kPieces>
-__global__ __launch_bounds__(kThreads) void norm_kernel(const NormParams p) {
+__global__ __launch_bounds__(threads_of(kRowWaves)) void norm_kernel(const NormParams p) {
     constexpr int kRowThreads = 64 * kRowWaves;
-    __shared__ float lds[kWaves];
+    constexpr int kRows = threads_of(kRowWaves) / kRowThreads;
+    __shared__ float lds[kRowWaves > 1 ? kRowWaves : 1];
     const int t = threadIdx.x % kRowThreads;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kRowThreads) + threadIdx.x / kRowThreads;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
     if (row >= p.rows) return;   // whole waves, and only where a row is a wave's own: no barrier is missed
     float sum = 0.0f;
     if constexpr (kPieces > 0) {
+        RawPiece<kType> x[kPieces], res[kPieces], w[kPieces];   // all loads ahead of the first use
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+            const int at = (c * kRowThreads + t) * kPiece;
+            x[c] = load_raw<kType, kVec>(row_at<kType>(p.x, row, p.ldx), at, p.cols - at);
+        }
+        if (p.residual) {
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c) {
+                const int at = (c * kRowThreads + t) * kPiece;
+                res[c] = load_raw<kType, kVec>(row_at<kType>(p.residual, row, p.ld_residual), at, p.cols - at);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+            const int at = (c * kRowThreads + t) * kPiece;
+            w[c] = weight_piece<kType, kVec>(p.weight, p.weight_fp32, at, p.cols - at);
+        }
         float v[kPieces][kPiece];
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
             const int at = (c * kRowThreads + t) * kPiece;
-            stream_piece<kType, kVec>(p, row, at, p.cols - at, v[c]);
+            stream_piece<kType, kVec>(p, row, at, p.cols - at, x[c], res[c], v[c]);
 #pragma unroll
             for (int i = 0; i < kPiece; ++i) sum += v[c][i] * v[c][i];
         }
@@ -117,26 +153,32 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const NormParams p) {
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
             const int at = (c * kRowThreads + t) * kPiece;
-            write_piece<kType, kVec>(p, row, at, p.cols - at, r, v[c]);
+            write_piece<kType, kVec>(p, row, at, p.cols - at, r, v[c], w[c]);
         }
     } else {
         const int steps = (p.cols + kRowThreads * kPiece - 1) / (kRowThreads * kPiece);
         for (int c = 0; c < steps; ++c) {
             const int at = (c * kRowThreads + t) * kPiece;
             float v[kPiece];
-            stream_piece<kType, kVec>(p, row, at, p.cols - at, v);
+            const RawPiece<kType> x = load_raw<kType, kVec>(row_at<kType>(p.x, row, p.ldx), at, p.cols - at);
+            RawPiece<kType> res{};
+            if (p.residual)
+                res = load_raw<kType, kVec>(row_at<kType>(p.residual, row, p.ld_residual), at, p.cols - at);
+            stream_piece<kType, kVec>(p, row, at, p.cols - at, x, res, v);
 #pragma unroll
             for (int i = 0; i < kPiece; ++i) sum += v[i] * v[i];
         }
         const float r = 1.0f / sqrtf(row_sum<kRowWaves>(sum, lds) / static_cast<float>(p.cols) + p.eps);
         if (t == 0 && p.rstd) p.rstd[row] = r;
+        // What a lane reads of h it wrote itself; a lane past the row's end reads the first piece and drops it.
         const void* from = p.residual ? row_at<kType>(static_cast<const void*>(p.h), row, p.ldh)
                                       : row_at<kType>(p.x, row, p.ldx);
         for (int c = 0; c < steps; ++c) {
             const int at = (c * kRowThreads + t) * kPiece;
             float v[kPiece];
-            load_piece<kType, kVec>(from, at, p.cols - at, v);   // what this lane itself wrote
-            write_piece<kType, kVec>(p, row, at, p.cols - at, r, v);
+            load_piece<kType, kVec>(from, at, p.cols - at, v);
+            write_piece<kType, kVec>(p, row, at, p.cols - at, r, v,
+                                     weight_piece<kType, kVec>(p.weight, p.weight_fp32, at, p.cols - at));
         }
     }
 }
@@ -144,42 +186,69 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const NormParams p) {
 // One piece of grad_h.
 template <int kType, bool kVec>
 __device__ __forceinline__ void write_grad(const NormBackwardParams& p, int64_t row, int at, int valid, float r,
-                                           float mean, const float (&g)[kPiece], const float (&n)[kPiece]) {
-    float out[kPiece];
+                                           float mean, const float (&g)[kPiece], const float (&n)[kPiece],
+                                           const RawPiece<kType>& grad_h_in) {
+    float out[kPiece], in[kPiece];
+    unpack(grad_h_in, in);
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) out[i] = r * (g[i] - n[i] * mean);
-    if (p.grad_h_in) {
-        float in[kPiece];
-        load_piece<kType, kVec>(row_at<kType>(p.grad_h_in, row, p.ld_grad_h_in), at, valid, in);
+    for (int i = 0; i < kPiece; ++i) out[i] = r * (g[i] - n[i] * mean) + in[i];
+    if (valid > 0) store_piece<kType, kVec>(row_at<kType>(p.grad_h, row, p.ld_grad_h), at, valid, out);
+}
+
+// One row's pieces of this lane, as loaded.
+template <int kType, int kPieces>
+struct NormRow {
+    RawPiece<kType> g[kPieces], h[kPieces], in[kPieces];
+    float r;
+};
+
+template <int kType, bool kVec, int kRowThreads, int kPieces>
+__device__ __forceinline__ void fetch_row(const NormBackwardParams& p, int64_t row, int t, NormRow<kType, kPieces>& f) {
+    f.r = p.rstd[row];
 #pragma unroll
-        for (int i = 0; i < kPiece; ++i) out[i] += in[i];
+    for (int c = 0; c < kPieces; ++c) {
+        const int at = (c * kRowThreads + t) * kPiece, valid = p.cols - at;
+        f.g[c] = load_raw<kType, kVec>(row_at<kType>(p.grad_y, row, p.ld_grad_y), at, valid);
+        f.h[c] = load_raw<kType, kVec>(row_at<kType>(p.h, row, p.ldh), at, valid);
+        f.in[c] = p.grad_h_in ? load_raw<kType, kVec>(row_at<kType>(p.grad_h_in, row, p.ld_grad_h_in), at, valid)
+                              : RawPiece<kType>{};
     }
-    store_piece<kType, kVec>(row_at<kType>(p.grad_h, row, p.ld_grad_h), at, valid, out);
 }
 
 // Rows blockIdx.x * R + (which of the workgroup's), and every gridDim.x * R on: the lanes keep the sums of grad_y n of
-// their columns over all of them.
+// their columns over all of them. The next row is on its way while a row's mean is taken.
 template <int kType, bool kVec, int kRowWaves, int kPieces>
-__global__ __launch_bounds__(kThreads) void norm_backward_kernel(const NormBackwardParams p) {
+__global__ __launch_bounds__(threads_of(kRowWaves)) void norm_backward_kernel(const NormBackwardParams p) {
     constexpr int kRowThreads = 64 * kRowWaves;
-    constexpr int kRows = kThreads / kRowThreads;
-    __shared__ float lds[kRowWaves > 1 ? kWaves : kWaves * 64 * kPiece];
+    constexpr int kRows = threads_of(kRowWaves) / kRowThreads;
+    __shared__ float lds[kRowWaves > 1 ? kRowWaves : kWaves * 64 * kPiece];
     const int t = threadIdx.x % kRowThreads;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
     float dw[kPieces][kPiece] = {};
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kRowThreads; row < p.rows;
-         row += static_cast<int64_t>(gridDim.x) * kRows) {
-        const float r = p.rstd[row];
+    RawPiece<kType> raw_w[kPieces];   // the weight's pieces where it has the activations' type
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+        const int at = (c * kRowThreads + t) * kPiece;
+        raw_w[c] = weight_piece<kType, kVec>(p.weight, p.weight_fp32, at, p.cols - at);
+    }
+    NormRow<kType, kPieces> next;
+    if (row < p.rows) fetch_row<kType, kVec, kRowThreads>(p, row, t, next);
+    for (; row < p.rows; row += step) {
+        NormRow<kType, kPieces> now = next;
+        if (row + step < p.rows) fetch_row<kType, kVec, kRowThreads>(p, row + step, t, next);
         float g[kPieces][kPiece], n[kPieces][kPiece], sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
-            const int at = (c * kRowThreads + t) * kPiece, valid = p.cols - at;
+            const int at = (c * kRowThreads + t) * kPiece;
             float w[kPiece];
-            load_piece<kType, kVec>(row_at<kType>(p.grad_y, row, p.ld_grad_y), at, valid, g[c]);
-            load_piece<kType, kVec>(row_at<kType>(p.h, row, p.ldh), at, valid, n[c]);
-            load_weight<kType, kVec>(p.weight, p.weight_fp32, at, valid, w);
+            unpack(now.g[c], g[c]);
+            unpack(now.h[c], n[c]);
+            if (p.weight_fp32) load_piece<FEATHER_FP32, kVec>(p.weight, at, p.cols - at, w);
+            else unpack(raw_w[c], w);
 #pragma unroll
             for (int i = 0; i < kPiece; ++i) {
-                n[c][i] *= r;
+                n[c][i] *= now.r;
                 dw[c][i] += g[c][i] * n[c][i];
                 g[c][i] *= w[i];
                 sum += g[c][i] * n[c][i];
@@ -189,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(const NormBackw
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
             const int at = (c * kRowThreads + t) * kPiece;
-            write_grad<kType, kVec>(p, row, at, p.cols - at, r, mean, g[c], n[c]);
+            write_grad<kType, kVec>(p, row, at, p.cols - at, now.r, mean, g[c], n[c], now.in[c]);
         }
     }
     if (!p.part) return;
@@ -211,9 +280,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(const NormBackw
                 dw[c][i] = s;
             }
         }
-#pragma unroll
-        for (int i = 0; i < kPiece; ++i)
-            if (at + i < p.cols) part[at + i] = dw[c][i];
+        store_piece<FEATHER_FP32, kVec>(part, at, p.cols - at, dw[c]);
     }
 }
 
@@ -231,14 +298,20 @@ __global__ __launch_bounds__(kThreads) void norm_backward_long_kernel(const Norm
             float g[kPiece], n[kPiece], w[kPiece];
             load_piece<kType, kVec>(row_at<kType>(p.grad_y, row, p.ld_grad_y), at, valid, g);
             load_piece<kType, kVec>(row_at<kType>(p.h, row, p.ldh), at, valid, n);
-            load_weight<kType, kVec>(p.weight, p.weight_fp32, at, valid, w);
+            if (p.weight_fp32) load_piece<FEATHER_FP32, kVec>(p.weight, at, valid, w);
+            else load_piece<kType, kVec>(p.weight, at, valid, w);
 #pragma unroll
             for (int i = 0; i < kPiece; ++i) {
                 n[i] *= r;
                 g[i] *= w[i];
                 sum += g[i] * n[i];
             }
-            if (pass == 1) write_grad<kType, kVec>(p, row, at, valid, r, mean, g, n);
+            if (pass == 1) {
+                write_grad<kType, kVec>(p, row, at, valid, r, mean, g, n,
+                                        p.grad_h_in ? load_raw<kType, kVec>(
+                                                          row_at<kType>(p.grad_h_in, row, p.ld_grad_h_in), at, valid)
+                                                    : RawPiece<kType>{});
+            }
         }
         if (pass == 0) mean = row_sum<kWaves>(sum, lds) / static_cast<float>(p.cols);
     }
@@ -259,23 +332,39 @@ __global__ __launch_bounds__(kThreads) void long_weight_kernel(const NormBackwar
         for (int i = 0; i < kPiece; ++i) dw[i] += g[i] * (n[i] * p.rstd[row]);
     }
     float* part = p.part + static_cast<int64_t>(blockIdx.y) * p.cols;
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-        if (i < valid) part[at + i] = dw[i];
+    store_piece<FEATHER_FP32, kVec>(part, at, valid, dw);
 }
 
-// out[j] = the sum of part[., j]: a workgroup takes 64 columns, its waves every fourth row each, joined in wave order.
+// out[j] = the sum of part[., j]: a workgroup takes 16 columns (a 64-byte piece of each row), its 16 groups of 16 lanes every
+// 16th row each with 8 rows in flight, joined in group order. 512 x 4096: 31 us with 64 columns and 4 groups a workgroup.
+constexpr int kSumCols = 16;
+constexpr int kSumGroups = kThreads / kSumCols;
+constexpr int kSumAhead = 8;
+
 template <int kType>
 __global__ __launch_bounds__(kThreads) void sum_rows_kernel(const float* part, void* out, int64_t rows, int64_t cols) {
-    __shared__ float lds[kThreads];
-    const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x % 64;
+    __shared__ float lds[kSumGroups][kSumCols];
+    const int group = threadIdx.x / kSumCols;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * kSumCols + threadIdx.x % kSumCols;
     float s = 0.0f;
-    if (col < cols)
-        for (int64_t i = threadIdx.x / 64; i < rows; i += kWaves) s += part[i * cols + col];
-    lds[threadIdx.x] = s;
+    if (col < cols) {
+        for (int64_t i = group; i < rows; i += kSumGroups * kSumAhead) {
+            float v[kSumAhead];
+#pragma unroll
+            for (int k = 0; k < kSumAhead; ++k) {
+                const int64_t row = i + k * kSumGroups;
+                v[k] = part[(row < rows ? row : rows - 1) * cols + col];   // no branch: 8 loads in flight
+            }
+#pragma unroll
+            for (int k = 0; k < kSumAhead; ++k) s += i + k * kSumGroups < rows ? v[k] : 0.0f;
+        }
+    }
+    lds[group][threadIdx.x % kSumCols] = s;
     __syncthreads();
-    if (threadIdx.x >= 64 || col >= cols) return;
-    s = (lds[threadIdx.x] + lds[threadIdx.x + 64]) + (lds[threadIdx.x + 128] + lds[threadIdx.x + 192]);
+    if (threadIdx.x >= kSumCols || col >= cols) return;
+    s = lds[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kSumGroups; ++k) s += lds[k][threadIdx.x];
     if constexpr (kType == FEATHER_FP32) static_cast<uint32_t*>(out)[col] = to_bits<kType>(s);
     else static_cast<uint16_t*>(out)[col] = static_cast<uint16_t>(to_bits<kType>(s));
 }
@@ -284,6 +373,7 @@ constexpr int64_t kMaxGrid = (int64_t{1} << 31) - 1;
 constexpr int64_t kWaveCols = 2048;       // rows up to here are one wave's
 constexpr int64_t kRegisterCols = 16384;  // and up to here in registers
 constexpr int64_t kLongParts = 64;
+constexpr int64_t kFewRows = 256;         // up to here (the CUs) a longer row has 16 waves
 
 // Workgroups of the backward: 512 (two a CU), fewer where the rows are.
 int64_t backward_groups(int64_t rows, int64_t cols) {
@@ -306,20 +396,22 @@ void by_type(int type, bool vec, F&& f) {
 
 // Calls f<waves per row, pieces per lane>() for rows of `cols` values (at most kRegisterCols).
 template <typename F>
-void by_cols(int64_t cols, F&& f) {
-    const auto go = [&](auto waves, auto pieces) { f(waves, pieces); };
+void by_cols(int64_t rows, int64_t cols, F&& f) {
     using W1 = std::integral_constant<int, 1>;
     using W4 = std::integral_constant<int, kWaves>;
-    if (cols <= 512) go(W1{}, std::integral_constant<int, 1>{});
-    else if (cols <= 1024) go(W1{}, std::integral_constant<int, 2>{});
-    else if (cols <= 2048) go(W1{}, std::integral_constant<int, 4>{});
-    else if (cols <= 4096) go(W4{}, std::integral_constant<int, 2>{});
-    else if (cols <= 6144) go(W4{}, std::integral_constant<int, 3>{});
-    else if (cols <= 8192) go(W4{}, std::integral_constant<int, 4>{});
-    else go(W4{}, std::integral_constant<int, 8>{});
+    using W16 = std::integral_constant<int, 16>;
+    using P1 = std::integral_constant<int, 1>;
+    using P2 = std::integral_constant<int, 2>;
+    if (cols <= 512) f(W1{}, P1{});
+    else if (cols <= 1024) f(W1{}, P2{});
+    else if (cols <= 2048) f(W1{}, std::integral_constant<int, 4>{});
+    else if (rows <= kFewRows && cols <= 8192) f(W16{}, P1{});
+    else if (rows <= kFewRows) f(W16{}, P2{});
+    else if (cols <= 4096) f(W4{}, P2{});
+    else if (cols <= 6144) f(W4{}, std::integral_constant<int, 3>{});
+    else if (cols <= 8192) f(W4{}, std::integral_constant<int, 4>{});
+    else f(W4{}, std::integral_constant<int, 8>{});
 }
-
-bool weight_on_16(const void* weight) { return on_16(weight); }
 
 }  // namespace
 }  // namespace feather
@@ -343,7 +435,7 @@ extern "C" bool feather_rms_norm(const void* x, int64_t ldx, const void* residua
         return false;
     const NormParams p{x, residual, weight, h, y, rstd, {codes, scale, ld_codes, scale_row, scale_block, e5m2},
                        ldx, ld_residual, ldh, ldy, rows, static_cast<int32_t>(cols), weight_fp32, eps};
-    const bool vec = rows_on_16(x, ldx, type) && weight_on_16(weight) &&
+    const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) && on_16(weight) &&
                      (!residual || (rows_on_16(residual, ld_residual, type) && rows_on_16(h, ldh, type))) &&
                      (y ? rows_on_16(y, ldy, type) : (on_16(codes) && ld_codes % 8 == 0));
     const int64_t groups = cols <= kWaveCols ? (rows + kWaves - 1) / kWaves : rows;
@@ -353,8 +445,9 @@ extern "C" bool feather_rms_norm(const void* x, int64_t ldx, const void* residua
             norm_kernel<t(), v(), kWaves, 0><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(p);
             return;
         }
-        by_cols(cols, [&](auto waves, auto pieces) {
-            norm_kernel<t(), v(), waves(), pieces()><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(p);
+        by_cols(rows, cols, [&](auto waves, auto pieces) {
+            norm_kernel<t(), v(), waves(), pieces()>
+                <<<static_cast<uint32_t>(groups), threads_of(waves()), 0, stream>>>(p);
         });
     });
     return true;
@@ -379,8 +472,8 @@ extern "C" bool feather_rms_norm_backward(const void* grad_y, int64_t ld_grad_y,
         return false;
     const NormBackwardParams p{grad_y, grad_h_in, h, weight, rstd, grad_h, part, ld_grad_y, ld_grad_h_in, ldh,
                                ld_grad_h, rows, static_cast<int32_t>(cols), weight_fp32};
-    const bool vec = rows_on_16(grad_y, ld_grad_y, type) && rows_on_16(h, ldh, type) &&
-                     rows_on_16(grad_h, ld_grad_h, type) && weight_on_16(weight) &&
+    const bool vec = cols % kPiece == 0 && on_16(part) && rows_on_16(grad_y, ld_grad_y, type) && rows_on_16(h, ldh, type) &&
+                     rows_on_16(grad_h, ld_grad_h, type) && on_16(weight) &&
                      (!grad_h_in || rows_on_16(grad_h_in, ld_grad_h_in, type));
     const auto groups = static_cast<uint32_t>(backward_groups(rows, cols));
     by_type(type, vec, [&](auto t, auto v) {
@@ -391,8 +484,8 @@ extern "C" bool feather_rms_norm_backward(const void* grad_y, int64_t ld_grad_y,
             long_weight_kernel<t(), v()><<<dim3(strips, groups), kThreads, 0, stream>>>(p);
             return;
         }
-        by_cols(cols, [&](auto waves, auto pieces) {
-            norm_backward_kernel<t(), v(), waves(), pieces()><<<groups, kThreads, 0, stream>>>(p);
+        by_cols(rows, cols, [&](auto waves, auto pieces) {
+            norm_backward_kernel<t(), v(), waves(), pieces()><<<groups, threads_of(waves()), 0, stream>>>(p);
         });
     });
     return true;
@@ -401,7 +494,7 @@ extern "C" bool feather_rms_norm_backward(const void* grad_y, int64_t ld_grad_y,
 extern "C" bool feather_sum_rows(const float* part, void* out, int type, int64_t rows, int64_t cols,
                                  hipStream_t stream) {
     if (!part || !out || !type_ok(type) || rows < 1 || cols < 1 || !aligned_to_type(out, type)) return false;
-    const int64_t groups = (cols + 63) / 64;
+    const int64_t groups = (cols + kSumCols - 1) / kSumCols;
     if (groups > kMaxGrid) return false;
     by_type(type, true, [&](auto t, auto) {
         sum_rows_kernel<t()><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(part, out, rows, cols);

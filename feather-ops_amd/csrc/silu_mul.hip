@@ -33,8 +33,15 @@ __device__ __forceinline__ const void* row_at(const void* p, int64_t row, int64_
     return static_cast<const uint8_t*>(p) + row * ld * type_bytes(kType);
 }
 
-// 1 / (1 + exp(-g)): exp overflows to infinity for g < -88, and the quotient is then zero.
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + __expf(-g)); }
+// 1 / (1 + exp(-g)) as q or t q with t = exp(-|g|), q = 1 / (1 + t): q's argument is in [1, 2], so the reciprocal instruction
+// (1 ulp) needs none of a division's scaling. t is a square, so that it reaches below the least normal without losing its
+// bits in the exponential. NaN stays NaN.
+__device__ __forceinline__ float sigmoid(float g) {
+    const float root = __expf(-0.5f * fabsf(g));
+    const float t = root * root;
+    const float q = __builtin_amdgcn_rcpf(1.0f + t);
+    return g < 0.0f ? t * q : q;
+}
 
 template <Op kOp, int kType, bool kVec>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsParams p) {
@@ -108,7 +115,8 @@ extern "C" bool feather_quantize_blocks(const void* x, int type, int64_t ldx, ui
         return false;
     const RowsParams p{x, nullptr, nullptr, {codes, scale, ld_codes, scale_row, scale_block, e5m2}, ldx, 0, 0, rows,
                        static_cast<int32_t>(cols), pieces_of(cols)};
-    return launch<Op::kQuantize>(p, type, rows_on_16(x, ldx, type) && on_16(codes) && ld_codes % 8 == 0, stream);
+    return launch<Op::kQuantize>(
+        p, type, cols % kPiece == 0 && rows_on_16(x, ldx, type) && on_16(codes) && ld_codes % 8 == 0, stream);
 }
 
 extern "C" bool feather_silu_mul(const void* x, int64_t ldx, int type, void* y, int64_t ldy, uint8_t* codes,
@@ -120,8 +128,8 @@ extern "C" bool feather_silu_mul(const void* x, int64_t ldx, int type, void* y, 
         return false;
     const RowsParams p{x, nullptr, y, {codes, scale, ld_codes, scale_row, scale_block, e5m2}, ldx, 0, ldy, rows,
                        static_cast<int32_t>(cols), pieces_of(cols)};
-    // up starts at column cols: on a 16-byte boundary too
-    const bool vec = rows_on_16(x, ldx, type) && cols * type_bytes(type) % 16 == 0 &&
+    // whole pieces; then up, which starts at column cols, is on a 16-byte boundary too
+    const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) &&
                      (y ? rows_on_16(y, ldy, type) : (on_16(codes) && ld_codes % 8 == 0));
     return launch<Op::kSiluMul>(p, type, vec, stream);
 }
@@ -135,7 +143,7 @@ extern "C" bool feather_silu_mul_backward(const void* grad_y, int64_t ld_grad_y,
         return false;
     const RowsParams p{x, grad_y, grad_x, {}, ldx, ld_grad_y, ld_grad_x, rows, static_cast<int32_t>(cols),
                        pieces_of(cols)};
-    const bool vec = rows_on_16(x, ldx, type) && cols * type_bytes(type) % 16 == 0 &&
+    const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) &&
                      rows_on_16(grad_y, ld_grad_y, type) && rows_on_16(grad_x, ld_grad_x, type);
     return launch<Op::kSiluMulBackward>(p, type, vec, stream);
 }

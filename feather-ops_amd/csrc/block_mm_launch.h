@@ -32,10 +32,8 @@ struct BlockMmPlan {
     int splits;             // K ranges, joined in the workspace
     int64_t tiles, slots;   // output tiles, and the parts of one that are joined by themselves
     int64_t tile_bytes;     // of a tile's fp32 sums
+    float cost;             // estimated microseconds
 };
-
-// The plan for a product of these sizes: the same one for every call of a shape.
-BlockMmPlan block_mm_plan(int64_t M, int64_t N, int64_t K);
 
 void block_mm_launch_00(const BlockMmParams& p, const BlockMmPlan& plan, bool by_row, hipStream_t stream);
 void block_mm_launch_01(const BlockMmParams& p, const BlockMmPlan& plan, bool by_row, hipStream_t stream);

@@ -221,16 +221,15 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
 
     f32x4 acc[RM][RN], t[T::kLag];
     i32x8 fa[2][2], fb[RN];     // two pairs of rows of a
-    float sa[RM];
-    ScaleB sb[kScalesB];
+    float sa[2][2];             // of two pairs of rows
+    ScaleB sb[kScalesB], sb_next{};
 #pragma unroll
     for (int j = 0; j < RN; ++j)
 #pragma unroll
         for (int i = 0; i < RM; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < T::kLag; ++n) t[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < RM; ++i) sa[i] = 0.0f;
+    sa[1][0] = sa[1][1] = 0.0f;
 #pragma unroll
     for (int j = 0; j < kScalesB; ++j) sb[j] = ScaleB{};
 
@@ -246,13 +245,6 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     fa[0][0] = read_fragment(0, a_rd, 0);
     fa[0][1] = read_fragment(0, a_rd, 1);
 
-    float sa_next[2], sb_next = 0.0f;
-    const auto read_first_scales = [&](uint32_t slot) {
-        sa_next[0] = *reinterpret_cast<const float*>(lds + slot + sa_rd);
-        sa_next[1] = *reinterpret_cast<const float*>(lds + slot + sa_rd + 64);
-        if constexpr (!kByRow) sb_next = *reinterpret_cast<const float*>(lds + slot + sb_rd);
-    };
-    read_first_scales(0);
     uint32_t cur = 0;
     uint32_t prv = (T::kSlots - 1) * T::kStageBytes;
     const auto stage = [&](int kb, auto may_end) {
@@ -267,7 +259,7 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
                 const int before = (n + T::kMfmas - T::kLag) % T::kMfmas;
                 const int bi = T::row(before), bj = T::col(before);
                 f32x4& sum = acc[bi][bj];
-                add_scaled(sum, t[n % T::kLag], sa[bi] * sb[kByRow ? bj : 0]);
+                add_scaled(sum, t[n % T::kLag], sa[bi / 2 % 2][bi % 2] * sb[kByRow ? bj : 0]);
                 asm volatile("" : "+v"(sum));
             }
             if (n == T::kBarrier) {
@@ -285,19 +277,20 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
                 fa[next_row / 2 % 2][q] = next_row < RM ? read_fragment(cur, a_rd, next_row + q) : read_fragment(nxt, a_rd, q);
             }
             if (n >= T::kBarrier && n % 2 == 1) fb[j] = read_fragment(nxt, b_rd, j);
-            // Scales: those of the first pair with the operands, the others once the stage before is done with them.
-            if (n == T::kBarrier + 2) read_first_scales(nxt);
-            if (n == T::kLag - 1) {
-                sa[0] = sa_next[0];
-                sa[1] = sa_next[1];
+            // Scales, kLag MFMAs ahead of their first use and behind the last one of what they replace: a pair of rows' at its
+            // start; a stage's of b in its first pair.
+            if (q < 2) {
+                const int pair = n / T::kPair;
+                sa[pair % 2][q] = *reinterpret_cast<const float*>(lds + cur + sa_rd + (2 * pair + q) * 64);
+            }
+            if constexpr (kByRow) {
 #pragma unroll
-                for (int r = 2; r < RM; ++r) sa[r] = *reinterpret_cast<const float*>(lds + cur + sa_rd + r * 64);
-                if constexpr (kByRow) {
-#pragma unroll
-                    for (int c = 0; c < RN; ++c) sb[c] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + c * 64 + g * 16);
-                } else {
-                    sb[0] = sb_next;
-                }
+                for (int c = 0; c < RN; ++c)
+                    if (n == (2 * c + 1 + T::kLag < T::kPair ? 0 : T::kLag - 1))
+                        sb[c] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + c * 64 + g * 16);
+            } else {
+                if (n == 0) sb_next = *reinterpret_cast<const float*>(lds + cur + sb_rd);
+                if (n == T::kLag - 1) sb[0] = sb_next;
             }
 #pragma unroll
             for (int d = 0; d < T::kLoads; ++d) {
@@ -317,7 +310,7 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     for (int n = 0; n < T::kLag; ++n) {
         constexpr int kFirst = T::kMfmas - T::kLag;
         const int i = T::row(kFirst + n), j = T::col(kFirst + n);
-        add_scaled(acc[i][j], t[(kFirst + n) % T::kLag], sa[i] * sb[kByRow ? j : 0]);
+        add_scaled(acc[i][j], t[(kFirst + n) % T::kLag], sa[i / 2 % 2][i % 2] * sb[kByRow ? j : 0]);
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // the last loads write LDS
     __builtin_amdgcn_s_waitcnt(kLgkm0Imm);

@@ -23,7 +23,7 @@ bool splits_fit(const BlockMmPlan& plan) {
 }
 
 BlockMmPlan stream_plan(BlockMmKernel kernel, int rm, int rn, int64_t M, int64_t N, int splits) {
-    BlockMmPlan plan{kernel, splits, ceil_div(M, 16 * rm) * ceil_div(N, 16 * rn), rm * rn, int64_t{1024} * rm * rn};
+    BlockMmPlan plan{kernel, splits, ceil_div(M, 16 * rm) * ceil_div(N, 16 * rn), rm * rn, int64_t{1024} * rm * rn, 0.0f};
     if (!splits_fit(plan)) plan.splits = 1;
     return plan;
 }
@@ -76,11 +76,10 @@ BlockMmPlan tile_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t blocks = std::max<int64_t>(1, ceil_div(K, kBlock));
     const float memory = static_cast<float>(N + M) * static_cast<float>(K) / 5.0e6f;   // us at 5 TB/s
     BlockMmPlan best{};
-    float least = 0.0f;
     for (const TileCost& t : kTiles) {
         const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
         for (const int splits : kSplits) {
-            const BlockMmPlan plan{t.kernel, splits, tiles, t.waves, int64_t{4} * t.bm * t.bn};
+            BlockMmPlan plan{t.kernel, splits, tiles, t.waves, int64_t{4} * t.bm * t.bn, 0.0f};
             if (splits > 1 && (splits > blocks || tiles * splits > 6 * kCUs || !splits_fit(plan))) break;
             const auto stages = static_cast<float>(ceil_div(blocks, splits));
             const int64_t groups = tiles * splits;
@@ -94,10 +93,8 @@ BlockMmPlan tile_plan(int64_t M, int64_t N, int64_t K) {
             cost = std::max(cost, memory);
             // the last of a tile's workgroups reads all of its sums back
             if (splits > 1) cost += 1.56f + 1.14f / 65536.0f * static_cast<float>(splits * plan.tile_bytes);
-            if (least == 0.0f || cost < least) {
-                least = cost;
-                best = plan;
-            }
+            plan.cost = cost;
+            if (best.cost == 0.0f || cost < best.cost) best = plan;
         }
     }
     return best;
@@ -112,22 +109,97 @@ bool sizes_ok(int64_t M, int64_t N, int64_t K) {
            ceil_div(M, 64) * ceil_div(N, 16) <= kMaxSize / 16;
 }
 
-}  // namespace
-
-BlockMmPlan block_mm_plan(int64_t M, int64_t N, int64_t K) {
+// One launch for a whole product.
+BlockMmPlan whole_plan(int64_t M, int64_t N, int64_t K) {
     // 33 to 64 rows stream only beside few columns: 64 x 2048 x 2048 6.5 us against 64 x 64 tiles' 7.7 and more, 64 x 4096 x
     // 4096 over 11 against 10.8.
-    return M <= 32 || (M <= 64 && N <= 2048) ? few_rows_plan(M, N, K) : tile_plan(M, N, K);
+    if (M > 64 || (M > 32 && N > 2048)) return tile_plan(M, N, K);
+    BlockMmPlan plan = few_rows_plan(M, N, K);
+    plan.cost = 2.0f + static_cast<float>(N) * static_cast<float>(K) / 4.5e6f;   // us: the weight at 4.5 TB/s
+    return plan;
 }
 
+// A part of a product: rows m0 .. + M, columns n0 .. + N.
+struct Part {
+    int64_t m0, n0, M, N;
+    BlockMmPlan plan;
+};
+
+struct Parts {
+    Part part[4];
+    int count;
+    float cost;
+};
+
+constexpr float kLaunchCost = 2.0f;   // us from the end of one launch to the next one's work
+
+// Large products go in up to four launches where whole rounds of tiles end at a column or row and the rest does better on
+// other tiles: 4096 x 14336 by 256 x 256 tiles is 3.5 rounds of the 256 CUs and takes 4; 12288 columns are 3, and the other
+// 2048 are one round of 128 x 256 (K = 4096: 234 us in one launch, 219 in two). Cuts fall on multiples of 256 and are
+// tried where a number of whole rounds of each tile ends, along either axis; a part may be cut once more.
+Parts cut(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, int depth) {
+    const BlockMmPlan whole = whole_plan(M, N, K);
+    Parts best{{{m0, n0, M, N, whole}}, 1, whole.cost};
+    if (depth == 0 || whole.cost < 20.0f) return best;
+    const auto attempt = [&](bool rows, int64_t at) {
+        const int64_t total = rows ? M : N;
+        if (at <= 0 || at >= total) return;
+        const BlockMmPlan first = rows ? whole_plan(at, N, K) : whole_plan(M, at, K);
+        if (first.cost + kLaunchCost >= best.cost) return;
+        const Parts heads = depth > 1 ? (rows ? cut(m0, n0, at, N, K, depth - 1) : cut(m0, n0, M, at, K, depth - 1))
+                                      : Parts{{{m0, n0, rows ? at : M, rows ? N : at, first}}, 1, first.cost};
+        const Parts rest = rows ? cut(m0 + at, n0, M - at, N, K, depth - 1) : cut(m0, n0 + at, M, N - at, K, depth - 1);
+        const float cost = heads.cost + rest.cost + kLaunchCost;
+        if (cost >= best.cost || heads.count + rest.count > 4) return;
+        best.count = 0;
+        for (int i = 0; i < heads.count; ++i) best.part[best.count++] = heads.part[i];
+        for (int i = 0; i < rest.count; ++i) best.part[best.count++] = rest.part[i];
+        best.cost = cost;
+    };
+    for (const TileCost& t : kTiles) {
+        const int64_t round = kCUs * t.per_cu;
+        const int64_t tiles_m = ceil_div(M, t.bm), tiles_n = ceil_div(N, t.bn);
+        const int64_t rounds = tiles_m * tiles_n / round;
+        if (rounds == 0) continue;
+        attempt(false, rounds * round / tiles_m * t.bn / 256 * 256);
+        attempt(true, rounds * round / tiles_n * t.bm / 256 * 256);
+    }
+    attempt(true, M / 256 * 256);
+    return best;
+}
+
+// The launches of a product: the same ones for every call of a shape. A search of large shapes takes up to 0.1 ms of the
+// host, so each thread keeps the last ones by shape.
+const Parts& parts_of(int64_t M, int64_t N, int64_t K) {
+    struct Entry {
+        int64_t M, N, K;
+        Parts parts;
+    };
+    constexpr uint64_t kEntries = 64;
+    thread_local Entry table[kEntries];
+    const auto hash = static_cast<uint64_t>(M) * 0x9e3779b97f4a7c15u + static_cast<uint64_t>(N) * 0xc2b2ae3d27d4eb4fu +
+                      static_cast<uint64_t>(K) * 0x165667b19e3779f9u;
+    Entry& e = table[(hash >> 32) % kEntries];
+    if (e.M != M || e.N != N || e.K != K || e.parts.count == 0) e = Entry{M, N, K, cut(0, 0, M, N, K, 2)};
+    return e.parts;
+}
+
+int64_t workspace_bytes_of(const Parts& parts) {
+    int64_t most = 0;
+    for (int i = 0; i < parts.count; ++i) {
+        const BlockMmPlan& plan = parts.part[i].plan;
+        if (plan.splits > 1) most = std::max(most, kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes);
+    }
+    return most;
+}
+
+}  // namespace
 }  // namespace feather
 
 using namespace feather;
 
 extern "C" int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (!sizes_ok(M, N, K)) return -1;
-    const BlockMmPlan plan = block_mm_plan(M, N, K);
-    return plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
+    return sizes_ok(M, N, K) ? workspace_bytes_of(parts_of(M, N, K)) : -1;
 }
 
 extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5m2, const float* a_scale,
@@ -137,8 +209,8 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
                                         int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                                         hipStream_t stream) {
     if (!sizes_ok(M, N, K) || !type_ok(out_type)) return false;
-    const BlockMmPlan plan = block_mm_plan(M, N, K);
-    const int64_t need = plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
+    const Parts& parts = parts_of(M, N, K);
+    const int64_t need = workspace_bytes_of(parts);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0))
         return false;
     if (K > 0 && (!a || !b || !a_scale || !b_scale || !on_16(a) || !on_16(b) || lda < K || ldb < K || lda % 16 != 0 ||
@@ -151,11 +223,18 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
     const int bytes = type_bytes(out_type);
     const bool store4 = (reinterpret_cast<uintptr_t>(c) & (4 * bytes - 1)) == 0 && ldc % 4 == 0;
     const bool store8 = rows_on_16(c, ldc, out_type) && N % 8 == 0 && on_16(bias);
-    const BlockMmParams p{a, b, a_scale, b_scale, lda, ldb, a_scale_row, a_scale_block, b_scale_row, b_scale_block,
-                          static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), plan.splits, bias, c,
-                          ldc, out_type, store4, store8, static_cast<uint32_t*>(workspace),
-                          need > 0 ? static_cast<uint8_t*>(workspace) + kCtrBytes : nullptr};
-    (a_e5m2 ? (b_e5m2 ? block_mm_launch_11 : block_mm_launch_10) : (b_e5m2 ? block_mm_launch_01 : block_mm_launch_00))(
-        p, plan, b_by_row, stream);
+    const auto launch = a_e5m2 ? (b_e5m2 ? block_mm_launch_11 : block_mm_launch_10)
+                               : (b_e5m2 ? block_mm_launch_01 : block_mm_launch_00);
+    for (int i = 0; i < parts.count; ++i) {
+        const Part& part = parts.part[i];   // n0 is a multiple of 256: whole squares and aligned pieces
+        const BlockMmParams p{
+            a + part.m0 * lda, b + part.n0 * ldb, a_scale + part.m0 * a_scale_row,
+            b_scale + (b_by_row ? part.n0 : part.n0 / kBlock) * b_scale_row, lda, ldb, a_scale_row, a_scale_block,
+            b_scale_row, b_scale_block, static_cast<int32_t>(part.M), static_cast<int32_t>(part.N), static_cast<int32_t>(K),
+            part.plan.splits, bias ? static_cast<const uint8_t*>(bias) + part.n0 * bytes : nullptr,
+            static_cast<uint8_t*>(c) + (part.m0 * ldc + part.n0) * bytes, ldc, out_type, store4, store8,
+            static_cast<uint32_t*>(workspace), need > 0 ? static_cast<uint8_t*>(workspace) + kCtrBytes : nullptr};
+        launch(p, part.plan, b_by_row, stream);
+    }
     return true;
 }

@@ -2,8 +2,7 @@
 // rows, and the quantization of blocks.
 //
 // A row is handled in pieces of 8 consecutive values, one per lane and step, so a block of 128 is the 16 lanes of one DPP
-// row: its largest value takes four row rotations and no LDS. Rows whose start or stride is not 16-byte aligned, and a
-// row's last piece where it is short, go value by value.
+// row: its largest value takes four row rotations and no LDS.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -61,26 +60,61 @@ struct RawPiece {
     uint32_t w[kWords];
 };
 
-// The 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are zero. kVec:
-// whole pieces are 16-byte aligned and rows are whole pieces (valid <= 0 or >= 8); then no load is a branch, so that all of a
-// lane's loads are in flight together: a lane past the end reads the row's first piece and drops it. (Behind branches each
-// waited for the one before: the norm of one row of 14336, 7 pieces a lane, took 10.7 us.)
+// 16 or 8 bytes from or to an address of any alignment, one access (the GPU runs in its unaligned mode, as HSA sets it).
+template <typename V>
+__device__ __forceinline__ V load_any(const void* p) {
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+
+template <typename V>
+__device__ __forceinline__ void store_any(void* p, V v) {
+    __builtin_memcpy(p, &v, sizeof(V));
+}
+
+// The piece without its first `n` (0 .. 8) values, the rest moved down and zeros behind.
+template <int kType>
+__device__ __forceinline__ RawPiece<kType> drop_values(RawPiece<kType> raw, int n) {
+    constexpr int kWords = RawPiece<kType>::kWords;
+    const int words = kType == FEATHER_FP32 ? n : n / 2;
+#pragma unroll
+    for (int by = kWords; by >= 1; by /= 2) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) raw.w[i] = words & by ? (i + by < kWords ? raw.w[i + by] : 0u) : raw.w[i];
+    }
+    if (kType != FEATHER_FP32 && n % 2) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) raw.w[i] = raw.w[i] >> 16 | (i + 1 < kWords ? raw.w[i + 1] << 16 : 0u);
+    }
+    return raw;
+}
+
+// The 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are zero. No load
+// is a branch, so that all of a lane's loads are in flight together. (Behind branches each waited for the one before: the
+// norm of one row of 14336, 7 pieces a lane, took 10.7 us.)
+// kVec: whole pieces are 16-byte aligned and rows are whole pieces (valid <= 0 or >= 8): a lane past the end reads the
+// row's first piece and drops it. Otherwise pieces of any alignment; one past or over the row's end reads the row's last 8
+// values and drops those before it; rows shorter than a piece go value by value. (Value by value throughout, the norm of
+// 4096 x 4097 took 76 us, with 4096 columns 25.)
 template <int kType, bool kVec>
 __device__ __forceinline__ RawPiece<kType> load_raw(const void* row, int at, int valid) {
+    constexpr int kWords = RawPiece<kType>::kWords;
     RawPiece<kType> raw;
-    if constexpr (kVec) {
-        const bool there = valid > 0;
-        const auto* p = reinterpret_cast<const u32x4v*>(static_cast<const uint8_t*>(row) + (there ? at : 0) * type_bytes(kType));
+    if (kVec || at + valid >= kPiece) {
+        const int over = kVec ? 0 : min(kPiece, max(0, kPiece - valid));   // values of the piece past the row's end
+        const int from = kVec ? (valid > 0 ? at : 0) : min(at, at + valid - kPiece);
+        const uint8_t* p = static_cast<const uint8_t*>(row) + static_cast<int64_t>(from) * type_bytes(kType);
 #pragma unroll
-        for (int h = 0; h < RawPiece<kType>::kWords / 4; ++h) {
-            const u32x4v v = p[h];
+        for (int h = 0; h < kWords / 4; ++h) {
+            const u32x4v v = kVec ? reinterpret_cast<const u32x4v*>(p)[h] : load_any<u32x4v>(p + 16 * h);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw.w[4 * h + i] = there ? v[i] : 0u;
+            for (int i = 0; i < 4; ++i) raw.w[4 * h + i] = !kVec || valid > 0 ? v[i] : 0u;
         }
-        return raw;
+        return kVec || over == 0 ? raw : drop_values(raw, over);
     }
 #pragma unroll
-    for (int i = 0; i < RawPiece<kType>::kWords; ++i) raw.w[i] = 0;
+    for (int i = 0; i < kWords; ++i) raw.w[i] = 0;
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
         if (i < valid) {
@@ -109,23 +143,28 @@ __device__ __forceinline__ void load_piece(const void* row, int at, int valid, f
 
 template <int kType, bool kVec>
 __device__ __forceinline__ void store_piece(void* row, int at, int valid, const float (&v)[kPiece]) {
-    if (kVec && valid >= kPiece) {
+    uint8_t* out = static_cast<uint8_t*>(row) + static_cast<int64_t>(at) * type_bytes(kType);
+    if (valid >= kPiece) {
+        u32x4v words[type_bytes(kType) / 2];
         if constexpr (kType == FEATHER_FP32) {
-            auto* p = reinterpret_cast<u32x4v*>(static_cast<float*>(row) + at);
-            p[0] = u32x4v{to_bits<kType>(v[0]), to_bits<kType>(v[1]), to_bits<kType>(v[2]), to_bits<kType>(v[3])};
-            p[1] = u32x4v{to_bits<kType>(v[4]), to_bits<kType>(v[5]), to_bits<kType>(v[6]), to_bits<kType>(v[7])};
+            words[0] = u32x4v{to_bits<kType>(v[0]), to_bits<kType>(v[1]), to_bits<kType>(v[2]), to_bits<kType>(v[3])};
+            words[1] = u32x4v{to_bits<kType>(v[4]), to_bits<kType>(v[5]), to_bits<kType>(v[6]), to_bits<kType>(v[7])};
         } else {
-            *reinterpret_cast<u32x4v*>(static_cast<uint16_t*>(row) + at) =
-                u32x4v{pack2<kType>(v[0], v[1]), pack2<kType>(v[2], v[3]), pack2<kType>(v[4], v[5]),
-                       pack2<kType>(v[6], v[7])};
+            words[0] = u32x4v{pack2<kType>(v[0], v[1]), pack2<kType>(v[2], v[3]), pack2<kType>(v[4], v[5]),
+                              pack2<kType>(v[6], v[7])};
+        }
+#pragma unroll
+        for (int h = 0; h < type_bytes(kType) / 2; ++h) {
+            if constexpr (kVec) reinterpret_cast<u32x4v*>(out)[h] = words[h];
+            else store_any(out + 16 * h, words[h]);
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
         if (i < valid) {
-            if constexpr (kType == FEATHER_FP32) static_cast<uint32_t*>(row)[at + i] = to_bits<kType>(v[i]);
-            else static_cast<uint16_t*>(row)[at + i] = static_cast<uint16_t>(to_bits<kType>(v[i]));
+            if constexpr (kType == FEATHER_FP32) reinterpret_cast<uint32_t*>(out)[i] = to_bits<kType>(v[i]);
+            else reinterpret_cast<uint16_t*>(out)[i] = static_cast<uint16_t>(to_bits<kType>(v[i]));
         }
     }
 }
@@ -206,8 +245,9 @@ __device__ __forceinline__ void write_codes(const Quantized& q, int64_t row, int
                                             float factor) {
     const u32x2v codes{codes4(v[0], v[1], v[2], v[3], factor, q.e5m2), codes4(v[4], v[5], v[6], v[7], factor, q.e5m2)};
     uint8_t* out = q.codes + row * q.ld_codes + at;
-    if (kVec && valid >= kPiece) {
-        *reinterpret_cast<u32x2v*>(out) = codes;
+    if (valid >= kPiece) {
+        if constexpr (kVec) *reinterpret_cast<u32x2v*>(out) = codes;
+        else store_any(out, codes);
     } else {
 #pragma unroll
         for (int i = 0; i < kPiece; ++i) {

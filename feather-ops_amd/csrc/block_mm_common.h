@@ -35,7 +35,6 @@ struct BlockMmParams {
     void* c;
     int64_t ldc;
     int32_t out_type;
-    int32_t store4, store8; // four and eight neighbouring outputs (and biases) are aligned stores
     uint32_t* split_ctr;
     uint8_t* split_part;
 };
@@ -87,18 +86,18 @@ __device__ __forceinline__ void store_out(const BlockMmParams& p, int m, int n, 
         }
         if constexpr (kType == FEATHER_FP32) {
             auto* out = static_cast<float*>(p.c) + at;
-            if (p.store4 && valid >= 4) {
-                *reinterpret_cast<f32x4*>(out) = v;
+            if (valid >= 4) {
+                store_any(out, v);
             } else {
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 3; ++i)
                     if (i < valid) out[i] = v[i];
             }
         } else {
             auto* out = static_cast<uint16_t*>(p.c) + at;
-            if (p.store4 && valid >= 4) {
-                *reinterpret_cast<u32x2*>(out) = u32x2{pack2<kType>(v[0], v[1]), pack2<kType>(v[2], v[3])};
+            if (valid >= 4) {
+                store_any(out, u32x2{pack2<kType>(v[0], v[1]), pack2<kType>(v[2], v[3])});
             } else {
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 3; ++i)
                     if (i < valid) out[i] = static_cast<uint16_t>(to_bits<kType>(v[i]));
             }
         }

@@ -221,18 +221,16 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
     if (!c || ldc < N || ldc > kMaxSize || !aligned_to_type(c, out_type) || (bias && !aligned_to_type(bias, out_type)))
         return false;
     const int bytes = type_bytes(out_type);
-    const bool store4 = (reinterpret_cast<uintptr_t>(c) & (4 * bytes - 1)) == 0 && ldc % 4 == 0;
-    const bool store8 = rows_on_16(c, ldc, out_type) && N % 8 == 0 && on_16(bias);
     const auto launch = a_e5m2 ? (b_e5m2 ? block_mm_launch_11 : block_mm_launch_10)
                                : (b_e5m2 ? block_mm_launch_01 : block_mm_launch_00);
     for (int i = 0; i < parts.count; ++i) {
-        const Part& part = parts.part[i];   // n0 is a multiple of 256: whole squares and aligned pieces
+        const Part& part = parts.part[i];   // n0 is a multiple of 256: whole squares
         const BlockMmParams p{
             a + part.m0 * lda, b + part.n0 * ldb, a_scale + part.m0 * a_scale_row,
             b_scale + (b_by_row ? part.n0 : part.n0 / kBlock) * b_scale_row, lda, ldb, a_scale_row, a_scale_block,
             b_scale_row, b_scale_block, static_cast<int32_t>(part.M), static_cast<int32_t>(part.N), static_cast<int32_t>(K),
             part.plan.splits, bias ? static_cast<const uint8_t*>(bias) + part.n0 * bytes : nullptr,
-            static_cast<uint8_t*>(c) + (part.m0 * ldc + part.n0) * bytes, ldc, out_type, store4, store8,
+            static_cast<uint8_t*>(c) + (part.m0 * ldc + part.n0) * bytes, ldc, out_type,
             static_cast<uint32_t*>(workspace), need > 0 ? static_cast<uint8_t*>(workspace) + kCtrBytes : nullptr};
         launch(p, part.plan, b_by_row, stream);
     }

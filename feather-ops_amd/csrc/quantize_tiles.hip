@@ -26,7 +26,6 @@ struct TilesParams {
     float* sums;            // null: left out
     int64_t ldx, rows;
     int32_t cols, tiles_n;
-    int32_t t_on_16;        // rows of the transposed codes start on 16-byte boundaries
 };
 
 template <int kType, bool kVec, bool kSquare>
@@ -162,8 +161,8 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
         if (col0 + j >= p.cols || valid <= 0) continue;
         const u32x4v codes = staged[j * 8 + (piece ^ (j / 2 % 8))];
         uint8_t* out = p.t.codes + (col0 + j) * p.t.ld_codes + row0 + 16 * piece;
-        if (p.t_on_16 && valid >= 16) {
-            *reinterpret_cast<u32x4v*>(out) = codes;
+        if (valid >= 16) {
+            store_any(out, codes);   // ld_codes_t is any
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -194,7 +193,7 @@ extern "C" bool feather_quantize_tiles(const void* x, int type, int64_t ldx, boo
     if (tiles > kMaxSize) return false;
     const TilesParams p{x, {codes, scale, ld_codes, scale_row, scale_block, e5m2},
                         {codes_t, scale_t, ld_codes_t, scale_t_row, scale_t_block, e5m2}, sums, ldx, rows,
-                        static_cast<int32_t>(cols), static_cast<int32_t>(tiles_n), on_16(codes_t) && ld_codes_t % 16 == 0};
+                        static_cast<int32_t>(cols), static_cast<int32_t>(tiles_n)};
     const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) && (!codes || (on_16(codes) && ld_codes % 8 == 0));
     const auto grid = static_cast<uint32_t>(tiles);
     const auto go = [&](auto t, auto v) {

@@ -33,9 +33,9 @@ void stream_rows(const BlockMmParams& p, bool by_row, hipStream_t stream) {
 void FEATHER_CAT(block_mm_launch_, FEATHER_A_E5M2, FEATHER_B_E5M2)(const BlockMmParams& p, const BlockMmPlan& plan,
                                                                     bool by_row, hipStream_t stream) {
     switch (plan.kernel) {
-        case kTile64x64: tile<BlockTile<64, 64, 1, 2, 4>>(p, by_row, stream); break;
-        case kTile64x128: tile<BlockTile<64, 128, 1, 4, 3>>(p, by_row, stream); break;
-        case kTile128x128: tile<BlockTile<128, 128, 2, 4, 4>>(p, by_row, stream); break;
+        case kTile64x64: tile<BlockTile<64, 64, 1, 2, 4, true>>(p, by_row, stream); break;
+        case kTile64x128: tile<BlockTile<64, 128, 1, 4, 3, true>>(p, by_row, stream); break;
+        case kTile128x128: tile<BlockTile<128, 128, 2, 4, 3, true>>(p, by_row, stream); break;
         case kTile128x256: tile<BlockTile<128, 256, 2, 4, 3>>(p, by_row, stream); break;
         case kTile256x128: tile<BlockTile<256, 128, 4, 2, 3>>(p, by_row, stream); break;
         case kTile256x256: tile<BlockTile<256, 256, 2, 4, 2>>(p, by_row, stream); break;

@@ -1,14 +1,29 @@
 // The tile kernel of the block-scaled fp8 product: a workgroup owns BM x BN outputs, its WM x WN waves split them, and K
 // streams through an LDS ring of one-block (128-deep) stages that direct global-to-LDS loads fill.
+//
+// A stage's 16 x 16 x 128 MFMAs take 32 clocks each and the four multiply-adds that add their result 16 of the vector unit,
+// which runs beside (an MFMA stream with 4 fp32 multiply-adds an MFMA ran at 34 clocks, with 8 at 46: scales by row of b,
+// which need 4 products more, are that much slower). Two waves a SIMD hide each other's LDS reads and barrier.
+//
+// What bounds the 256 x 256 tile is power: at 4096 x 16384 x 4096 a stage takes 2540 clocks where its MFMAs alone take 2048, but
+// the clock falls to 1.6 GHz on random operands (an MFMA stream alone: 2.0 GHz). Without the multiply-adds the product took 205
+// us of 235, without LDS reads 168, without the loads 206, without the barrier 233; as many LDS reads again for half the
+// fragments cost 20 us. Rows of a instead of pairs, loads spread over 3 or 6 eighths of a stage, and raised wave priority
+// around the MFMAs were the same or slower; 4 x 2 waves of 64 x 128 368 us.
+//
+// Smaller tiles have the registers to read the next stage's fragments a stage ahead (kAhead: 128 x 128 tiles 3-4% faster, 64 x
+// 64 up to 8%, 64 x 128 even); they are bound by a stage's fixed costs: at 1024 x 4096 x 4096 a 128 x 128 stage takes 0.69 us, of
+// which the loads' issue is 0.23, the LDS reads 0.10 and the MFMAs 0.26.
 #pragma once
 
 #include "block_mm_common.h"
 
 namespace feather {
 
-template <int BM_, int BN_, int WM_, int WN_, int kSlots_, int kSpread = 5>
+template <int BM_, int BN_, int WM_, int WN_, int kSlots_, bool kAhead_ = false, int kSpread = 5>
 struct BlockTile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kSlots = kSlots_;
+    static constexpr bool kAhead = kAhead_;
     static constexpr int kWaves = WM * WN;
     static constexpr int kThreads = 64 * kWaves;
     static constexpr int RM = BM / WM / 16;             // 16-row fragments of a per wave
@@ -34,6 +49,11 @@ struct BlockTile {
     // a stage's MFMAs: load d after MFMA at(d), from kMfmas on in the next stage.
     static constexpr int kBarrier = kMfmas - kPair;
     static constexpr int at(int d) { return kBarrier + 1 + d * (kMfmas * kSpread / 8) / kLoads; }
+    // kAhead: the barrier comes before the first MFMA, and load d after MFMA ahead_at(d) of the same stage; the next stage's
+    // fragments are read in the order of their use over the stage.
+    static constexpr int ahead_at(int d) { return d * kMfmas / kLoads; }
+    static constexpr int kFragments = RM + RN;
+    static constexpr int read_at(int f) { return f * kMfmas / kFragments; }
     static constexpr int kEarly = [] {
         int n = 0;
         while (n < kLoads && at(n) < kMfmas) ++n;
@@ -44,6 +64,7 @@ struct BlockTile {
     static_assert(kABytes % (1024 * kWaves) == 0 && kBBytes % (1024 * kWaves) == 0, "whole loads");
     static_assert(RM % 4 == 0, "pairs of rows go through two sets of registers");
     static_assert(kBlock % (BN / WN) == 0, "a wave's columns have one square scale");
+    static_assert(!kAhead || kMfmas > kLag, "scales are replaced after their last use");
     static_assert((kSlots - 1) * kLoads < 64, "vmcnt range");
 };
 
@@ -205,97 +226,187 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     static_assert(T::kWaves * 16 * OutRow<RN>::kPitch * 4 <= T::kLdsBytes, "the epilogue's rows fit");
 
     f32x4 acc[RM][RN], t[T::kLag];
-    i32x8 fa[2][2], fb[RN];     // two pairs of rows of a
-    float sa[2][2];             // of two pairs of rows
-    ScaleB sb[kScalesB], sb_next{};
 #pragma unroll
     for (int j = 0; j < RN; ++j)
 #pragma unroll
         for (int i = 0; i < RM; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < T::kLag; ++n) t[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    sa[1][0] = sa[1][1] = 0.0f;
+    if constexpr (T::kAhead) {
+        i32x8 fa[2][RM], fb[2][RN];     // of a stage and the next
+        float sa[2][RM];
+        ScaleB sb[2][kScalesB];
 #pragma unroll
-    for (int j = 0; j < kScalesB; ++j) sb[j] = ScaleB{};
+        for (int i = 0; i < RM; ++i) sa[1][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kScalesB; ++j) sb[1][j] = ScaleB{};
+        // Fragment f of a stage in the order of its use: two rows of a, the columns of b, the other rows.
+        const auto read = [&](auto set, uint32_t slot, int f) {
+            constexpr int s = set();
+            if (f < 2) fa[s][f] = read_fragment(slot, a_rd, f);
+            else if (f < 2 + RN) fb[s][f - 2] = read_fragment(slot, b_rd, f - 2);
+            else fa[s][f - RN] = read_fragment(slot, a_rd, f - RN);
+        };
+        const auto read_scales = [&](auto set, uint32_t slot) {
+            constexpr int s = set();
+#pragma unroll
+            for (int i = 0; i < RM; ++i) sa[s][i] = *reinterpret_cast<const float*>(lds + slot + sa_rd + i * 64);
+#pragma unroll
+            for (int j = 0; j < kScalesB; ++j) {
+                if constexpr (kByRow) sb[s][j] = *reinterpret_cast<const f32x4*>(lds + slot + sb_rd + j * 64 + g * 16);
+                else sb[s][j] = *reinterpret_cast<const float*>(lds + slot + sb_rd);
+            }
+        };
+        using Even = std::integral_constant<int, 0>;
+        using Odd = std::integral_constant<int, 1>;
 
 #pragma unroll
-    for (int s = 0; s < T::kSlots; ++s)
+        for (int s = 0; s < T::kSlots; ++s)
 #pragma unroll
-        for (int d = 0; d < (s + 1 < T::kSlots ? T::kLoads : T::kEarly); ++d) load(d, s, s * T::kStageBytes);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads + T::kEarly));
-    barrier_only();
-    if (tail && stages == 1) clear_tail(0);
+            for (int d = 0; d < T::kLoads; ++d) load(d, s, s * T::kStageBytes);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 1) * T::kLoads));
+        barrier_only();
+        if (tail && stages == 1) clear_tail(0);
 #pragma unroll
-    for (int j = 0; j < RN; ++j) fb[j] = read_fragment(0, b_rd, j);
-    fa[0][0] = read_fragment(0, a_rd, 0);
-    fa[0][1] = read_fragment(0, a_rd, 1);
+        for (int f = 0; f < T::kFragments; ++f) read(Even{}, 0, f);
+        read_scales(Even{}, 0);
 
-    uint32_t cur = 0;
-    uint32_t prv = (T::kSlots - 1) * T::kStageBytes;
-    const auto stage = [&](int kb, auto may_end) {
-        const uint32_t nxt = cur + T::kStageBytes == T::kLdsBytes ? 0 : cur + T::kStageBytes;
+        uint32_t cur = 0;
+        const auto stage = [&](int kb, auto set, auto other) {
+            const uint32_t nxt = cur + T::kStageBytes == T::kLdsBytes ? 0 : cur + T::kStageBytes;
+            // This stage is in registers, and the next has landed, for every wave past the barrier: the slot is free.
+            __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads));
+            barrier_only();
+            if (tail && kb + 2 == stages) clear_tail(nxt);
 #pragma unroll
-        for (int n = 0; n < T::kMfmas; ++n) {
-            const int i = T::row(n), j = T::col(n);
-            {
-                // The product of kLag MFMAs ago (at first: of the stage before, with its scales) leaves its registers to this
-                // one's. The empty asm keeps the compiler from gathering the multiply-adds behind the stage's MFMAs, where
-                // nothing hides them.
+            for (int n = 0; n < T::kMfmas; ++n) {
+                const int i = T::row(n), j = T::col(n);
                 const int before = (n + T::kMfmas - T::kLag) % T::kMfmas;
                 const int bi = T::row(before), bj = T::col(before);
+                constexpr int s = set(), o = other();
                 f32x4& sum = acc[bi][bj];
-                add_scaled(sum, t[n % T::kLag], sa[bi / 2 % 2][bi % 2] * sb[kByRow ? bj : 0]);
-                asm volatile("" : "+v"(sum));
-            }
-            if (n == T::kBarrier) {
-                // All of this stage's operands are read and the next stage has landed, for every wave past the barrier.
-                __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads));
-                barrier_only();
-                if (may_end() && kb + 2 == stages) clear_tail(nxt);
-            }
-            t[n % T::kLag] = mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i / 2 % 2][i % 2]);
-            // Operands: a pair of rows during the pair before, a column of b after its last use.
-            const int q = n % T::kPair;
-            const int next_row = n / T::kPair * 2 + 2;
-            if (q < 2) {
-                fa[next_row / 2 % 2][q] = next_row < RM ? read_fragment(cur, a_rd, next_row + q) : read_fragment(nxt, a_rd, q);
-            }
-            if (n >= T::kBarrier && n % 2 == 1) fb[j] = read_fragment(nxt, b_rd, j);
-            // Scales, kLag MFMAs ahead of their first use and behind the last one of what they replace: a pair of rows' at its
-            // start; a stage's of b in its first pair.
-            if (q < 2) {
-                const int pair = n / T::kPair;
-                sa[pair % 2][q] = *reinterpret_cast<const float*>(lds + cur + sa_rd + (2 * pair + q) * 64);
-            }
-            if constexpr (kByRow) {
+                if (n < T::kLag) add_scaled(sum, t[n % T::kLag], sa[o][bi] * sb[o][kByRow ? bj : 0]);
+                else add_scaled(sum, t[n % T::kLag], sa[s][bi] * sb[s][kByRow ? bj : 0]);
+                asm volatile("" : "+v"(sum));   // as below: in place, not behind the MFMAs
+                t[n % T::kLag] = mfma_block<kAE5M2, kBE5M2>(fb[s][j], fa[s][i]);
 #pragma unroll
-                for (int c = 0; c < RN; ++c)
-                    if (n == (2 * c + 1 + T::kLag < T::kPair ? 0 : T::kLag - 1))
-                        sb[c] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + c * 64 + g * 16);
-            } else {
-                if (n == 0) sb_next = *reinterpret_cast<const float*>(lds + cur + sb_rd);
-                if (n == T::kLag - 1) sb[0] = sb_next;
-            }
+                for (int f = 0; f < T::kFragments; ++f)
+                    if (T::read_at(f) == n) read(other, nxt, f);
+                if (n == T::kLag) read_scales(other, nxt);
 #pragma unroll
-            for (int d = 0; d < T::kLoads; ++d) {
-                if (T::at(d) == n) load(d, kb + T::kSlots, cur);
-                if (T::at(d) - T::kMfmas == n) load(d, kb + T::kSlots - 1, prv);
+                for (int d = 0; d < T::kLoads; ++d)
+                    if (T::ahead_at(d) == n) load(d, kb + T::kSlots, cur);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            cur = nxt;
+        };
+        for (int kb = 0; kb < stages; kb += 2) {
+            stage(kb, Even{}, Odd{});
+            if (kb + 1 < stages) stage(kb + 1, Odd{}, Even{});
         }
-        prv = cur;
-        cur = nxt;
-    };
-    const int plain = !tail ? stages : stages < 2 ? 0 : stages - 2;
-    int kb = 0;
-    for (; kb < plain; ++kb) stage(kb, std::false_type{});
-    for (; kb < stages; ++kb) stage(kb, std::true_type{});
+        const auto last = [&](auto set) {
+            constexpr int kFirst = T::kMfmas - T::kLag;
+            constexpr int s = set();
 #pragma unroll
-    for (int n = 0; n < T::kLag; ++n) {
-        constexpr int kFirst = T::kMfmas - T::kLag;
-        const int i = T::row(kFirst + n), j = T::col(kFirst + n);
-        add_scaled(acc[i][j], t[(kFirst + n) % T::kLag], sa[i / 2 % 2][i % 2] * sb[kByRow ? j : 0]);
+            for (int n = 0; n < T::kLag; ++n) {
+                const int i = T::row(kFirst + n), j = T::col(kFirst + n);
+                add_scaled(acc[i][j], t[(kFirst + n) % T::kLag], sa[s][i] * sb[s][kByRow ? j : 0]);
+            }
+        };
+        if (stages % 2 == 0) last(Odd{});
+        else last(Even{});
+    } else {
+        i32x8 fa[2][2], fb[RN];     // two pairs of rows of a
+        float sa[2][2];             // of two pairs of rows
+        ScaleB sb[kScalesB], sb_next{};
+        sa[1][0] = sa[1][1] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kScalesB; ++j) sb[j] = ScaleB{};
+
+#pragma unroll
+        for (int s = 0; s < T::kSlots; ++s)
+#pragma unroll
+            for (int d = 0; d < (s + 1 < T::kSlots ? T::kLoads : T::kEarly); ++d) load(d, s, s * T::kStageBytes);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads + T::kEarly));
+        barrier_only();
+        if (tail && stages == 1) clear_tail(0);
+#pragma unroll
+        for (int j = 0; j < RN; ++j) fb[j] = read_fragment(0, b_rd, j);
+        fa[0][0] = read_fragment(0, a_rd, 0);
+        fa[0][1] = read_fragment(0, a_rd, 1);
+
+        uint32_t cur = 0;
+        uint32_t prv = (T::kSlots - 1) * T::kStageBytes;
+        const auto stage = [&](int kb, auto may_end) {
+            const uint32_t nxt = cur + T::kStageBytes == T::kLdsBytes ? 0 : cur + T::kStageBytes;
+#pragma unroll
+            for (int n = 0; n < T::kMfmas; ++n) {
+                const int i = T::row(n), j = T::col(n);
+                {
+                    // The product of kLag MFMAs ago (at first: of the stage before, with its scales) leaves its registers to this
+                    // one's. The empty asm keeps the compiler from gathering the multiply-adds behind the stage's MFMAs, where
+                    // nothing hides them.
+                    const int before = (n + T::kMfmas - T::kLag) % T::kMfmas;
+                    const int bi = T::row(before), bj = T::col(before);
+                    f32x4& sum = acc[bi][bj];
+                    add_scaled(sum, t[n % T::kLag], sa[bi / 2 % 2][bi % 2] * sb[kByRow ? bj : 0]);
+                    asm volatile("" : "+v"(sum));
+                }
+                if (n == T::kBarrier) {
+                    // All of this stage's operands are read and the next stage has landed, for every wave past the barrier.
+                    __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
+                    __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::kSlots - 2) * T::kLoads));
+                    barrier_only();
+                    if (may_end() && kb + 2 == stages) clear_tail(nxt);
+                }
+                t[n % T::kLag] = mfma_block<kAE5M2, kBE5M2>(fb[j], fa[i / 2 % 2][i % 2]);
+                // Operands: a pair of rows during the pair before, a column of b after its last use.
+                const int q = n % T::kPair;
+                const int next_row = n / T::kPair * 2 + 2;
+                if (q < 2) {
+                    fa[next_row / 2 % 2][q] = next_row < RM ? read_fragment(cur, a_rd, next_row + q) : read_fragment(nxt, a_rd, q);
+                }
+                if (n >= T::kBarrier && n % 2 == 1) fb[j] = read_fragment(nxt, b_rd, j);
+                // Scales, ahead of their first use, behind the last one of what they replace and, being the stage's, ahead of its
+                // barrier: the first pair of rows' at the start, the others' once the pair before last is done; those of b in the
+                // first pair.
+#pragma unroll
+                for (int pair = 0; pair < RM / 2; ++pair) {
+                    if (n != (pair == 0 ? 0 : (pair - 1) * T::kPair + (T::kLag < T::kPair ? T::kLag : T::kPair - 1))) continue;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        sa[pair % 2][r] = *reinterpret_cast<const float*>(lds + cur + sa_rd + (2 * pair + r) * 64);
+                }
+                if constexpr (kByRow) {
+#pragma unroll
+                    for (int c = 0; c < RN; ++c)
+                        if (n == (2 * c + 1 + T::kLag < T::kPair ? 0 : T::kLag - 1))
+                            sb[c] = *reinterpret_cast<const f32x4*>(lds + cur + sb_rd + c * 64 + g * 16);
+                } else {
+                    if (n == 0) sb_next = *reinterpret_cast<const float*>(lds + cur + sb_rd);
+                    if (n == T::kLag - 1) sb[0] = sb_next;
+                }
+#pragma unroll
+                for (int d = 0; d < T::kLoads; ++d) {
+                    if (T::at(d) == n) load(d, kb + T::kSlots, cur);
+                    if (T::at(d) - T::kMfmas == n) load(d, kb + T::kSlots - 1, prv);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            prv = cur;
+            cur = nxt;
+        };
+        const int plain = !tail ? stages : stages < 2 ? 0 : stages - 2;
+        int kb = 0;
+        for (; kb < plain; ++kb) stage(kb, std::false_type{});
+        for (; kb < stages; ++kb) stage(kb, std::true_type{});
+#pragma unroll
+        for (int n = 0; n < T::kLag; ++n) {
+            constexpr int kFirst = T::kMfmas - T::kLag;
+            const int i = T::row(kFirst + n), j = T::col(kFirst + n);
+            add_scaled(acc[i][j], t[(kFirst + n) % T::kLag], sa[i / 2 % 2][i % 2] * sb[kByRow ? j : 0]);
+        }
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // the last loads write LDS
     __builtin_amdgcn_s_waitcnt(kLgkm0Imm);

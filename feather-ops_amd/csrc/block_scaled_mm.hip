@@ -59,16 +59,16 @@ BlockMmPlan few_rows_plan(int64_t M, int64_t N, int64_t K) {
 
 // A tile of the ring kernel: workgroups that share a CU's LDS, and microseconds fitted to 3300 timings of 115 shapes (33 to
 // 12288 rows, N and K 256 to 16384): a workgroup's start and end, and a stage with the CU full of workgroups and with one. The
-// tile and splits with the least estimate took at most 1.10 of the best pair's time on any of them, 1.009 in geometric mean.
+// tile and splits with the least estimate took at most 1.12 of the best pair's time on any of them, 1.005 in geometric mean.
 struct TileCost {
     BlockMmKernel kernel;
     int bm, bn, waves, per_cu;
     float fixed, full, alone;
 };
 constexpr TileCost kTiles[] = {
-    {kTile64x64, 64, 64, 2, 4, 2.60f, 1.058f, 0.350f},     {kTile64x128, 64, 128, 4, 2, 1.37f, 0.944f, 0.659f},
-    {kTile128x128, 128, 128, 8, 1, 1.69f, 0.662f, 0.662f}, {kTile256x128, 256, 128, 8, 1, 5.10f, 0.905f, 0.905f},
-    {kTile128x256, 128, 256, 8, 1, 2.55f, 1.103f, 1.103f}, {kTile256x256, 256, 256, 8, 1, 5.36f, 1.695f, 1.695f},
+    {kTile64x64, 64, 64, 2, 4, 2.48f, 1.578f, 0.350f},     {kTile64x128, 64, 128, 4, 2, 2.09f, 0.938f, 0.485f},
+    {kTile128x128, 128, 128, 8, 1, 1.70f, 0.715f, 0.715f}, {kTile256x128, 256, 128, 8, 1, 4.43f, 0.879f, 0.879f},
+    {kTile128x256, 128, 256, 8, 1, 2.78f, 1.144f, 1.144f}, {kTile256x256, 256, 256, 8, 1, 4.42f, 1.584f, 1.584f},
 };
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
 
@@ -92,7 +92,7 @@ BlockMmPlan tile_plan(int64_t M, int64_t N, int64_t K) {
             }
             cost = std::max(cost, memory);
             // the last of a tile's workgroups reads all of its sums back
-            if (splits > 1) cost += 1.56f + 1.14f / 65536.0f * static_cast<float>(splits * plan.tile_bytes);
+            if (splits > 1) cost += 0.88f + 1.44f / 65536.0f * static_cast<float>(splits * plan.tile_bytes);
             plan.cost = cost;
             if (best.cost == 0.0f || cost < best.cost) best = plan;
         }

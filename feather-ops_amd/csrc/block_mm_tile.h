@@ -45,6 +45,12 @@ struct BlockTile {
     static constexpr int kLag = 4;
     static constexpr int row(int n) { return n / kPair * 2 + (n + n / 2) % 2; }
     static constexpr int col(int n) { return n % kPair / 2; }
+    // The pair of rows whose scales are read after MFMA n, or -1: the first at the start, the others once the pair before
+    // last is done.
+    static constexpr int scales_at(int n) {
+        const int into = kLag < kPair ? kLag : kPair - 1;
+        return n == 0 ? 0 : n % kPair == into && n / kPair + 1 < RM / 2 ? n / kPair + 1 : -1;
+    }
     // The barrier that hands a slot over comes before the last pair. The refill's loads follow it, spread over kSpread / 8 of
     // a stage's MFMAs: load d after MFMA at(d), from kMfmas on in the next stage.
     static constexpr int kBarrier = kMfmas - kPair;
@@ -369,14 +375,11 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
                 }
                 if (n >= T::kBarrier && n % 2 == 1) fb[j] = read_fragment(nxt, b_rd, j);
                 // Scales, ahead of their first use, behind the last one of what they replace and, being the stage's, ahead of its
-                // barrier: the first pair of rows' at the start, the others' once the pair before last is done; those of b in the
-                // first pair.
-#pragma unroll
-                for (int pair = 0; pair < RM / 2; ++pair) {
-                    if (n != (pair == 0 ? 0 : (pair - 1) * T::kPair + (T::kLag < T::kPair ? T::kLag : T::kPair - 1))) continue;
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        sa[pair % 2][r] = *reinterpret_cast<const float*>(lds + cur + sa_rd + (2 * pair + r) * 64);
+                // barrier; those of b in the first pair.
+                const int pair = T::scales_at(n);
+                if (pair >= 0) {
+                    sa[pair % 2][0] = *reinterpret_cast<const float*>(lds + cur + sa_rd + pair * 128);
+                    sa[pair % 2][1] = *reinterpret_cast<const float*>(lds + cur + sa_rd + pair * 128 + 64);
                 }
                 if constexpr (kByRow) {
 #pragma unroll

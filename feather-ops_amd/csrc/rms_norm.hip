@@ -6,9 +6,12 @@
 //
 // Both directions are streams through memory: a row is read once into registers (pieces of 8 values a lane), its sums
 // are taken there, and what is written follows from the registers. Rows of up to 2048 values belong to one wave (sums
-// by DPP, no barrier), longer ones to the four waves of a workgroup (one LDS exchange; sixteen waves where there are no more
-// rows than CUs: one row of 14336 9.6 -> 5.6 us), and those past 16384 are read twice by one workgroup, the second time h as
-// it was just written.
+// by DPP, no barrier), longer ones to the four to sixteen waves of a workgroup (one LDS exchange; sixteen where there are no
+// more rows than CUs: one row of 14336 9.6 -> 5.5 us), and those past 16384 are read twice by one workgroup, the second time h
+// as it was just written.
+//
+// Measured against a copy's 4.96 TB/s (read and written): forward with fp8 output 4112 x 5120 fp16 30.0 us, 4.9 TB/s; backward
+// of 4096 x 4096 bf16 25 us, 5.4 TB/s, and 5 us for the weight's sums; one row of 4096 4.2 us, a launch's time.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -71,7 +74,7 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
         __syncthreads();
         v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kRowWaves; w += 2) v += lds[w] + lds[w + 1];
+        for (int w = 0; w < kRowWaves; ++w) v += lds[w];
     }
     return v;
 }
@@ -394,23 +397,41 @@ void by_type(int type, bool vec, F&& f) {
     else go(std::integral_constant<int, FEATHER_FP32>{});
 }
 
-// Calls f<waves per row, pieces per lane>() for rows of `cols` values (at most kRegisterCols).
-template <typename F>
+// Calls f<waves per row, pieces per lane>() for rows of `cols` values (at most kRegisterCols). Measured (us, 16-bit rows with a
+// residual): as many waves as two pieces a lane make instead of four with three to eight, forward: 4112 x 5120 30.9 -> 30.0,
+// 4096 x 8192 49.0 -> 47.0, 2048 x 12288 41.5 -> 34.9. The backward, which holds the next row too, has four waves up to 6144
+// columns (4112 x 5120 37 against 43), then two pieces (4096 x 8192 81 -> 62, 2048 x 12288 71 -> 50), and four past 12288,
+// where sixteen waves would leave a lane 128 registers (2048 x 16384 96).
+template <bool kBackward, typename F>
 void by_cols(int64_t rows, int64_t cols, F&& f) {
     using W1 = std::integral_constant<int, 1>;
     using W4 = std::integral_constant<int, kWaves>;
+    using W8 = std::integral_constant<int, 8>;
+    using W12 = std::integral_constant<int, 12>;
     using W16 = std::integral_constant<int, 16>;
     using P1 = std::integral_constant<int, 1>;
     using P2 = std::integral_constant<int, 2>;
+    using P3 = std::integral_constant<int, 3>;
+    using P4 = std::integral_constant<int, 4>;
     if (cols <= 512) f(W1{}, P1{});
     else if (cols <= 1024) f(W1{}, P2{});
-    else if (cols <= 2048) f(W1{}, std::integral_constant<int, 4>{});
+    else if (cols <= 2048) f(W1{}, P4{});
     else if (rows <= kFewRows && cols <= 8192) f(W16{}, P1{});
-    else if (rows <= kFewRows) f(W16{}, P2{});
     else if (cols <= 4096) f(W4{}, P2{});
-    else if (cols <= 6144) f(W4{}, std::integral_constant<int, 3>{});
-    else if (cols <= 8192) f(W4{}, std::integral_constant<int, 4>{});
-    else f(W4{}, std::integral_constant<int, 8>{});
+    else if constexpr (kBackward) {
+        if (cols <= 6144) f(W4{}, P3{});
+        else if (cols <= 8192) f(W8{}, P2{});
+        else if (cols <= 12288) f(W12{}, P2{});
+        else f(W8{}, P4{});
+    } else {
+        if (rows <= kFewRows) f(W16{}, P2{});
+        else if (cols <= 5120) f(std::integral_constant<int, 5>{}, P2{});
+        else if (cols <= 6144) f(std::integral_constant<int, 6>{}, P2{});
+        else if (cols <= 8192) f(W8{}, P2{});
+        else if (cols <= 10240) f(std::integral_constant<int, 10>{}, P2{});
+        else if (cols <= 12288) f(W12{}, P2{});
+        else f(W16{}, P2{});
+    }
 }
 
 }  // namespace
@@ -445,7 +466,7 @@ extern "C" bool feather_rms_norm(const void* x, int64_t ldx, const void* residua
             norm_kernel<t(), v(), kWaves, 0><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(p);
             return;
         }
-        by_cols(rows, cols, [&](auto waves, auto pieces) {
+        by_cols<false>(rows, cols, [&](auto waves, auto pieces) {
             norm_kernel<t(), v(), waves(), pieces()>
                 <<<static_cast<uint32_t>(groups), threads_of(waves()), 0, stream>>>(p);
         });
@@ -484,7 +505,7 @@ extern "C" bool feather_rms_norm_backward(const void* grad_y, int64_t ld_grad_y,
             long_weight_kernel<t(), v()><<<dim3(strips, groups), kThreads, 0, stream>>>(p);
             return;
         }
-        by_cols(rows, cols, [&](auto waves, auto pieces) {
+        by_cols<true>(rows, cols, [&](auto waves, auto pieces) {
             norm_backward_kernel<t(), v(), waves(), pieces()><<<groups, threads_of(waves()), 0, stream>>>(p);
         });
     });

@@ -136,7 +136,7 @@ class _Linear(torch.autograd.Function):
         ctx.save_for_backward(xt, xts, wt, wts, kept)
         ctx.e5m2, ctx.x_shape, ctx.x_dtype, ctx.weight_dtype = e5m2, x.shape, x.dtype, weight.dtype
         ctx.bias_dtype = bias.dtype if need_b else None
-        return y.reshape(*x.shape[:-1], y.shape[-1])
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
     @staticmethod
     @once_differentiable
@@ -149,7 +149,9 @@ class _Linear(torch.autograd.Function):
         if need_x:
             if weight is not None:
                 wt, wts = tiles(weight, ctx.e5m2, True, False, True, False)[2:4]
-            grad_x = block_scaled_mm(gq, gs, wt, wts, None, ctx.x_dtype).reshape(ctx.x_shape)
+            grad_x = block_scaled_mm(gq, gs, wt, wts, None, ctx.x_dtype)
+            if len(ctx.x_shape) != 2:
+                grad_x = grad_x.reshape(ctx.x_shape)
         if need_w:
             grad_w = block_scaled_mm(gt, gts, xt, xts, None, ctx.weight_dtype)
         if need_b:

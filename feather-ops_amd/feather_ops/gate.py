@@ -23,13 +23,15 @@ class _SiluMul(torch.autograd.Function):
         rows = as_rows(x)
         ctx.save_for_backward(rows)
         ctx.shape = x.shape
-        return torch.ops.feather_ops.silu_mul.default(rows).reshape(*x.shape[:-1], x.shape[-1] // 2)
+        y = torch.ops.feather_ops.silu_mul.default(rows)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], x.shape[-1] // 2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         rows, = ctx.saved_tensors
-        return torch.ops.feather_ops.silu_mul_backward.default(as_rows(grad), rows).reshape(ctx.shape)
+        grad_x = torch.ops.feather_ops.silu_mul_backward.default(as_rows(grad), rows)
+        return grad_x if len(ctx.shape) == 2 else grad_x.reshape(ctx.shape)
 
 
 def silu_mul(x: torch.Tensor) -> torch.Tensor:

@@ -31,12 +31,13 @@ class _RmsNorm(torch.autograd.Function):
             rows, weight, None if residual is None else as_rows(residual), eps, True)
         ctx.shape = x.shape
         ctx.set_materialize_grads(False)
+        if x.dim() != 2:   # a view costs a few microseconds of host time, with small tensors as much as a kernel
+            y, h = y.reshape(x.shape), h if residual is None else h.reshape(x.shape)
         if residual is None:
             ctx.save_for_backward(rows, weight, rstd)
-            return y.reshape(x.shape)
-        h = h.reshape(x.shape)
+            return y
         ctx.save_for_backward(h, weight, rstd)
-        return y.reshape(x.shape), h
+        return y, h
 
     @staticmethod
     @once_differentiable
@@ -47,7 +48,8 @@ class _RmsNorm(torch.autograd.Function):
             return grad_h if need_x else None, None, grad_h if need_residual else None, None
         grad, grad_w = torch.ops.feather_ops.rms_norm_backward.default(
             as_rows(grad_y), None if grad_h is None else as_rows(grad_h), as_rows(h), weight, rstd, need_w)
-        grad = grad.reshape(ctx.shape)
+        if len(ctx.shape) != 2:
+            grad = grad.reshape(ctx.shape)
         return grad if need_x else None, grad_w if need_w else None, grad if need_residual else None, None
 
 

@@ -414,7 +414,7 @@ __global__ __launch_bounds__(T::kThreads) void block_tile_kernel(const BlockMmPa
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // the last loads write LDS
     __builtin_amdgcn_s_waitcnt(kLgkm0Imm);
     barrier_only();
-    if (p.splits > 1 && !join_split<T::kWaves, RM, RN>(p, acc, tile, split, wave, lane)) return;
+    if (p.splits > 1 && !join_splits<T::kWaves, RM, RN>(p, acc, tile, split, wave, lane)) return;
     store_tile<RM, RN>(p, acc, m0 + wave_m * 16 * RM, n0 + wave_n * 16 * RN, lane,
                        reinterpret_cast<float*>(lds + wave * (16 * OutRow<RN>::kPitch * 4)));
 }

@@ -442,8 +442,8 @@ constexpr int kDeviceScope = 16;
 // The others return false and end. No wave ever waits for another workgroup, so the join cannot stall
 // whatever the dispatch order. Agent-scope fences would do instead of the coherent accesses, but they write
 // back and invalidate the whole L2 of the XCD under every co-resident workgroup (measured 1.5-2x slower).
-template <int kSlots, int RM, int RN, typename P>
-__device__ __forceinline__ bool join_split(const P& p, f32x4 (&acc)[RM][RN], int tile_id, int split, int slot_id,
+template <int kSlots, int RM, int RN>
+__device__ __forceinline__ bool join_split(const Params& p, f32x4 (&acc)[RM][RN], int tile_id, int split, int slot_id,
                                            int lane) {
     constexpr uint32_t kSlotBytes = RM * RN * kWave * 16;
     const rsrc_t part = make_rsrc(p.split_part, 0x7fffffffu);

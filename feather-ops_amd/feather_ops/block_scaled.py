@@ -109,7 +109,7 @@ def _codes(t: torch.Tensor, name: str) -> torch.Tensor:
     pitch, step = t.stride()
     if (step == 1 or cols <= 1) and t.storage_offset() % 16 == 0 and ((pitch % 16 == 0 and pitch >= cols) or rows <= 1):
         return t
-    out = torch.empty_strided((rows, cols), (-(-cols // 16) * 16, 1), dtype=t.dtype, device=t.device)
+    out = torch.empty_strided((rows, cols), (-(-cols // 64) * 64, 1), dtype=t.dtype, device=t.device)
     return out.copy_(t)
 
 
@@ -246,7 +246,7 @@ def _blocks(n: int) -> int:
 
 def _fake_codes(x: torch.Tensor, rows: int, cols: int, scale_rows: int, e5m2: bool) -> tuple[torch.Tensor, torch.Tensor]:
     dtype = torch.float8_e5m2 if e5m2 else torch.float8_e4m3fn
-    codes = torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=dtype, device=x.device)
+    codes = torch.empty_strided((rows, cols), ((cols + 63) // 64 * 64, 1), dtype=dtype, device=x.device)
     scale = torch.empty_strided((scale_rows, _blocks(cols)), (1, scale_rows), dtype=torch.float32, device=x.device)
     return codes, scale
 

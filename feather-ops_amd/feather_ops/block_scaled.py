@@ -4,7 +4,7 @@ reference, whose weights have one scale per tensor or column.
 A quantized matrix is a pair (codes, scale): fp8 codes `[rows, K]` and fp32 scales `[rows, ceil(K / 128)]`, one for each
 row and 128 columns, or `[ceil(rows / 128), ceil(K / 128)]`, one for each 128 x 128 square (weights). Codes times scales
 are the values; a block's scale is its largest magnitude (at least 2**-100) over the format's largest value. The functions
-here store rows of codes padded to 16 bytes and scales block by block (`scale.t()` is contiguous), which is what the
+here store rows of codes padded to 64 bytes and scales block by block (`scale.t()` is contiguous), which is what the
 product reads fastest; it takes any strides.
 
 Kernels: `csrc/block_scaled_mm.hip`, `csrc/quantize_tiles.hip`, `csrc/silu_mul.hip`. C ABI: `include/feather_block_ops.h`.

@@ -1,5 +1,7 @@
 // The streaming kernel of the block-scaled fp8 product, for few rows: both operands go from memory straight into registers,
-// and a workgroup's waves split K.
+// and a workgroup's waves split K. What bounds it is the reading of b: one row against 14336 x 4096 takes 14.2 us, against
+// 4096 x 14336 12.4, where reading the same rows in the same order and nothing else took 11.1-11.8, and in one linear run
+// 9.6-10.1. With more rows a's come from L2 once for each workgroup, which is why RN grows with them: 24 rows 16.2 and 16.6.
 #pragma once
 
 #include "block_mm_common.h"

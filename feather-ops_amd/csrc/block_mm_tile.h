@@ -6,14 +6,14 @@
 // which need 4 products more, are that much slower). Two waves a SIMD hide each other's LDS reads and barrier.
 //
 // What bounds the 256 x 256 tile is power: at 4096 x 16384 x 4096 a stage takes 2540 clocks where its MFMAs alone take 2048, but
-// the clock falls to 1.6 GHz on random operands (an MFMA stream alone: 2.0 GHz). Without the multiply-adds the product took 205
+// the clock falls to 1.6 GHz on random operands (an MFMA stream alone: 1.8-2.0 GHz). Without the multiply-adds the product took 205
 // us of 235, without LDS reads 168, without the loads 206, without the barrier 233; as many LDS reads again for half the
 // fragments cost 20 us. Rows of a instead of pairs, loads spread over 3 or 6 eighths of a stage, and raised wave priority
 // around the MFMAs were the same or slower; 4 x 2 waves of 64 x 128 368 us.
 //
 // Smaller tiles have the registers to read the next stage's fragments a stage ahead (kAhead: 128 x 128 tiles 3-4% faster, 64 x
-// 64 up to 8%, 64 x 128 even); they are bound by a stage's fixed costs: at 1024 x 4096 x 4096 a 128 x 128 stage takes 0.69 us, of
-// which the loads' issue is 0.23, the LDS reads 0.10 and the MFMAs 0.26.
+// 64 up to 8%, 64 x 128 even); they are bound by a stage's fixed costs: at 1024 x 4096 x 4096 a 128 x 128 stage took 0.69 us,
+// without its loads 0.46 and without its LDS reads too 0.41, where the MFMAs alone are 0.26 by their clocks.
 #pragma once
 
 #include "block_mm_common.h"

@@ -135,7 +135,7 @@ constexpr float kLaunchCost = 2.0f;   // us from the end of one launch to the ne
 
 // Large products go in up to four launches where whole rounds of tiles end at a column or row and the rest does better on
 // other tiles: 4096 x 14336 by 256 x 256 tiles is 3.5 rounds of the 256 CUs and takes 4; 12288 columns are 3, and the other
-// 2048 are one round of 128 x 256 (K = 4096: 234 us in one launch, 219 in two). Cuts fall on multiples of 256 and are
+// 2048 are one round of 128 x 256 (K = 4096: 234 us in one launch, 224 in two). Cuts fall on multiples of 256 and are
 // tried where a number of whole rounds of each tile ends, along either axis; a part may be cut once more.
 Parts cut(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, int depth) {
     const BlockMmPlan whole = whole_plan(M, N, K);

@@ -6,6 +6,9 @@
 // lane then walks two neighbouring columns over 32 rows (one LDS word a row, lanes on consecutive words: no conflicts).
 // The four waves' quarters of a column meet in LDS for its largest value and its sum, in wave order; its codes pass through
 // LDS once more to leave as whole lines.
+//
+// Memory bounds it, once the transposed stores are whole lines: bf16 4096 x 12288 in both directions 42.7 us, 4.8 TB/s, as
+// squares in both 38.4 (58 with scattered stores and branching loads).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

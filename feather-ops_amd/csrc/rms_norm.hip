@@ -10,8 +10,8 @@
 // more rows than CUs: one row of 14336 9.6 -> 5.5 us), and those past 16384 are read twice by one workgroup, the second time h
 // as it was just written.
 //
-// Measured against a copy's 4.96 TB/s (read and written): forward with fp8 output 4112 x 5120 fp16 30.0 us, 4.9 TB/s; backward
-// of 4096 x 4096 bf16 25 us, 5.4 TB/s, and 5 us for the weight's sums; one row of 4096 4.2 us, a launch's time.
+// Measured against a copy's 4.96 TB/s (read and written): forward with fp8 output 4112 x 5120 fp16 28.6 us, 5.1 TB/s; backward
+// of 4096 x 4096 bf16 25 us, 5.4 TB/s, and 4 us for the weight's sums; one row of 4096 2.9 us, a launch's time.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

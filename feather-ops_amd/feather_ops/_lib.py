@@ -1,4 +1,5 @@
-"""Loading of the native code: `_C` (the torch library) and, through it, `libfeather_ops_gfx950.so`.
+"""Loading of the native code: `_C` (the torch library), through it `libfeather_ops_gfx950.so`, and `_autograd.so` (the
+autograd nodes of its ops).
 
 There is no fallback: if the extension is not built, importing `feather_ops` fails with the build
 command, and the ops only have a CUDA (HIP) dispatch key, so CPU tensors are rejected by the dispatcher.
@@ -7,22 +8,28 @@ command, and the ops only have a CUDA (HIP) dispatch key, so CPU tensors are rej
 import ctypes
 import pathlib
 
+import torch
+
 HERE = pathlib.Path(__file__).resolve().parent
 LIBRARY = HERE / "libfeather_ops_gfx950.so"
 EXTENSION = HERE / "_C.so"
+AUTOGRAD = HERE / "_autograd.so"
 BUILD_HINT = "build it with `make -C feather-ops_amd -j8` or `python -c 'import __graft_entry__ as g; g.build()'`"
 
 _loaded = False
 
 
 def load() -> None:
-    """Import `_C`, which registers `torch.ops.feather_ops.*` and loads the HIP library."""
+    """Import `_C`, which registers `torch.ops.feather_ops.*` and loads the HIP library, and load `_autograd.so`."""
     global _loaded
     if _loaded:
         return
-    if not EXTENSION.exists() or not LIBRARY.exists():
-        raise ImportError(f"feather_ops native extension missing ({EXTENSION.name}, {LIBRARY.name}): {BUILD_HINT}")
+    if not EXTENSION.exists() or not LIBRARY.exists() or not AUTOGRAD.exists():
+        raise ImportError(f"feather_ops native extension missing ({EXTENSION.name}, {LIBRARY.name}, {AUTOGRAD.name}): "
+                          f"{BUILD_HINT}")
     from . import _C  # noqa: F401  registers the feather_ops torch library
+
+    torch.ops.load_library(str(AUTOGRAD))
 
     _loaded = True
 

@@ -1,11 +1,10 @@
 """Gated activation `silu(gate) * up`, in 16 bits, fp32 or fp8 with a scale for each block of 128; not in the reference.
-Kernels: `csrc/silu_mul.hip`.
+Kernels: `csrc/silu_mul.hip`; autograd node: `csrc/block_autograd.cpp`.
 
 x holds gate and up side by side, `[..., 2 F]`, as one projection of both gives them.
 """
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .block_scaled import _TYPES, _fake_codes, _is_e5m2, _plain, as_rows
 
@@ -17,31 +16,12 @@ def _checked(x: torch.Tensor) -> None:
         raise ValueError(f"x must have an even last dimension (gate and up side by side), got {tuple(x.shape)}")
 
 
-class _SiluMul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x):
-        rows = as_rows(x)
-        ctx.save_for_backward(rows)
-        ctx.shape = x.shape
-        y = torch.ops.feather_ops.silu_mul.default(rows)
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], x.shape[-1] // 2)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        rows, = ctx.saved_tensors
-        grad_x = torch.ops.feather_ops.silu_mul_backward.default(as_rows(grad), rows)
-        return grad_x if len(ctx.shape) == 2 else grad_x.reshape(ctx.shape)
-
-
 def silu_mul(x: torch.Tensor) -> torch.Tensor:
     """`silu(x[..., :F]) * x[..., F:]` in x's dtype (bfloat16, float16 or float32), computed in fp32 and rounded once.
-    Differentiable."""
+    Differentiable once."""
     _checked(x)
     if x.numel() == 0:
         return x[..., : x.shape[-1] // 2] * 1
-    if x.requires_grad and torch.is_grad_enabled():
-        return _SiluMul.apply(x)
     y = torch.ops.feather_ops.silu_mul.default(as_rows(x))
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 

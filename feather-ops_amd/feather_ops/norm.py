@@ -1,5 +1,5 @@
 """Root-mean-square norm with the residual's addition, in 16 bits, fp32 or fp8 with a scale for each block of 128; not in
-the reference. Kernels: `csrc/rms_norm.hip`.
+the reference. Kernels: `csrc/rms_norm.hip`; autograd node: `csrc/block_autograd.cpp`.
 
     h = x + residual (in x's dtype)    y = h / sqrt(mean(h^2) + eps) * weight
 
@@ -8,7 +8,6 @@ and everything after it is fp32 until y is rounded once.
 """
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .block_scaled import _TYPES, _fake_codes, _is_e5m2, _plain, as_rows
 
@@ -23,40 +22,10 @@ def _checked(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
                          f"{tuple(x.shape)} {x.dtype}")
 
 
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        rows = as_rows(x)
-        y, h, rstd = torch.ops.feather_ops.rms_norm.default(
-            rows, weight, None if residual is None else as_rows(residual), eps, True)
-        ctx.shape = x.shape
-        ctx.set_materialize_grads(False)
-        if x.dim() != 2:   # a view costs a few microseconds of host time, with small tensors as much as a kernel
-            y, h = y.reshape(x.shape), h if residual is None else h.reshape(x.shape)
-        if residual is None:
-            ctx.save_for_backward(rows, weight, rstd)
-            return y
-        ctx.save_for_backward(h, weight, rstd)
-        return y, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y, grad_h=None):
-        h, weight, rstd = ctx.saved_tensors
-        need_x, need_w, need_residual = ctx.needs_input_grad[:3]
-        if grad_y is None:   # only h was used further on
-            return grad_h if need_x else None, None, grad_h if need_residual else None, None
-        grad, grad_w = torch.ops.feather_ops.rms_norm_backward.default(
-            as_rows(grad_y), None if grad_h is None else as_rows(grad_h), as_rows(h), weight, rstd, need_w)
-        if len(ctx.shape) != 2:
-            grad = grad.reshape(ctx.shape)
-        return grad if need_x else None, grad_w if need_w else None, grad if need_residual else None, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
              eps: float = 1e-6) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """y in x's dtype, or (y, h) with a residual; x `[..., D]` in bfloat16, float16 or float32, weight `[D]` in x's dtype
-    or float32. Differentiable in x, weight and residual, through y and h."""
+    or float32. Differentiable once, in x, weight and residual, through y and h."""
     _checked(x, weight, residual)
     if x.numel() == 0:
         h = x if residual is None else x + residual
@@ -64,12 +33,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
         return y if residual is None else (y, h)
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, weight, residual, eps)
     y, h, _ = torch.ops.feather_ops.rms_norm.default(as_rows(x), weight,
                                                      None if residual is None else as_rows(residual), eps, False)
-    if x.dim() != 2:
+    if x.dim() != 2:   # a view costs a few microseconds of host time, with small tensors as much as a kernel
         y = y.reshape(x.shape)
         h = h if residual is None else h.reshape(x.shape)
     return y if residual is None else (y, h)

@@ -3,9 +3,9 @@
 The reference installs the same package name with setuptools and a torch CUDAExtension
 (`setup.py:132-145` there). Here the native code is built by this directory's Makefile, which the
 build_py step runs before copying the package: `feather_ops/libfeather_ops_gfx950.so` (the HIP kernels and
-the C ABI of include/feather_ops.h) and `feather_ops/_C.so` (the torch library, which finds the former
-through its $ORIGIN run path). Both ship inside the package, so an installed `import feather_ops` loads
-the installed native code. The build needs the repository's `include/` next to this directory, hipcc and
+the C ABI of include/feather_ops.h), `feather_ops/_C.so` (the torch library, which finds the former
+through its $ORIGIN run path) and `feather_ops/_autograd.so` (autograd nodes of its ops). All ship inside the
+package, so an installed `import feather_ops` loads the installed native code. The build needs the repository's `include/` next to this directory, hipcc and
 the ROCm torch it links against; it is a platform wheel (gfx950 code objects, a CPython-linked extension).
 """
 
@@ -18,7 +18,7 @@ from setuptools.command.build_py import build_py
 from setuptools.dist import Distribution
 
 HERE = pathlib.Path(__file__).resolve().parent
-NATIVE = ["libfeather_ops_gfx950.so", "_C.so"]
+NATIVE = ["libfeather_ops_gfx950.so", "_C.so", "_autograd.so"]
 
 
 class MakeThenBuildPy(build_py):

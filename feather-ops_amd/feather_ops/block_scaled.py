@@ -7,7 +7,8 @@ are the values; a block's scale is its largest magnitude (at least 2**-100) over
 here store rows of codes padded to 64 bytes and scales block by block (`scale.t()` is contiguous), which is what the
 product reads fastest; it takes any strides.
 
-Kernels: `csrc/block_scaled_mm.hip`, `csrc/quantize_tiles.hip`, `csrc/silu_mul.hip`. C ABI: `include/feather_block_ops.h`.
+Kernels: `csrc/block_scaled_mm.hip`, `csrc/quantize_tiles.hip`, `csrc/silu_mul.hip`; the layer and its
+autograd node: `csrc/block_autograd.cpp`. C ABI: `include/feather_block_ops.h`.
 """
 
 import functools
@@ -16,7 +17,6 @@ from collections.abc import Callable
 import torch
 from torch import nn
 from torch._subclasses.fake_tensor import FakeTensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .modules import relabel_modules
@@ -130,49 +130,10 @@ def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_s
                                                          _workspace(a, need) if need else None)
 
 
-class _Linear(torch.autograd.Function):
-    """y = x @ w^T + bias in fp8: x and w quantized by rows and by squares; dx = dy @ w and dw = dy^T @ x with dy, dy^T and
-    x^T quantized by rows, and w^T by the same squares. What is kept for the backward is fp8."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, dtype, weight_fp8, weight_scale):
-        e5m2 = _is_e5m2(dtype)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        tiles = torch.ops.feather_ops.quantize_tiles.default
-        rows = as_rows(x)
-        xq, xs, xt, xts, _ = tiles(rows, e5m2, False, True, need_w, False)
-        wt = wts = None
-        if weight_fp8 is None:
-            weight_fp8, weight_scale, wt, wts, _ = tiles(weight, e5m2, True, True, need_x, False)
-        y = block_scaled_mm(xq, xs, weight_fp8, weight_scale, bias, x.dtype)
-        if not need_w:
-            xt = xts = None
-        # A weight quantized before the call is not kept transposed: the backward quantizes it again.
-        kept = weight if need_x and wt is None else None
-        ctx.save_for_backward(xt, xts, wt, wts, kept)
-        ctx.e5m2, ctx.x_shape, ctx.x_dtype, ctx.weight_dtype = e5m2, x.shape, x.dtype, weight.dtype
-        ctx.bias_dtype = bias.dtype if need_b else None
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        xt, xts, wt, wts, weight = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        tiles = torch.ops.feather_ops.quantize_tiles.default
-        gq, gs, gt, gts, sums = tiles(as_rows(grad), ctx.e5m2, False, need_x, need_w, need_b)
-        grad_x = grad_w = grad_b = None
-        if need_x:
-            if weight is not None:
-                wt, wts = tiles(weight, ctx.e5m2, True, False, True, False)[2:4]
-            grad_x = block_scaled_mm(gq, gs, wt, wts, None, ctx.x_dtype)
-            if len(ctx.x_shape) != 2:
-                grad_x = grad_x.reshape(ctx.x_shape)
-        if need_w:
-            grad_w = block_scaled_mm(gt, gts, xt, xts, None, ctx.weight_dtype)
-        if need_b:
-            grad_b = torch.ops.feather_ops.sum_rows.default(sums, _TYPES[ctx.bias_dtype])
-        return grad_x, grad_w, grad_b, None, None, None
+@functools.lru_cache(maxsize=4096)
+def _train_workspace_bytes(M: int, N: int, K: int) -> int:
+    """For a layer's product and those of its gradients."""
+    return max(_workspace_bytes(M, N, K), _workspace_bytes(M, K, N), _workspace_bytes(N, K, M))
 
 
 def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -181,7 +142,7 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     """`x @ weight^T + bias` in fp8 with a scale for each block of 128: x `[..., K]`, weight `[N, K]`, y `[..., N]` in x's
     dtype (bfloat16, float16 or float32).
 
-    Differentiable in x, weight and bias: the gradients are products of fp8 operands too, each quantized along the axis it
+    Differentiable once, in x, weight and bias: the gradients are products of fp8 operands too, each quantized along the axis it
     is summed over (dx and dw are the exact gradients of the product but for that rounding, with the quantization itself
     taken as the identity). Weight and activations are quantized on every call; `quantized_weight`, the result of
     `quantize_blocks(weight, dtype, square=True)`, saves that for a weight that does not change. bias is taken in x's
@@ -195,12 +156,13 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     if x.numel() == 0 or weight.numel() == 0:
         return nn.functional.linear(x, weight.to(x.dtype), bias)
     codes, scale = quantized_weight if quantized_weight is not None else (None, None)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        return _Linear.apply(x, as_rows(weight), bias, dtype, codes, scale)
-    if codes is None:
-        codes, scale = quantize_blocks(weight, dtype, square=True)
-    xq, xs = torch.ops.feather_ops.quantize_blocks.default(as_rows(x), _FP8[dtype])
-    y = block_scaled_mm(xq, xs, codes, scale, bias, x.dtype)
+    if codes is not None:
+        codes = _codes(codes, "the weight's codes")
+    rows, weight = as_rows(x), as_rows(weight)
+    trains = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    need = (_train_workspace_bytes if trains else _workspace_bytes)(rows.shape[0], *weight.shape)
+    y = torch.ops.feather_ops.block_scaled_linear.default(rows, weight, bias, _FP8[dtype], codes, scale,
+                                                          _workspace(rows, need) if need else None)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
 

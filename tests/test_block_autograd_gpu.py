@@ -92,3 +92,73 @@ def test_accumulation_and_reuse(leaves):
         assert torch.equal(leaf.grad, grad + grad)
     with pytest.raises(RuntimeError, match="second time"):
         y.backward(plain)
+
+
+def _layer(m, n, k, seed=8):
+    g = torch.Generator("cpu").manual_seed(seed)
+    return [torch.randn(shape, generator=g).to(torch.bfloat16).cuda().requires_grad_() for shape in ((m, k), (n, k), (n,))]
+
+
+def test_layer_second_derivatives_are_refused(cuda_device):
+    args = _layer(20, 64, 256)
+    first = torch.autograd.grad(fo.block_scaled_linear(*args).float().square().sum(), args, create_graph=True)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        torch.autograd.grad(sum(grad.float().sum() for grad in first), args)
+
+
+def test_layer_with_and_without_a_graph(cuda_device):
+    x, w, b = _layer(20, 64, 256)
+    with torch.no_grad():
+        want = fo.block_scaled_linear(x, w, b)
+    assert want.grad_fn is None and torch.equal(fo.block_scaled_linear(x, w, b), want)
+    with torch.inference_mode():
+        assert torch.equal(fo.block_scaled_linear(x.detach(), w.detach(), b.detach()), want)
+    codes = fo.quantize_blocks(w, square=True)
+    assert torch.equal(fo.block_scaled_linear(x, w, b, quantized_weight=codes), want)
+    assert torch.equal(fo.block_scaled_linear(x.detach(), w.detach(), b.detach(), quantized_weight=codes), want)
+    with pytest.raises(RuntimeError, match="go together"):
+        torch.ops.feather_ops.block_scaled_linear(x, w, b, False, codes[0], None, None)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_layer_captured(cuda_device, apart):
+    """A training pass in one graph, and forward and backward in two that share their memory; with split products. Replays
+    with new inputs, eager passes between them."""
+    from feather_ops import block_scaled
+
+    m, n, k = 64, 256, 4096
+    assert block_scaled._train_workspace_bytes(m, n, k) > 0
+    x, w, b = _layer(m, n, k)
+    gy = torch.randn(m, n, generator=torch.Generator("cpu").manual_seed(9)).to(torch.bfloat16).cuda()
+
+    def eager():
+        y = fo.block_scaled_linear(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), gy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph()]
+    if apart:
+        graphs.append(torch.cuda.CUDAGraph())
+        pool = torch.cuda.graph_pool_handle()
+        with torch.cuda.graph(graphs[0], pool=pool, stream=side):
+            y = fo.block_scaled_linear(x, w, b)
+        with torch.cuda.graph(graphs[1], pool=pool, stream=side):
+            grads = torch.autograd.grad(y, (x, w, b), gy)
+    else:
+        with torch.cuda.graph(graphs[0], stream=side):
+            y = fo.block_scaled_linear(x, w, b)
+            grads = torch.autograd.grad(y, (x, w, b), gy)
+    for replay in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(m, k, generator=torch.Generator("cpu").manual_seed(10 + replay)).to(torch.bfloat16))
+            gy.copy_(torch.randn(m, n, generator=torch.Generator("cpu").manual_seed(20 + replay)).to(torch.bfloat16))
+        want = eager()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for got, expected in zip((y.detach(), *grads), want):
+            assert torch.equal(got, expected), replay

@@ -125,7 +125,7 @@ def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_s
     a, b = _codes(a, "a"), _codes(b, "b")
     m, k = a.shape
     n = b.shape[0]
-    need = _workspace_bytes(m, n, k)
+    need = _workspace_bytes(int(m), int(n), int(k))   # int: the plan of a traced call fixes its sizes
     return torch.ops.feather_ops.block_scaled_mm.default(a, a_scale, b, b_scale, bias, out_type,
                                                          _workspace(a, need) if need else None)
 
@@ -160,7 +160,7 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
         codes = _codes(codes, "the weight's codes")
     rows, weight = as_rows(x), as_rows(weight)
     trains = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
-    need = (_train_workspace_bytes if trains else _workspace_bytes)(rows.shape[0], *weight.shape)
+    need = (_train_workspace_bytes if trains else _workspace_bytes)(int(rows.shape[0]), *map(int, weight.shape))
     y = torch.ops.feather_ops.block_scaled_linear.default(rows, weight, bias, _FP8[dtype], codes, scale,
                                                           _workspace(rows, need) if need else None)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])

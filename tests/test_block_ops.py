@@ -173,3 +173,20 @@ def test_relabelling_leaves_trained_layers_to_each_pass():
     assert not hasattr(model[0], "weight_fp8") and set(model.state_dict()) == keys
     with pytest.raises(ValueError, match="fp8 dtype"):
         fo.to_block_scaled_linear(model, torch.float16)
+
+
+def test_tracing_with_symbolic_sizes():
+    """Sizes that the tracer makes symbolic: each call goes into the graph; a product's own are fixed by its plan."""
+    def empty(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype)
+
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    for call, args, want in (
+            (fo.block_scaled_mm, (empty(20, 256, dtype=f8), empty(20, 2, dtype=f32), empty(64, 256, dtype=f8),
+                                  empty(1, 2, dtype=f32)), 1),
+            (fo.block_scaled_linear, (empty(2, 20, 256), empty(64, 256), empty(64)), 3),
+            (fo.quantize_blocks, (empty(3, 20, 256),), 1), (fo.rms_norm, (empty(3, 20, 256), empty(256)), 1),
+            (fo.rms_norm_quantized, (empty(3, 20, 256), empty(256)), 1), (fo.silu_mul, (empty(3, 20, 256),), 1),
+            (fo.silu_mul_quantized, (empty(3, 20, 256),), 1)):
+        graph = make_fx(lambda *a: call(*a), tracing_mode="symbolic")(*args).graph
+        assert len([n for n in graph.nodes if "feather_ops" in str(n.target)]) == want, call

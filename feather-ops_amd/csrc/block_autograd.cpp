@@ -171,6 +171,16 @@ std::optional<Tensor> workspace_of(const c10::IValue& kept) {
     return own;
 }
 
+// A gradient that cannot be differentiated, as the graph's node for it.
+struct Refuse : public Function<Refuse> {
+    static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&) { return grad.alias(); }
+
+    static variable_list backward(AutogradContext*, const variable_list&) {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "second derivatives of block_scaled_linear are not implemented");
+        return {};
+    }
+};
+
 // y = x w^T + bias in fp8: x and w quantized by rows and by squares; dx = dy w and dw = dy^T x with dy, dy^T and x^T quantized
 // by rows, and w^T by the same squares. What is kept for the backward is fp8.
 struct Linear : public Function<Linear> {
@@ -209,6 +219,8 @@ struct Linear : public Function<Linear> {
         const bool e5m2 = ctx->saved_data["e5m2"].toBool();
         const int64_t x_type = ctx->saved_data["x_type"].toInt();
         const variable_list saved = ctx->get_saved_variables();
+        const bool twice = at::GradMode::is_enabled() && grads[0].requires_grad();
+        const at::NoGradGuard once;
         const std::optional<Tensor> workspace = workspace_of(ctx->saved_data["workspace"]);
         const auto [gq, gs, gt, gts, sums] = quantize_tiles(as_rows(grads[0]), e5m2, false, need_x, need_w, need_b);
         Tensor grad_x, grad_w, grad_b;
@@ -225,6 +237,11 @@ struct Linear : public Function<Linear> {
         if (need_w)
             grad_w = block_scaled_mm(gt, gts, saved[0], saved[1], std::nullopt, ctx->saved_data["w_type"].toInt(), workspace);
         if (need_b) grad_b = sum_rows(sums, x_type);
+        if (twice) {
+            const at::AutoGradMode graph(true);
+            for (Tensor* grad : {&grad_x, &grad_w, &grad_b})
+                if (grad->defined()) *grad = Refuse::apply(*grad, grads[0]);
+        }
         return {grad_x, grad_w, grad_b, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
@@ -260,7 +277,4 @@ TORCH_LIBRARY_IMPL(feather_ops, AutogradCUDA, m) {
     // A gradient of a gradient is refused with an error.
     m.impl("silu_mul_backward", torch::autograd::autogradNotImplementedFallback());
     m.impl("rms_norm_backward", torch::autograd::autogradNotImplementedFallback());
-    m.impl("quantize_tiles", torch::autograd::autogradNotImplementedFallback());
-    m.impl("sum_rows", torch::autograd::autogradNotImplementedFallback());
-    m.impl("block_scaled_mm", torch::autograd::autogradNotImplementedFallback());
 }

@@ -10,6 +10,8 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/inductor/aoti_torch/c/shim.h>
 #include <torch/library.h>
 
@@ -17,8 +19,10 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <memory>
 #include <optional>
 #include <tuple>
+#include <utility>
 
 namespace {
 
@@ -174,15 +178,16 @@ std::optional<Tensor> workspace_of(const c10::IValue& kept) {
     return own;
 }
 
-// A gradient that cannot be differentiated, as the graph's node for it.
-struct Refuse : public Function<Refuse> {
-    static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&) { return grad.alias(); }
-
-    static variable_list backward(AutogradContext*, const variable_list&) {
-        TORCH_CHECK_NOT_IMPLEMENTED(false, "second derivatives of block_scaled_linear are not implemented");
-        return {};
-    }
-};
+// Makes `grad` depend on what it was computed from, by way of a node that refuses to go on: the gradient that came in and an
+// operand, by the edge that the layer's node has to it (the operand itself is not kept, its fp8 copies are).
+void refuse_second(Tensor& grad, const Tensor& grad_y, const torch::autograd::Edge& operand) {
+    torch::autograd::edge_list from;
+    if (grad_y.requires_grad()) from.push_back(torch::autograd::impl::gradient_edge(grad_y));
+    if (operand.is_valid()) from.push_back(operand);
+    if (!grad.defined() || from.empty()) return;
+    torch::autograd::set_history(grad, std::make_shared<torch::autograd::Error>(
+                                           "second derivatives of block_scaled_linear are not implemented", std::move(from)));
+}
 
 // y = x w^T + bias in fp8: x and w quantized by rows and by squares; dx = dy w and dw = dy^T x with dy, dy^T and x^T quantized
 // by rows, and w^T by the same squares. What is kept for the backward is fp8.
@@ -222,7 +227,7 @@ struct Linear : public Function<Linear> {
         const bool e5m2 = ctx->saved_data["e5m2"].toBool();
         const int64_t x_type = ctx->saved_data["x_type"].toInt();
         const variable_list saved = ctx->get_saved_variables();
-        const bool twice = at::GradMode::is_enabled() && grads[0].requires_grad();
+        const bool twice = at::GradMode::is_enabled();
         const at::NoGradGuard once;
         const std::optional<Tensor> workspace = workspace_of(ctx->saved_data["workspace"]);
         const auto [gq, gs, gt, gts, sums] = quantize_tiles(as_rows(grads[0]), e5m2, false, need_x, need_w, need_b);
@@ -240,10 +245,12 @@ struct Linear : public Function<Linear> {
         if (need_w)
             grad_w = block_scaled_mm(gt, gts, saved[0], saved[1], std::nullopt, ctx->saved_data["w_type"].toInt(), workspace);
         if (need_b) grad_b = sum_rows(sums, x_type);
-        if (twice) {
-            const at::AutoGradMode graph(true);
-            for (Tensor* grad : {&grad_x, &grad_w, &grad_b})
-                if (grad->defined()) *grad = Refuse::apply(*grad, grads[0]);
+        if (twice) {   // dx depends on the weight, dW on x, all three on dy
+            const auto node = torch::autograd::get_current_node();
+            TORCH_CHECK(node, "block_scaled_linear: its backward runs outside of its node");
+            refuse_second(grad_x, grads[0], node->next_edge(1));
+            refuse_second(grad_w, grads[0], node->next_edge(0));
+            refuse_second(grad_b, grads[0], {});
         }
         return {grad_x, grad_w, grad_b, Tensor(), Tensor(), Tensor(), Tensor()};
     }

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <memory>
 #include <optional>
 #include <tuple>
@@ -100,6 +101,14 @@ Tensor as_rows(const Tensor& t) {
 
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 
+// Forward mode has no formulas here: an operand's tangent is refused, with and without a graph, and never dropped. (Under a
+// transform the op is called once more for each level, with that level's tangents.)
+void refuse_tangents(const char* name, std::initializer_list<std::optional<Tensor>> operands) {
+    for (const auto& t : operands)
+        TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "forward-mode derivatives of ", name,
+                                    " are not implemented");
+}
+
 struct SiluMul : public Function<SiluMul> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x) {
         const at::AutoDispatchBelowADInplaceOrView below;
@@ -114,6 +123,7 @@ struct SiluMul : public Function<SiluMul> {
 };
 
 Tensor silu_mul_autograd(const Tensor& x) {
+    refuse_tangents("silu_mul", {x});
     if (at::GradMode::is_enabled() && wants_grad(x)) return SiluMul::apply(x);
     const at::AutoDispatchBelowADInplaceOrView below;
     return silu_mul(x);
@@ -150,6 +160,7 @@ struct RmsNorm : public Function<RmsNorm> {
 
 Norm rms_norm_autograd(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& residual, double eps,
                        bool need_rstd) {
+    refuse_tangents("rms_norm", {x, weight, residual});
     if (at::GradMode::is_enabled() &&
         (wants_grad(x) || wants_grad(weight) || (residual.has_value() && wants_grad(*residual)))) {
         const variable_list out = RmsNorm::apply(x, weight, residual, eps);
@@ -227,6 +238,7 @@ struct Linear : public Function<Linear> {
         const bool e5m2 = ctx->saved_data["e5m2"].toBool();
         const int64_t x_type = ctx->saved_data["x_type"].toInt();
         const variable_list saved = ctx->get_saved_variables();
+        refuse_tangents("block_scaled_linear", {grads[0]});
         const bool twice = at::GradMode::is_enabled();
         const at::NoGradGuard once;
         const std::optional<Tensor> workspace = workspace_of(ctx->saved_data["workspace"]);
@@ -262,6 +274,7 @@ Tensor block_scaled_linear(const Tensor& x, const Tensor& weight, const std::opt
                            const std::optional<Tensor>& weight_codes, const std::optional<Tensor>& weight_scale,
                            const std::optional<Tensor>& workspace) {
     TORCH_CHECK(weight_codes.has_value() == weight_scale.has_value(), "codes and scale of the weight go together");
+    refuse_tangents("block_scaled_linear", {x, weight, bias});
     if (at::GradMode::is_enabled() &&
         (wants_grad(x) || wants_grad(weight) || (bias.has_value() && wants_grad(*bias))))
         return Linear::apply(x, weight, bias, e5m2, weight_codes, weight_scale, workspace);

@@ -18,7 +18,7 @@ def _checked(x: torch.Tensor) -> None:
 
 def silu_mul(x: torch.Tensor) -> torch.Tensor:
     """`silu(x[..., :F]) * x[..., F:]` in x's dtype (bfloat16, float16 or float32), computed in fp32 and rounded once.
-    Differentiable once."""
+    Differentiable once, in reverse mode."""
     _checked(x)
     if x.numel() == 0:
         return x[..., : x.shape[-1] // 2] * 1

@@ -25,7 +25,7 @@ def _checked(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
              eps: float = 1e-6) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """y in x's dtype, or (y, h) with a residual; x `[..., D]` in bfloat16, float16 or float32, weight `[D]` in x's dtype
-    or float32. Differentiable once, in x, weight and residual, through y and h."""
+    or float32. Differentiable once, in reverse mode, in x, weight and residual, through y and h."""
     _checked(x, weight, residual)
     if x.numel() == 0:
         h = x if residual is None else x + residual

@@ -3,6 +3,8 @@ They are refused, never left out of a sum."""
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 
 import feather_ops as fo
 
@@ -89,3 +91,47 @@ def test_first_gradients_with_a_graph_have_the_same_values(plain_ops, leaves):
     for again in kept:
         with pytest.raises(RuntimeError, match="not implemented"):
             torch.autograd.grad(again.sum(), grad, retain_graph=True)
+
+
+# ---- forward mode ----
+
+
+def _entry_points(x, w, b):
+    norm = w[0]
+    return {"silu_mul": lambda x=x: fo.silu_mul(x), "silu_mul batch": lambda x=x: fo.silu_mul(x[None]),
+            "rms_norm": lambda x=x: fo.rms_norm(x, norm), "rms_norm weight": lambda x=norm: fo.rms_norm(b, x),
+            "rms_norm residual": lambda x=x: fo.rms_norm(w[:M], norm, x),
+            "linear": lambda x=x: fo.block_scaled_linear(x, w), "linear weight": lambda x=w: fo.block_scaled_linear(b, x),
+            "linear bias": lambda x=norm[:N]: fo.block_scaled_linear(b, w, x)}
+
+
+NAMES = ["silu_mul", "silu_mul batch", "rms_norm", "rms_norm weight", "rms_norm residual", "linear", "linear weight",
+         "linear bias"]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name, graph):
+    """A dual tensor's tangent, of any operand, with and without a gradient beside it and outside of grad mode."""
+    with FakeTensorMode():
+        x, w, b = (torch.empty(shape, dtype=torch.bfloat16, device="cuda") for shape in ((M, K), (N, K), (M, K)))
+        call = _entry_points(x, w, b)[name]
+        primal, = call.__defaults__
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(primal.clone().requires_grad_(graph), torch.empty_like(primal))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+            call()
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (primal,), (torch.empty_like(primal),))
+
+
+def test_tangent_of_the_layers_gradient_is_refused(plain_ops, leaves):
+    y = fo.block_scaled_linear(*leaves)
+    with forward_ad.dual_level():
+        grad = forward_ad.make_dual(torch.ones(M, N), torch.ones(M, N))
+        for inputs in (leaves, leaves[0], leaves[2]):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, inputs, grad, retain_graph=True)

@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import feather_ops as fo
 
@@ -28,3 +29,20 @@ def test_gradient_penalty_on_the_last_layer(leaves):
     plain = torch.autograd.grad(fo.block_scaled_linear(x, w, b).sum(), leaves)
     kept = torch.autograd.grad(fo.block_scaled_linear(x, w, b).sum(), leaves, create_graph=True)
     assert all(torch.equal(a, c) for a, c in zip(plain, kept))
+
+
+def test_forward_mode_is_refused(leaves):
+    x, w, b = (leaf.detach() for leaf in leaves)
+    calls = {"silu_mul": fo.silu_mul, "rms_norm": lambda t: fo.rms_norm(t, w[0]),
+             "block_scaled_linear": lambda t: fo.block_scaled_linear(t, w, b)}
+    for name, call in calls.items():
+        with pytest.raises(NotImplementedError, match=f"forward-mode derivatives of {name}"):
+            torch.func.jvp(call, (x,), (x,))
+        leaf = x.clone().requires_grad_()
+        y = call(leaf)
+        with forward_ad.dual_level():
+            for tensor in (x, leaf):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(forward_ad.make_dual(tensor, x))
+            with pytest.raises(RuntimeError, match="forward"):   # the tangent of a gradient that comes in
+                torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))

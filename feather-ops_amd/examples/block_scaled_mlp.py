@@ -44,9 +44,9 @@ class BlockScaledMLP(nn.Module):
             y, h = fo.rms_norm(x, self.norm, residual, self.eps)
             return self.down(fo.silu_mul(self.gate_up(y))), h
         codes, scale, h = fo.rms_norm_quantized(x, self.norm, residual, self.eps)
-        gate_up = fo.block_scaled_mm(codes, scale, self.gate_up.weight_fp8, self.gate_up.weight_scale, None, x.dtype)
+        gate_up = fo.block_scaled_mm(codes, scale, *self.gate_up.quantized_weight(), None, x.dtype)
         codes, scale = fo.silu_mul_quantized(gate_up)
-        return fo.block_scaled_mm(codes, scale, self.down.weight_fp8, self.down.weight_scale, None, x.dtype), h
+        return fo.block_scaled_mm(codes, scale, *self.down.quantized_weight(), None, x.dtype), h
 
 
 def reference(mlp: BlockScaledMLP, x: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:

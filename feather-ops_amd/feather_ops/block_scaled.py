@@ -12,6 +12,7 @@ autograd node: `csrc/block_autograd.cpp`. C ABI: `include/feather_block_ops.h`.
 """
 
 import functools
+import weakref
 from collections.abc import Callable
 
 import torch
@@ -166,23 +167,66 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
 
+class _Source:
+    """The weight that codes were taken of, and its state then."""
+
+    __slots__ = ("weight", "address", "version")
+
+    def __init__(self, weight: torch.Tensor | None) -> None:
+        self.weight = None if weight is None else weakref.ref(weight)
+        self.address, self.version = (None, None) if weight is None else self._state(weight)
+
+    @staticmethod
+    def _state(weight: torch.Tensor) -> tuple[int, int | None]:
+        address = 0 if isinstance(weight, FakeTensor) else weight.data_ptr()
+        return address, None if weight.is_inference() else weight._version   # inference tensors do not count their changes
+
+    def is_still(self, weight: torch.Tensor) -> bool:
+        return self.weight is not None and self.weight() is weight and (self.address, self.version) == self._state(weight)
+
+    def __reduce__(self) -> tuple:   # copied or stored: of no weight
+        return _Source, (None,)
+
+
 class BlockScaledLinear:
     """Mixin for `nn.Linear` (via `relabel_modules`): `forward` is `block_scaled_linear`, 16-bit (or fp32) in and out.
 
     A frozen weight (`requires_grad` False) is quantized once, by `quantize_weight_` (which `to_block_scaled_linear`
-    calls), into two non-persistent buffers, `weight_fp8` and `weight_scale`; call it again after changing the weight. A
-    weight that takes gradients is quantized on every pass. Parameters and `state_dict` stay as they were."""
+    calls), into two non-persistent buffers, `weight_fp8` and `weight_scale`. A pass that finds the weight changed
+    (`load_state_dict`, a step of training, another parameter in its place) quantizes it into them again, so a captured
+    graph follows when the layer is next called or `quantize_weight_` is; what a layer that is itself being captured or
+    traced finds changed is quantized in that pass alone. Only writes through `weight.data`, which torch does not count,
+    and those to a weight made in inference mode need a call of `quantize_weight_`. A weight that takes gradients is
+    quantized on every pass. Parameters and `state_dict` stay as they were."""
 
     def quantize_weight_(self, fp8_dtype: torch.dtype = torch.float8_e4m3fn) -> None:
         codes, scale = quantize_blocks(self.weight, fp8_dtype, square=True)
-        self.register_buffer("weight_fp8", codes, persistent=False)
-        self.register_buffer("weight_scale", scale, persistent=False)
+        kept = self._buffers.get("weight_fp8")
+        if (kept is not None and kept.dtype == codes.dtype and kept.shape == codes.shape and kept.device == codes.device
+                and (torch.is_inference_mode_enabled() or not kept.is_inference())):
+            kept.copy_(codes)   # in place, for graphs that read them
+            self.weight_scale.copy_(scale)
+        else:
+            self.register_buffer("weight_fp8", codes, persistent=False)
+            self.register_buffer("weight_scale", scale, persistent=False)
         self._fp8_dtype = fp8_dtype
+        self._codes_of = _Source(self.weight)
+
+    def quantized_weight(self) -> tuple[torch.Tensor, torch.Tensor] | None:
+        """The kept codes and scales of a frozen weight, brought up to date; None where every pass quantizes it."""
+        weight = self.weight
+        if weight.requires_grad or "weight_fp8" not in self._buffers:
+            return None
+        if not torch.compiler.is_compiling() and not self._codes_of.is_still(weight):
+            if (not isinstance(weight, nn.Parameter) or torch._C._len_torch_dispatch_stack()
+                    or (weight.is_cuda and torch.cuda.is_current_stream_capturing())):
+                return None
+            self.quantize_weight_(self._fp8_dtype)
+        return self.weight_fp8, self.weight_scale
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        frozen = not self.weight.requires_grad and hasattr(self, "weight_fp8")
         return block_scaled_linear(x, self.weight, self.bias, getattr(self, "_fp8_dtype", torch.float8_e4m3fn),
-                                   quantized_weight=(self.weight_fp8, self.weight_scale) if frozen else None)
+                                   quantized_weight=self.quantized_weight())
 
 
 def to_block_scaled_linear(root: nn.Module, fp8_dtype: torch.dtype = torch.float8_e4m3fn,

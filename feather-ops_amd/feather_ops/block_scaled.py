@@ -156,11 +156,16 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
         bias = bias.to(x.dtype)
     if x.numel() == 0 or weight.numel() == 0:
         return nn.functional.linear(x, weight.to(x.dtype), bias)
-    codes, scale = quantized_weight if quantized_weight is not None else (None, None)
-    if codes is not None:
-        codes = _codes(codes, "the weight's codes")
     rows, weight = as_rows(x), as_rows(weight)
     trains = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    codes, scale = quantized_weight if quantized_weight is not None else (None, None)
+    if codes is not None:
+        # the backward takes the weight itself, in squares of dtype
+        if (codes.shape != weight.shape or codes.dtype != dtype
+                or (trains and scale.shape != _square_shape(weight.shape))):
+            raise ValueError(f"quantized_weight must be the weight's {tuple(weight.shape)} in squares of {dtype}, got codes "
+                             f"{tuple(codes.shape)} {codes.dtype} and scales {tuple(scale.shape)}")
+        codes = _codes(codes, "the weight's codes")
     need = (_train_workspace_bytes if trains else _workspace_bytes)(int(rows.shape[0]), *map(int, weight.shape))
     y = torch.ops.feather_ops.block_scaled_linear.default(rows, weight, bias, _FP8[dtype], codes, scale,
                                                           _workspace(rows, need) if need else None)

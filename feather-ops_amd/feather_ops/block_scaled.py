@@ -12,7 +12,6 @@ autograd node: `csrc/block_autograd.cpp`. C ABI: `include/feather_block_ops.h`.
 """
 
 import functools
-import weakref
 from collections.abc import Callable
 
 import torch
@@ -178,7 +177,7 @@ class _Source:
     __slots__ = ("weight", "address", "version")
 
     def __init__(self, weight: torch.Tensor | None) -> None:
-        self.weight = None if weight is None else weakref.ref(weight)
+        self.weight = weight   # not a weak reference: torch swaps no tensor that has one
         self.address, self.version = (None, None) if weight is None else self._state(weight)
 
     @staticmethod
@@ -187,7 +186,7 @@ class _Source:
         return address, None if weight.is_inference() else weight._version   # inference tensors do not count their changes
 
     def is_still(self, weight: torch.Tensor) -> bool:
-        return self.weight is not None and self.weight() is weight and (self.address, self.version) == self._state(weight)
+        return self.weight is weight and (self.address, self.version) == self._state(weight)
 
     def __reduce__(self) -> tuple:   # copied or stored: of no weight
         return _Source, (None,)
@@ -216,6 +215,25 @@ class BlockScaledLinear:
             self.register_buffer("weight_scale", scale, persistent=False)
         self._fp8_dtype = fp8_dtype
         self._codes_of = _Source(self.weight)
+
+    def register_parameter(self, name: str, param: nn.Parameter | None) -> None:
+        super().register_parameter(name, param)
+        if name == "weight":   # another one: what its codes were of is let go
+            self._codes_of = _Source(None)
+
+    def _apply(self, fn: Callable[[torch.Tensor], torch.Tensor], recurse: bool = True) -> nn.Module:
+        """To another device or type (`to`, `half`, ...), which the weight takes, and codes and scales do not: they are taken
+        of the weight as it is then, or (off the GPU, where they wait for the way back) moved."""
+        kept = [self._buffers.pop(name, None) for name in ("weight_fp8", "weight_scale")]
+        super()._apply(fn, recurse)
+        if kept[0] is not None:
+            if self.weight.is_cuda:
+                self.quantize_weight_(self._fp8_dtype)
+            else:
+                for name, buffer in zip(("weight_fp8", "weight_scale"), kept):
+                    self.register_buffer(name, buffer.to(self.weight.device), persistent=False)
+                self._codes_of = _Source(None)
+        return self
 
     def quantized_weight(self) -> tuple[torch.Tensor, torch.Tensor] | None:
         """The kept codes and scales of a frozen weight, brought up to date; None where every pass quantizes it."""

@@ -1,5 +1,4 @@
-"""Codes that are passed to block_scaled_linear beside the weight, and layers that move to another type or device; under fake
-tensors."""
+"""Codes that are passed to block_scaled_linear beside the weight, under fake tensors."""
 
 import pytest
 import torch

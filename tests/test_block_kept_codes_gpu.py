@@ -144,3 +144,29 @@ def test_inference_mode(layer):
         assert _is_current(made)
     _double(layer)
     assert _is_current(layer) and _is_current(layer)
+
+
+@pytest.mark.parametrize("swap", [False, True])
+@pytest.mark.parametrize("move", [lambda m: m.half(), lambda m: m.to(torch.float32), lambda m: m.float().bfloat16(),
+                                  lambda m: m.to("cuda"), lambda m: torch.nn.Sequential(m).float()[0].half(),
+                                  lambda m: m.cpu().cuda(), lambda m: m.cpu().half().cuda()])
+def test_in_another_type_or_on_another_device(layer, move, swap):
+    """Codes stay fp8 and scales fp32, and are those of the weight in its new type."""
+    before = torch.__future__.get_swap_module_params_on_conversion()
+    torch.__future__.set_swap_module_params_on_conversion(swap)
+    try:
+        moved = move(layer)
+    finally:
+        torch.__future__.set_swap_module_params_on_conversion(before)
+    assert moved is layer and layer.weight_fp8.dtype == torch.float8_e4m3fn and layer.weight_scale.dtype == torch.float32
+    assert layer.weight_fp8.is_cuda and layer.weight_scale.is_cuda and not layer.weight.requires_grad
+    assert _is_current(layer, _x().to(layer.weight.dtype))
+
+
+def test_format_is_kept(layer):
+    layer.quantize_weight_(torch.float8_e5m2)
+    layer.cpu()
+    assert {t.device.type for t in (layer.weight, layer.weight_fp8, layer.weight_scale)} == {"cpu"}
+    layer.half().cuda()
+    assert layer.weight_fp8.dtype == torch.float8_e5m2
+    assert torch.equal(layer(_x().half()), fo.block_scaled_linear(_x().half(), layer.weight, layer.bias, torch.float8_e5m2))

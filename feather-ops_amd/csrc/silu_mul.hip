@@ -44,6 +44,12 @@ __device__ __forceinline__ float sigmoid(float g) {
     return g < 0.0f ? t * q : q;
 }
 
+// a b c for |c| <= 1 without a step that leaves the range where the product does not: the larger of a and b takes c.
+__device__ __forceinline__ float product(float a, float b, float c) {
+    const bool first = fabsf(a) > fabsf(b);
+    return (first ? a : b) * c * (first ? b : a);
+}
+
 template <Op kOp, int kType, bool kVec>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsParams p) {
     // The workgroup's first piece as (row, piece of it), then this lane's from there in 32 bits.
@@ -70,8 +76,10 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsParams p) {
 #pragma unroll
             for (int i = 0; i < kPiece; ++i) {
                 const float s = sigmoid(v[i]);
-                const float grad_up = g[i] * v[i] * s;
-                v[i] = g[i] * up[i] * s * (1.0f + v[i] * (1.0f - s));
+                // v s first: of a gate masked with the type's lowest value it is 0, and grad_y v may be infinite. 13.8 million
+                // gradients in cache, 21.5 us with products from the left, take 21.8 so.
+                const float grad_up = g[i] * (v[i] * s);
+                v[i] = 2.0f * product(g[i], up[i], s * (0.5f + v[i] * (0.5f - 0.5f * s)));   // silu's slope is at most 1.1
                 up[i] = grad_up;
             }
             void* out = static_cast<uint8_t*>(p.y) + row * p.ldy * type_bytes(kType);

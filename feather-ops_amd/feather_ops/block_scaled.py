@@ -101,16 +101,29 @@ def _workspace(a: torch.Tensor, nbytes: int) -> torch.Tensor:
     return _workspace_for(a, nbytes)
 
 
+# The C ABI's limits of the strides from row to row (from square to square).
+_FAR_CODES = 1 << 22
+_FAR_SCALES = 1 << 20
+
+
 def _codes(t: torch.Tensor, name: str) -> torch.Tensor:
-    """Codes as the product reads them: rows on 16-byte boundaries (copied where they are not)."""
+    """Codes as the product reads them: rows on 16-byte boundaries, at most _FAR_CODES apart (copied where they are not)."""
     if t.dim() != 2:
         raise ValueError(f"{name} must be a matrix, got {t.dim()} dimensions")
     rows, cols = t.shape
     pitch, step = t.stride()
-    if (step == 1 or cols <= 1) and t.storage_offset() % 16 == 0 and ((pitch % 16 == 0 and pitch >= cols) or rows <= 1):
+    if (step == 1 or cols <= 1) and t.storage_offset() % 16 == 0 and (
+            (pitch % 16 == 0 and cols <= pitch <= _FAR_CODES) or rows <= 1):
         return t
     out = torch.empty_strided((rows, cols), (-(-cols // 64) * 64, 1), dtype=t.dtype, device=t.device)
     return out.copy_(t)
+
+
+def _scales(t: torch.Tensor) -> torch.Tensor:
+    """Scales as the product reads them: rows at most _FAR_SCALES apart (copied where they are not)."""
+    if t.dim() != 2 or t.shape[0] <= 1 or t.stride(0) <= _FAR_SCALES:
+        return t
+    return torch.empty_strided(t.shape, (1, t.shape[0]), dtype=t.dtype, device=t.device).copy_(t)
 
 
 def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -119,10 +132,11 @@ def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_s
 
     a_scale is `[M, ceil(K / 128)]`; b_scale `[ceil(N / 128), ceil(K / 128)]` or, one for each row of b,
     `[N, ceil(K / 128)]`. Each operand has its own fp8 format. bias: `[N]` in out_dtype. Sums are fp32 (each block's on the
-    matrix cores, then times its scales), the result is rounded once. Codes whose rows do not start on 16-byte boundaries
-    are copied first: keep weights as `quantize_blocks` lays them out. Not differentiable (`block_scaled_linear` is)."""
+    matrix cores, then times its scales), the result is rounded once. Codes whose rows do not start on 16-byte boundaries,
+    or are over 4 MiB apart, and scales whose rows are over 2**20 apart are copied first: keep weights as `quantize_blocks`
+    lays them out. K is at most 2**22. Not differentiable (`block_scaled_linear` is)."""
     out_type = _type_number(out_dtype)
-    a, b = _codes(a, "a"), _codes(b, "b")
+    a, b, a_scale, b_scale = _codes(a, "a"), _codes(b, "b"), _scales(a_scale), _scales(b_scale)
     m, k = a.shape
     n = b.shape[0]
     need = _workspace_bytes(int(m), int(n), int(k))   # int: the plan of a traced call fixes its sizes
@@ -164,7 +178,7 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
                 or (trains and scale.shape != _square_shape(weight.shape))):
             raise ValueError(f"quantized_weight must be the weight's {tuple(weight.shape)} in squares of {dtype}, got codes "
                              f"{tuple(codes.shape)} {codes.dtype} and scales {tuple(scale.shape)}")
-        codes = _codes(codes, "the weight's codes")
+        codes, scale = _codes(codes, "the weight's codes"), _scales(scale)
     need = (_train_workspace_bytes if trains else _workspace_bytes)(int(rows.shape[0]), *map(int, weight.shape))
     y = torch.ops.feather_ops.block_scaled_linear.default(rows, weight, bias, _FP8[dtype], codes, scale,
                                                           _workspace(rows, need) if need else None)

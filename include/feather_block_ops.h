@@ -16,8 +16,9 @@
  *
  * Every function enqueues on `stream` and returns true, or returns false and enqueues nothing where its contract is not
  * met; launch errors are left to the caller (hipGetLastError). Strides are in elements and may exceed a row. No function
- * allocates, synchronizes or keeps anything between calls. Sizes: rows, columns and strides under 2^31, each row under
- * 2 GiB; a whole matrix may be larger than 4 GiB.
+ * allocates, synchronizes or keeps anything between calls (but for each thread's memory of which kernels a product's shape
+ * goes to). Sizes: rows under 2^31, columns and row strides under 2^29 (the product's own limits stand at it); a whole matrix
+ * may be larger than 4 GiB.
  */
 #ifndef FEATHER_BLOCK_OPS_H
 #define FEATHER_BLOCK_OPS_H
@@ -41,7 +42,8 @@ enum { FEATHER_BF16 = 0, FEATHER_FP16 = 1, FEATHER_FP32 = 2 };
  * in fp32, which costs about 1.5e-5 of a result (2-norm, random operands); whole numbers within those bits are exact.
  *
  *   a, b      [M, K] and [N, K] fp8 codes, each of its own format; row strides lda and ldb, multiples of 16 up to 2^22;
- *             16-byte aligned. Bytes between K and the next row are not used (up to 3 of them are read where K % 4 != 0).
+ *             16-byte aligned. Bytes between K and the next row are not used, but read: up to the end of a piece of 16, behind
+ *             the last row of the matrix up to 3 (where K % 4 != 0).
  *   a_scale   fp32 [M, ceil(K / 128)]: element (m, k) at m * a_scale_row + k * a_scale_block. Block-major (a_scale_row = 1,
  *             what the functions below write) is the layout that reads fastest. Strides from row to row (for b: from
  *             square to square) are 0 .. 2^20, those from block to block not negative.
@@ -53,7 +55,7 @@ enum { FEATHER_BF16 = 0, FEATHER_FP16 = 1, FEATHER_FP32 = 2 };
  *             is 0. As feather_scaled_mm_splitk's: its first 64 KiB all zero before its first use, left zero by every call;
  *             calls that share it must be ordered.
  *
- * M, N >= 1 and K >= 0 (K = 0: c is the bias, or zero). Deterministic: the same operands give the same bits.
+ * 1 <= M, N < 2^29, ceil(M / 64) * ceil(N / 16) < 2^27, 0 <= K <= 2^22 (K = 0: c is the bias, or zero). Deterministic: the same operands give the same bits.
  */
 bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5m2, const float* a_scale, int64_t a_scale_row,
                              int64_t a_scale_block, const uint8_t* b, int64_t ldb, bool b_e5m2, const float* b_scale,

@@ -7,6 +7,7 @@
 
 #include "block_mm_common.h"
 #include "block_mm_launch.h"
+#include "feather_internal.h"
 
 namespace feather {
 namespace {
@@ -200,6 +201,17 @@ using namespace feather;
 
 extern "C" int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     return sizes_ok(M, N, K) ? workspace_bytes_of(parts_of(M, N, K)) : -1;
+}
+
+extern "C" int feather_block_scaled_mm_launches(int64_t M, int64_t N, int64_t K, int64_t out[16]) {
+    if (!sizes_ok(M, N, K)) return 0;
+    const Parts& parts = parts_of(M, N, K);
+    for (int i = 0; i < parts.count; ++i) {
+        const Part& part = parts.part[i];
+        const int64_t launch[4] = {part.plan.kernel, part.plan.splits, part.M, part.N};
+        std::copy(launch, launch + 4, out + 4 * i);
+    }
+    return parts.count;
 }
 
 extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5m2, const float* a_scale,

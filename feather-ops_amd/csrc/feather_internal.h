@@ -1,5 +1,5 @@
-// Entry points of libfeather_ops_gfx950.so that only this package's torch library calls (extension.cpp); the public C
-// ABI is include/feather_ops.h.
+// Entry points of libfeather_ops_gfx950.so that only this package calls (extension.cpp) or its tests; the public C ABI is
+// include/feather_ops.h and include/feather_block_ops.h.
 #ifndef FEATHER_INTERNAL_H
 #define FEATHER_INTERNAL_H
 
@@ -62,6 +62,13 @@ bool feather_prepack_rows(const uint8_t* w, uint8_t* out, int64_t N, int64_t K, 
  */
 bool feather_quantize_rows(const void* w, int source, uint8_t* out, float* scale, uint32_t* amax, int64_t N, int64_t K,
                            bool use_fp8_e5m2, bool per_row, hipStream_t stream);
+
+/*
+ * What feather_block_scaled_mm launches for a shape (host only), for tests that mean to reach every kernel: the number of
+ * launches (at most 4; 0 outside the contract), and of each the kernel (BlockMmKernel of block_mm_launch.h), the K ranges and
+ * the rows and columns, four numbers a launch.
+ */
+int feather_block_scaled_mm_launches(int64_t M, int64_t N, int64_t K, int64_t out[16]);
 
 }  // extern "C"
 

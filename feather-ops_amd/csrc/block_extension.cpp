@@ -4,6 +4,7 @@
 // line more (4096 x 5000 x 2576: rows of 2576 bytes 76 us, 2624 68, 2688 67; 16 x 5000 x 2576: 7.1, 6.7, 8.3). Scales are
 // stored block by block ([blocks, rows], handed out as its transpose). Outputs that a call does not ask for come back empty.
 #include <torch/csrc/stable/library.h>
+#include <torch/csrc/stable/ops.h>
 
 #include <cstdint>
 #include <optional>
@@ -108,9 +109,14 @@ const float* floats(const Tensor& t) { return static_cast<const float*>(t.const_
 float* floats(Tensor& t) { return static_cast<float*>(t.mutable_data_ptr()); }
 uint8_t* bytes(Tensor& t) { return static_cast<uint8_t*>(t.mutable_data_ptr()); }
 
+// Scales whose rows are at most 2^20 apart, as the product takes them: copied where they are not.
+Tensor near_rows(const Tensor& scale) {
+    return scale.size(0) > 1 && scale.stride(0) > (1 << 20) ? torch::stable::contiguous(scale) : scale;
+}
+
 // feather_ops::block_scaled_mm (feather_block_scaled_mm); out_type: 0 bfloat16, 1 float16, 2 float32. workspace: uint8,
 // as scaled_mm_splitk's, where the shape needs one.
-Tensor block_scaled_mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
+Tensor block_scaled_mm(const Tensor& a, Tensor a_scale, const Tensor& b, Tensor b_scale,
                        const std::optional<Tensor>& bias, const int64_t out_type, std::optional<Tensor> workspace) {
     STD_TORCH_CHECK(a.is_cuda() && b.is_cuda() && a_scale.is_cuda() && b_scale.is_cuda(),
                     "a, b and their scales must be CUDA tensors");
@@ -140,9 +146,10 @@ Tensor block_scaled_mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, 
                     "b_scale must be [", blocks_of(N), ", ", kb, "], one scale for each 128 x 128 block of b, or [", N,
                     ", ", kb, "], one for each row and block of 128 columns");
     const bool by_row = b_scale.size(0) != blocks_of(N);
+    a_scale = near_rows(a_scale);
+    b_scale = near_rows(b_scale);
     const int64_t as_row = a_scale.size(0) > 1 ? a_scale.stride(0) : 0;
     const int64_t bs_row = b_scale.size(0) > 1 ? b_scale.stride(0) : 0;
-    STD_TORCH_CHECK(as_row <= (1 << 20) && bs_row <= (1 << 20), "the scales' rows are too far apart");
     STD_TORCH_CHECK(out_type >= 0 && out_type <= 2, "the output must be bfloat16, float16 or float32");
     const int type = static_cast<int>(out_type);
     if (bias.has_value()) {

@@ -101,9 +101,8 @@ def _workspace(a: torch.Tensor, nbytes: int) -> torch.Tensor:
     return _workspace_for(a, nbytes)
 
 
-# The C ABI's limits of the strides from row to row (from square to square).
+# The C ABI's limit of the stride from row to row.
 _FAR_CODES = 1 << 22
-_FAR_SCALES = 1 << 20
 
 
 def _codes(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -119,13 +118,6 @@ def _codes(t: torch.Tensor, name: str) -> torch.Tensor:
     return out.copy_(t)
 
 
-def _scales(t: torch.Tensor) -> torch.Tensor:
-    """Scales as the product reads them: rows at most _FAR_SCALES apart (copied where they are not)."""
-    if t.dim() != 2 or t.shape[0] <= 1 or t.stride(0) <= _FAR_SCALES:
-        return t
-    return torch.empty_strided(t.shape, (1, t.shape[0]), dtype=t.dtype, device=t.device).copy_(t)
-
-
 def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
                     bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """`(a * a_scale) @ (b * b_scale)^T + bias` for quantized a `[M, K]` and b `[N, K]`: `[M, N]` in out_dtype.
@@ -136,7 +128,14 @@ def block_scaled_mm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_s
     or are over 4 MiB apart, and scales whose rows are over 2**20 apart are copied first: keep weights as `quantize_blocks`
     lays them out. K is at most 2**22. Not differentiable (`block_scaled_linear` is)."""
     out_type = _type_number(out_dtype)
-    a, b, a_scale, b_scale = _codes(a, "a"), _codes(b, "b"), _scales(a_scale), _scales(b_scale)
+    if torch.compiler.is_compiling():
+        return _block_scaled_mm_auto(a, a_scale, b, b_scale, bias, out_type)
+    return _product(a, a_scale, b, b_scale, bias, out_type)
+
+
+def _product(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, bias: torch.Tensor | None,
+             out_type: int) -> torch.Tensor:
+    a, b = _codes(a, "a"), _codes(b, "b")
     m, k = a.shape
     n = b.shape[0]
     need = _workspace_bytes(int(m), int(n), int(k))   # int: the plan of a traced call fixes its sizes
@@ -161,6 +160,13 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     taken as the identity). Weight and activations are quantized on every call; `quantized_weight`, the result of
     `quantize_blocks(weight, dtype, square=True)`, saves that for a weight that does not change. bias is taken in x's
     dtype."""
+    return _checked_linear(x, weight, bias, dtype, quantized_weight, _UNKNOWN)
+
+
+def _checked_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, dtype: torch.dtype,
+                    quantized_weight: tuple[torch.Tensor, torch.Tensor] | None, source: tuple[int, int]) -> torch.Tensor:
+    """block_scaled_linear; source: which state of the weight the codes are of (_Source), for a traced program's passes to
+    see for themselves."""
     _type_number(x.dtype)
     _is_e5m2(dtype)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
@@ -169,7 +175,6 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
         bias = bias.to(x.dtype)
     if x.numel() == 0 or weight.numel() == 0:
         return nn.functional.linear(x, weight.to(x.dtype), bias)
-    rows, weight = as_rows(x), as_rows(weight)
     trains = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
     codes, scale = quantized_weight if quantized_weight is not None else (None, None)
     if codes is not None:
@@ -178,29 +183,37 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
                 or (trains and scale.shape != _square_shape(weight.shape))):
             raise ValueError(f"quantized_weight must be the weight's {tuple(weight.shape)} in squares of {dtype}, got codes "
                              f"{tuple(codes.shape)} {codes.dtype} and scales {tuple(scale.shape)}")
-        codes, scale = _codes(codes, "the weight's codes"), _scales(scale)
+    if torch.compiler.is_compiling():
+        return _block_scaled_linear_auto(x, weight, bias, _FP8[dtype], codes, scale, *source)
+    return _linear(x, weight, bias, _FP8[dtype], codes, scale, trains)
+
+
+def _linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, e5m2: bool, codes: torch.Tensor | None,
+            scale: torch.Tensor | None, trains: bool) -> torch.Tensor:
+    rows, weight = as_rows(x), as_rows(weight)
+    if codes is not None:
+        codes = _codes(codes, "the weight's codes")
     need = (_train_workspace_bytes if trains else _workspace_bytes)(int(rows.shape[0]), *map(int, weight.shape))
-    y = torch.ops.feather_ops.block_scaled_linear.default(rows, weight, bias, _FP8[dtype], codes, scale,
+    y = torch.ops.feather_ops.block_scaled_linear.default(rows, weight, bias, e5m2, codes, scale,
                                                           _workspace(rows, need) if need else None)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+# The state of a weight that is not known, or that has none: inference tensors do not count their changes.
+_UNKNOWN = (0, -1)
+
+
+def _state_of(weight: torch.Tensor) -> tuple[int, int]:
+    """(address, version) of a weight: one of them is another after every change that torch sees."""
+    return 0 if isinstance(weight, FakeTensor) else weight.data_ptr(), -1 if weight.is_inference() else weight._version
 
 
 class _Source:
     """The weight that codes were taken of, and its state then."""
 
-    __slots__ = ("weight", "address", "version")
-
     def __init__(self, weight: torch.Tensor | None) -> None:
         self.weight = weight   # not a weak reference: torch swaps no tensor that has one
-        self.address, self.version = (None, None) if weight is None else self._state(weight)
-
-    @staticmethod
-    def _state(weight: torch.Tensor) -> tuple[int, int | None]:
-        address = 0 if isinstance(weight, FakeTensor) else weight.data_ptr()
-        return address, None if weight.is_inference() else weight._version   # inference tensors do not count their changes
-
-    def is_still(self, weight: torch.Tensor) -> bool:
-        return self.weight is weight and (self.address, self.version) == self._state(weight)
+        self.state = _UNKNOWN if weight is None else _state_of(weight)
 
     def __reduce__(self) -> tuple:   # copied or stored: of no weight
         return _Source, (None,)
@@ -250,20 +263,29 @@ class BlockScaledLinear:
         return self
 
     def quantized_weight(self) -> tuple[torch.Tensor, torch.Tensor] | None:
-        """The kept codes and scales of a frozen weight, brought up to date; None where every pass quantizes it."""
-        weight = self.weight
-        if weight.requires_grad or "weight_fp8" not in self._buffers:
+        """The kept codes and scales of a frozen weight, brought up to date; None where every pass quantizes it. In a program
+        that torch.compile traces they are not looked at: the layer's own node does that."""
+        return self._kept_codes(self.weight)
+
+    def _kept_codes(self, weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor] | None:
+        if weight.requires_grad or self._buffers.get("weight_fp8") is None:
             return None
-        if not torch.compiler.is_compiling() and not self._codes_of.is_still(weight):
+        source = self._codes_of
+        if torch.compiler.is_compiling():
+            if source.weight is None or not isinstance(weight, nn.Parameter):
+                return None
+        elif source.weight is not weight or source.state != _state_of(weight):
             if (not isinstance(weight, nn.Parameter) or torch._C._len_torch_dispatch_stack()
                     or (weight.is_cuda and torch.cuda.is_current_stream_capturing())):
                 return None
             self.quantize_weight_(self._fp8_dtype)
-        return self.weight_fp8, self.weight_scale
+        return self._buffers["weight_fp8"], self._buffers["weight_scale"]
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return block_scaled_linear(x, self.weight, self.bias, getattr(self, "_fp8_dtype", torch.float8_e4m3fn),
-                                   quantized_weight=self.quantized_weight())
+        weight = self.weight
+        codes = self._kept_codes(weight)
+        return _checked_linear(x, weight, self.bias, self.__dict__.get("_fp8_dtype", torch.float8_e4m3fn), codes,
+                               _UNKNOWN if codes is None else self._codes_of.state)
 
 
 def to_block_scaled_linear(root: nn.Module, fp8_dtype: torch.dtype = torch.float8_e4m3fn,
@@ -278,6 +300,82 @@ def to_block_scaled_linear(root: nn.Module, fp8_dtype: torch.dtype = torch.float
             if not module.weight.requires_grad:
                 module.quantize_weight_(fp8_dtype)
     return count
+
+
+# ---- one node each under torch.compile ----
+
+
+@torch.library.custom_op("feather_ops::block_scaled_mm_auto", mutates_args=())
+def _block_scaled_mm_auto(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+                          bias: torch.Tensor | None, out_type: int) -> torch.Tensor:
+    """block_scaled_mm as one opaque op: neither the copies of what lies off the kernels' boundaries nor the workspace are
+    traced."""
+    return _product(a, a_scale, b, b_scale, bias, out_type)
+
+
+@_block_scaled_mm_auto.register_fake
+def _(a, a_scale, b, b_scale, bias, out_type):
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=_DTYPE_OF[out_type])
+
+
+@torch.library.custom_op("feather_ops::block_scaled_linear_auto", mutates_args=())
+def _block_scaled_linear_auto(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, e5m2: bool,
+                              codes: torch.Tensor | None, scale: torch.Tensor | None, address: int,
+                              version: int) -> torch.Tensor:
+    """block_scaled_linear as one opaque op. The weight's codes are taken if it is as they were taken of it, as far as that is
+    known."""
+    if codes is not None and (address, version) != _UNKNOWN and (address, version) != _state_of(weight):
+        codes = scale = None
+    return _linear(x, weight, bias, e5m2, codes, scale, False)
+
+
+@_block_scaled_linear_auto.register_fake
+def _(x, weight, bias, e5m2, codes, scale, address, version):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+@torch.library.custom_op("feather_ops::block_scaled_linear_auto_backward", mutates_args=())
+def _block_scaled_linear_auto_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, e5m2: bool, need_x: bool,
+                                       need_weight: bool, need_bias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of x, weight and bias, each empty where it is not asked for. x and the weight are kept as they are and
+    quantized again: what the program's other nodes hold of them anyway."""
+    ops = torch.ops.feather_ops
+    gy, rows, weight = as_rows(grad), as_rows(x), as_rows(weight)
+    m, (n, k) = gy.shape[0], weight.shape
+    need = _train_workspace_bytes(m, n, k)
+    workspace = _workspace(gy, need) if need else None
+    grad_x, grad_weight, grad_bias = (t.new_empty(0) for t in (x, weight, x))
+    codes, scale, codes_t, scale_t, sums = ops.quantize_tiles.default(gy, e5m2, False, need_x, need_weight, need_bias)
+    if need_x:
+        _, _, w, w_scale, _ = ops.quantize_tiles.default(weight, e5m2, True, False, True, False)
+        grad_x = ops.block_scaled_mm.default(codes, scale, w, w_scale, None, _TYPES[x.dtype], workspace).reshape(x.shape)
+    if need_weight:
+        _, _, xt, xt_scale, _ = ops.quantize_tiles.default(rows, e5m2, False, False, True, False)
+        grad_weight = ops.block_scaled_mm.default(codes_t, scale_t, xt, xt_scale, None, _TYPES[weight.dtype], workspace)
+    if need_bias:
+        grad_bias = ops.sum_rows.default(sums, _TYPES[x.dtype])
+    return grad_x, grad_weight, grad_bias
+
+
+@_block_scaled_linear_auto_backward.register_fake
+def _(grad, x, weight, e5m2, need_x, need_weight, need_bias):
+    return (x.new_empty(x.shape if need_x else (0,)), weight.new_empty(weight.shape if need_weight else (0,)),
+            x.new_empty((weight.shape[0],) if need_bias else (0,)))
+
+
+def _linear_auto_context(ctx, inputs, output) -> None:
+    x, weight, bias, ctx.e5m2, *_ = inputs
+    ctx.save_for_backward(x, weight)
+
+
+def _linear_auto_backward(ctx, grad: torch.Tensor) -> tuple:
+    x, weight = ctx.saved_tensors
+    needs = ctx.needs_input_grad[:3]
+    grads = _block_scaled_linear_auto_backward(grad, x, weight, ctx.e5m2, *needs)
+    return (*(g if need else None for g, need in zip(grads, needs)), None, None, None, None, None)
+
+
+_block_scaled_linear_auto.register_autograd(_linear_auto_backward, setup_context=_linear_auto_context)
 
 
 # ---- shapes, for tracing ----

@@ -91,10 +91,10 @@ _COUNTER_BYTES = 64 * 1024
 
 
 def _workspace(a: torch.Tensor, nbytes: int) -> torch.Tensor:
-    """A workspace for a product of a, shared with the other split launches of its stream; in a captured graph one of its
-    own, whose counters each replay clears (all of it, as those launches do, is 33 MB at 512 x 14336 -> 4096: 62 us a replay
-    against 47)."""
-    if a.is_cuda and not isinstance(a, FakeTensor) and torch.cuda.is_current_stream_capturing():
+    """A workspace for a product of a, shared with the other split launches of its stream; in a captured graph or a traced
+    program one of its own, whose counters each run clears (all of it, as those launches do, is 33 MB at 512 x 14336 ->
+    4096: 62 us a replay against 47)."""
+    if isinstance(a, FakeTensor) or (a.is_cuda and torch.cuda.is_current_stream_capturing()):
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
         workspace[:_COUNTER_BYTES].zero_()
         return workspace

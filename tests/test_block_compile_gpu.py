@@ -5,6 +5,7 @@ import pytest
 import torch
 from torch import nn
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import feather_ops as fo
 
@@ -153,3 +154,12 @@ def test_derivatives_that_are_not_there_are_refused(backend):
         for shape in ((20, 300), (2, 10, 300)):
             with forward_ad.dual_level(), pytest.raises(NotImplementedError):
                 compiled(forward_ad.make_dual(tensor.view(shape), torch.ones_like(x).view(shape)), w.detach())
+
+
+def test_traced_program_runs_again():
+    """Products that are split along K: the program's own workspace, cleared where it has to be in each run."""
+    operands = _operands(64, 256, 4096)
+    traced = make_fx(lambda *a: fo.block_scaled_mm(*a), tracing_mode="fake")(*operands)
+    for seed in range(3):
+        fresh_ones = (*fo.quantize_blocks(_randn(64, 4096, seed=30 + seed)), *operands[2:])
+        assert torch.equal(traced(*fresh_ones), fo.block_scaled_mm(*fresh_ones))

@@ -90,7 +90,8 @@ __device__ __forceinline__ RawPiece<kType> drop_values(RawPiece<kType> raw, int 
     return raw;
 }
 
-// The 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are zero. No load
+// The 8 values at element `at` of the row `row`, of which `valid` (may be <= 0 or > 8) are there; the others are zero. The row
+// has at + valid values, no fewer: what lies past them is not read. No load
 // is a branch, so that all of a lane's loads are in flight together. (Behind branches each waited for the one before: the
 // norm of one row of 14336, 7 pieces a lane, took 10.7 us.)
 // kVec: whole pieces are 16-byte aligned and rows are whole pieces (valid <= 0 or >= 8): a lane past the end reads the

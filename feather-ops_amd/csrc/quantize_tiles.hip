@@ -52,10 +52,10 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
     Raw raw[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-        const int r = s * 16 + tid / 16;   // past the last row: nothing of the last row
+        const int r = s * 16 + tid / 16;
         const int64_t row = row0 + (r < rows ? r : rows - 1);
-        raw[s] = load_raw<kType, kVec>(static_cast<const uint8_t*>(p.x) + row * p.ldx * type_bytes(kType), at,
-                                       r < rows ? p.cols - at : 0);
+        const int from = r < rows ? at : p.cols;   // past the last row: what lies past its end, nothing
+        raw[s] = load_raw<kType, kVec>(static_cast<const uint8_t*>(p.x) + row * p.ldx * type_bytes(kType), from, p.cols - from);
     }
     uint32_t most = 0;
 #pragma unroll

@@ -240,6 +240,15 @@ struct Quantized {
     int e5m2;
 };
 
+// q from row `row` on (null codes: left out).
+inline Quantized from_row(Quantized q, int64_t row) {
+    if (q.codes) {
+        q.codes += row * q.ld_codes;
+        q.scale += row * q.scale_row;
+    }
+    return q;
+}
+
 // One piece's codes. kVec: ld_codes and codes are multiples of 8, and valid is <= 0 or >= 8.
 template <bool kVec>
 __device__ __forceinline__ void write_codes(const Quantized& q, int64_t row, int at, int valid, const float (&v)[kPiece],
@@ -278,6 +287,10 @@ inline bool on_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 inline bool rows_on_16(const void* p, int64_t ld, int type) { return on_16(p) && ld * type_bytes(type) % 16 == 0; }
 
 constexpr int64_t kMaxSize = (int64_t{1} << 31) - 1;
+
+// Threads of one launch. The runtime takes their number modulo 2^32 without an error (2^26 + 5 rows, four to a workgroup of
+// 256 threads, wrote the first 8): more rows go in several launches.
+constexpr int64_t kMaxThreads = (int64_t{1} << 32) - 1;
 
 // A matrix that the kernels can walk: sizes under 2^31 and rows under 2 GiB, no stride under the row's length.
 inline bool matrix_ok(const void* p, int64_t ld, int64_t rows, int64_t cols) {

@@ -194,13 +194,23 @@ int64_t workspace_bytes_of(const Parts& parts) {
     return most;
 }
 
+// Whether each launch has fewer than 2^32 threads.
+bool launchable(const Parts& parts) {
+    for (int i = 0; i < parts.count; ++i) {
+        const BlockMmPlan& plan = parts.part[i].plan;
+        const int64_t threads = plan.kernel < kStream1x1 ? 64 * plan.slots : plan.kernel == kStream1x1Wide ? 1024 : 512;
+        if (plan.tiles * plan.splits > kMaxThreads / threads) return false;   // (a tile's slots are its waves)
+    }
+    return true;
+}
+
 }  // namespace
 }  // namespace feather
 
 using namespace feather;
 
 extern "C" int64_t feather_block_scaled_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return sizes_ok(M, N, K) ? workspace_bytes_of(parts_of(M, N, K)) : -1;
+    return sizes_ok(M, N, K) && launchable(parts_of(M, N, K)) ? workspace_bytes_of(parts_of(M, N, K)) : -1;
 }
 
 extern "C" int feather_block_scaled_mm_launches(int64_t M, int64_t N, int64_t K, int64_t out[16]) {
@@ -222,6 +232,7 @@ extern "C" bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5
                                         hipStream_t stream) {
     if (!sizes_ok(M, N, K) || !type_ok(out_type)) return false;
     const Parts& parts = parts_of(M, N, K);
+    if (!launchable(parts)) return false;
     const int64_t need = workspace_bytes_of(parts);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0))
         return false;

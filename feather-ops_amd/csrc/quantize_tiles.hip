@@ -11,6 +11,7 @@
 // squares in both 38.4 (58 with scattered stores and branching loads).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -176,6 +177,23 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
     }
 }
 
+// p from row of tiles `tile` on.
+TilesParams from_tile(TilesParams p, int64_t tile, int type, bool square) {
+    const int64_t row = tile * kBlock;
+    p.x = static_cast<const uint8_t*>(p.x) + row * p.ldx * type_bytes(type);
+    if (p.q.codes) {
+        p.q.codes += row * p.q.ld_codes;
+        p.q.scale += (square ? tile : row) * p.q.scale_row;
+    }
+    if (p.t.codes) {
+        p.t.codes += row;
+        p.t.scale += tile * p.t.scale_block;
+    }
+    if (p.sums) p.sums += tile * p.cols;
+    p.rows -= row;
+    return p;
+}
+
 }  // namespace
 }  // namespace feather
 
@@ -192,16 +210,19 @@ extern "C" bool feather_quantize_tiles(const void* x, int type, int64_t ldx, boo
     if (codes_t && (rows > kMaxSize / 4 || !quantized_ok(codes_t, ld_codes_t, scale_t, cols, rows))) return false;
     if (!codes && !codes_t && !sums) return false;
     const int64_t tiles_n = (cols + kBlock - 1) / kBlock;
-    const int64_t tiles = tiles_n * ((rows + kBlock - 1) / kBlock);
-    if (tiles > kMaxSize) return false;
     const TilesParams p{x, {codes, scale, ld_codes, scale_row, scale_block, e5m2},
                         {codes_t, scale_t, ld_codes_t, scale_t_row, scale_t_block, e5m2}, sums, ldx, rows,
                         static_cast<int32_t>(cols), static_cast<int32_t>(tiles_n)};
     const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) && (!codes || (on_16(codes) && ld_codes % 8 == 0));
-    const auto grid = static_cast<uint32_t>(tiles);
+    const int64_t tiles_m = (rows + kBlock - 1) / kBlock;
+    const int64_t most = kMaxThreads / kThreads / tiles_n;   // rows of tiles of a launch
     const auto go = [&](auto t, auto v) {
-        if (square) tiles_kernel<t(), v(), true><<<grid, kThreads, 0, stream>>>(p);
-        else tiles_kernel<t(), v(), false><<<grid, kThreads, 0, stream>>>(p);
+        for (int64_t tile = 0; tile < tiles_m; tile += most) {
+            const TilesParams part = from_tile(p, tile, type, square);
+            const auto grid = static_cast<uint32_t>(std::min(tiles_m - tile, most) * tiles_n);
+            if (square) tiles_kernel<t(), v(), true><<<grid, kThreads, 0, stream>>>(part);
+            else tiles_kernel<t(), v(), false><<<grid, kThreads, 0, stream>>>(part);
+        }
     };
     const auto typed = [&](auto t) {
         if (vec) go(t, std::true_type{});

@@ -14,6 +14,7 @@
 // of 4096 x 4096 bf16 25 us, 5.4 TB/s, and 4 us for the weight's sums; one row of 4096 2.9 us, a launch's time.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -345,7 +346,8 @@ constexpr int kSumGroups = kThreads / kSumCols;
 constexpr int kSumAhead = 8;
 
 template <int kType>
-__global__ __launch_bounds__(kThreads) void sum_rows_kernel(const float* part, void* out, int64_t rows, int64_t cols) {
+__global__ __launch_bounds__(kThreads) void sum_rows_kernel(const float* part, void* out, int64_t rows, int64_t cols,
+                                                            int64_t ld) {
     __shared__ float lds[kSumGroups][kSumCols];
     const int group = threadIdx.x / kSumCols;
     const int64_t col = static_cast<int64_t>(blockIdx.x) * kSumCols + threadIdx.x % kSumCols;
@@ -356,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void sum_rows_kernel(const float* part, v
 #pragma unroll
             for (int k = 0; k < kSumAhead; ++k) {
                 const int64_t row = i + k * kSumGroups;
-                v[k] = part[(row < rows ? row : rows - 1) * cols + col];   // no branch: 8 loads in flight
+                v[k] = part[(row < rows ? row : rows - 1) * ld + col];   // no branch: 8 loads in flight
             }
 #pragma unroll
             for (int k = 0; k < kSumAhead; ++k) s += i + k * kSumGroups < rows ? v[k] : 0.0f;
@@ -372,7 +374,6 @@ __global__ __launch_bounds__(kThreads) void sum_rows_kernel(const float* part, v
     else static_cast<uint16_t*>(out)[col] = static_cast<uint16_t>(to_bits<kType>(s));
 }
 
-constexpr int64_t kMaxGrid = (int64_t{1} << 31) - 1;
 constexpr int64_t kWaveCols = 2048;       // rows up to here are one wave's
 constexpr int64_t kRegisterCols = 16384;  // and up to here in registers
 constexpr int64_t kLongParts = 64;
@@ -383,6 +384,19 @@ int64_t backward_groups(int64_t rows, int64_t cols) {
     if (cols > kRegisterCols) return rows < kLongParts ? rows : kLongParts;
     const int64_t groups = cols <= kWaveCols ? (rows + kWaves - 1) / kWaves : rows;
     return groups < 512 ? groups : 512;
+}
+
+// p from row `row` on.
+NormParams from_row(NormParams p, int64_t row, int type) {
+    const int bytes = type_bytes(type);
+    p.x = static_cast<const uint8_t*>(p.x) + row * p.ldx * bytes;
+    if (p.residual) p.residual = static_cast<const uint8_t*>(p.residual) + row * p.ld_residual * bytes;
+    if (p.h) p.h = static_cast<uint8_t*>(p.h) + row * p.ldh * bytes;
+    if (p.y) p.y = static_cast<uint8_t*>(p.y) + row * p.ldy * bytes;
+    if (p.rstd) p.rstd += row;
+    p.q = from_row(p.q, row);
+    p.rows -= row;
+    return p;
 }
 
 // Calls f<type, vec>() for the runtime values.
@@ -459,16 +473,21 @@ extern "C" bool feather_rms_norm(const void* x, int64_t ldx, const void* residua
     const bool vec = cols % kPiece == 0 && rows_on_16(x, ldx, type) && on_16(weight) &&
                      (!residual || (rows_on_16(residual, ld_residual, type) && rows_on_16(h, ldh, type))) &&
                      (y ? rows_on_16(y, ldy, type) : (on_16(codes) && ld_codes % 8 == 0));
-    const int64_t groups = cols <= kWaveCols ? (rows + kWaves - 1) / kWaves : rows;
-    if (groups > kMaxGrid) return false;
+    const auto launch = [&](auto kernel, int threads, int64_t group_rows) {
+        const int64_t most = kMaxThreads / threads * group_rows;   // rows of a launch
+        for (int64_t row = 0; row < rows; row += most) {
+            NormParams part = from_row(p, row, type);
+            part.rows = std::min(part.rows, most);
+            kernel<<<static_cast<uint32_t>((part.rows + group_rows - 1) / group_rows), threads, 0, stream>>>(part);
+        }
+    };
     by_type(type, vec, [&](auto t, auto v) {
         if (cols > kRegisterCols) {
-            norm_kernel<t(), v(), kWaves, 0><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(p);
+            launch(norm_kernel<t(), v(), kWaves, 0>, kThreads, 1);
             return;
         }
         by_cols<false>(rows, cols, [&](auto waves, auto pieces) {
-            norm_kernel<t(), v(), waves(), pieces()>
-                <<<static_cast<uint32_t>(groups), threads_of(waves()), 0, stream>>>(p);
+            launch(norm_kernel<t(), v(), waves(), pieces()>, threads_of(waves()), waves() == 1 ? kWaves : 1);
         });
     });
     return true;
@@ -491,6 +510,7 @@ extern "C" bool feather_rms_norm_backward(const void* grad_y, int64_t ld_grad_y,
     if (!aligned_to_type(grad_y, type) || !aligned_to_type(h, type) || !aligned_to_type(grad_h, type) ||
         !aligned_to_type(weight, weight_type))
         return false;
+    if (cols > kRegisterCols && rows > kMaxThreads / kThreads) return false;
     const NormBackwardParams p{grad_y, grad_h_in, h, weight, rstd, grad_h, part, ld_grad_y, ld_grad_h_in, ldh,
                                ld_grad_h, rows, static_cast<int32_t>(cols), weight_fp32};
     const bool vec = cols % kPiece == 0 && on_16(part) && rows_on_16(grad_y, ld_grad_y, type) && rows_on_16(h, ldh, type) &&
@@ -515,10 +535,14 @@ extern "C" bool feather_rms_norm_backward(const void* grad_y, int64_t ld_grad_y,
 extern "C" bool feather_sum_rows(const float* part, void* out, int type, int64_t rows, int64_t cols,
                                  hipStream_t stream) {
     if (!part || !out || !type_ok(type) || rows < 1 || cols < 1 || !aligned_to_type(out, type)) return false;
-    const int64_t groups = (cols + kSumCols - 1) / kSumCols;
-    if (groups > kMaxGrid) return false;
+    constexpr int64_t kMost = kMaxThreads / kThreads * kSumCols;   // columns of a launch
     by_type(type, true, [&](auto t, auto) {
-        sum_rows_kernel<t()><<<static_cast<uint32_t>(groups), kThreads, 0, stream>>>(part, out, rows, cols);
+        for (int64_t col = 0; col < cols; col += kMost) {
+            const int64_t here = std::min(cols - col, kMost);
+            const auto groups = static_cast<uint32_t>((here + kSumCols - 1) / kSumCols);
+            sum_rows_kernel<t()><<<groups, kThreads, 0, stream>>>(
+                part + col, static_cast<uint8_t*>(out) + col * type_bytes(type), rows, here, cols);
+        }
     });
     return true;
 }

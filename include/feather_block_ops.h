@@ -55,7 +55,9 @@ enum { FEATHER_BF16 = 0, FEATHER_FP16 = 1, FEATHER_FP32 = 2 };
  *             is 0. As feather_scaled_mm_splitk's: its first 64 KiB all zero before its first use, left zero by every call;
  *             calls that share it must be ordered.
  *
- * 1 <= M, N < 2^29, ceil(M / 64) * ceil(N / 16) < 2^27, 0 <= K <= 2^22 (K = 0: c is the bias, or zero). Deterministic: the same operands give the same bits.
+ * 1 <= M, N < 2^29, 0 <= K <= 2^22 (K = 0: c is the bias, or zero), and few enough outputs for a launch to have under 2^32
+ * threads (more than 2^36 of them, or beside up to 64 rows 2^26 columns, may be refused). Deterministic: the same operands
+ * give the same bits.
  */
 bool feather_block_scaled_mm(const uint8_t* a, int64_t lda, bool a_e5m2, const float* a_scale, int64_t a_scale_row,
                              int64_t a_scale_block, const uint8_t* b, int64_t ldb, bool b_e5m2, const float* b_scale,

@@ -58,3 +58,13 @@ def test_products_are_cut_along_both_axes(launches):
 def test_shapes_without_a_plan(launches):
     assert launches(0, 5, 128) == launches(5, 0, 128) == launches(5, 5, -1) == launches(5, 5, 1 << 23) == []
     assert len(launches(1, 1, 0)) == 1
+
+
+def test_launches_have_fewer_than_2_32_threads():
+    """A grid of more would be cut off without an error: such shapes are refused."""
+    from feather_ops import _lib
+
+    need = _lib.c_library().feather_block_scaled_mm_workspace_bytes
+    assert need(1, (1 << 26) - 16, 16) >= 0 and need(64, (1 << 26) - 16, 16) >= 0 and need((1 << 29) - 1, 1, 16) >= 0
+    for m, n, k in ((1, 1 << 27, 16), (8, 1 << 27, 16), (1, (1 << 29) - 1, 16), (1, 1 << 26, 4096), ((1 << 21) + 1, 1 << 17, 16)):
+        assert need(m, n, k) == -1

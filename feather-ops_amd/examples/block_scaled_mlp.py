@@ -32,7 +32,7 @@ class BlockScaledMLP(nn.Module):
         fo.to_block_scaled_linear(self)
 
     def freeze_(self) -> "BlockScaledMLP":
-        """For inference: the weights take no gradients and are quantized once."""
+        """For inference: the weights take no gradients and are quantized once. (Inputs may still ask for theirs.)"""
         self.requires_grad_(False)
         self.gate_up.quantize_weight_()
         self.down.quantize_weight_()
@@ -40,13 +40,14 @@ class BlockScaledMLP(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(the layer's output, the residual stream h) for x and residual `[tokens, width]`."""
-        if self.gate_up.weight.requires_grad:
+        wide, narrow = self.gate_up.quantized_weight(), self.down.quantized_weight()
+        differentiable = torch.is_grad_enabled() and any(t.requires_grad for t in (x, residual, *self.parameters()))
+        if differentiable or wide is None or narrow is None:
             y, h = fo.rms_norm(x, self.norm, residual, self.eps)
             return self.down(fo.silu_mul(self.gate_up(y))), h
         codes, scale, h = fo.rms_norm_quantized(x, self.norm, residual, self.eps)
-        gate_up = fo.block_scaled_mm(codes, scale, *self.gate_up.quantized_weight(), None, x.dtype)
-        codes, scale = fo.silu_mul_quantized(gate_up)
-        return fo.block_scaled_mm(codes, scale, *self.down.quantized_weight(), None, x.dtype), h
+        codes, scale = fo.silu_mul_quantized(fo.block_scaled_mm(codes, scale, *wide, None, x.dtype))
+        return fo.block_scaled_mm(codes, scale, *narrow, None, x.dtype), h
 
 
 def reference(mlp: BlockScaledMLP, x: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:

@@ -58,9 +58,11 @@ BlockMmPlan few_rows_plan(int64_t M, int64_t N, int64_t K) {
     return stream_plan(kernel, 1, 1, M, N, splits(tiles, 256, 16));
 }
 
-// A tile of the ring kernel: workgroups that share a CU's LDS, and microseconds fitted to 3300 timings of 115 shapes (33 to
-// 12288 rows, N and K 256 to 16384): a workgroup's start and end, and a stage with the CU full of workgroups and with one. The
-// tile and splits with the least estimate took at most 1.12 of the best pair's time on any of them, 1.005 in geometric mean.
+// A tile of the ring kernel, and microseconds fitted to 3300 timings of 115 shapes (33 to 12288 rows, N and K 256 to 16384): a
+// workgroup's start and end, and a stage with per_cu workgroups on a CU and with one. per_cu is the model's: of the 64 x 64 tile
+// two fit a CU's LDS at a time (66 KiB each), and its figures for four hold what the second two wait. On the shapes of the fit
+// the tile and splits with the least estimate took at most 1.12 of the best pair's time, 1.005 in geometric mean; others were
+// not timed against all pairs, and large ones take more than their estimate (4096 x 14336 x 4096: 200 us, in fact 218).
 struct TileCost {
     BlockMmKernel kernel;
     int bm, bn, waves, per_cu;

@@ -230,7 +230,10 @@ class BlockScaledLinear:
     and those to a weight made in inference mode need a call of `quantize_weight_`. A weight that takes gradients is
     quantized on every pass. Parameters and `state_dict` stay as they were."""
 
-    def quantize_weight_(self, fp8_dtype: torch.dtype = torch.float8_e4m3fn) -> None:
+    def quantize_weight_(self, fp8_dtype: torch.dtype | None = None) -> None:
+        """Keep the weight's codes as it is now, in fp8_dtype (None: the format that the layer has, at first e4m3fn)."""
+        if fp8_dtype is None:
+            fp8_dtype = getattr(self, "_fp8_dtype", torch.float8_e4m3fn)
         codes, scale = quantize_blocks(self.weight, fp8_dtype, square=True)
         kept = self._buffers.get("weight_fp8")
         if (kept is not None and kept.dtype == codes.dtype and kept.shape == codes.shape and kept.device == codes.device
@@ -255,7 +258,7 @@ class BlockScaledLinear:
         super()._apply(fn, recurse)
         if kept[0] is not None:
             if self.weight.is_cuda:
-                self.quantize_weight_(self._fp8_dtype)
+                self.quantize_weight_()
             else:
                 for name, buffer in zip(("weight_fp8", "weight_scale"), kept):
                     self.register_buffer(name, buffer.to(self.weight.device), persistent=False)
@@ -278,7 +281,7 @@ class BlockScaledLinear:
             if (not isinstance(weight, nn.Parameter) or torch._C._len_torch_dispatch_stack()
                     or (weight.is_cuda and torch.cuda.is_current_stream_capturing())):
                 return None
-            self.quantize_weight_(self._fp8_dtype)
+            self.quantize_weight_()
         return self._buffers["weight_fp8"], self._buffers["weight_scale"]
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

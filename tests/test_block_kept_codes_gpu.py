@@ -170,3 +170,14 @@ def test_format_is_kept(layer):
     layer.half().cuda()
     assert layer.weight_fp8.dtype == torch.float8_e5m2
     assert torch.equal(layer(_x().half()), fo.block_scaled_linear(_x().half(), layer.weight, layer.bias, torch.float8_e5m2))
+
+
+def test_quantizing_again_keeps_the_layers_format(cuda_device):
+    layer = torch.nn.Linear(300, 130, device="cuda", dtype=torch.bfloat16).requires_grad_(False)
+    fo.to_block_scaled_linear(layer, torch.float8_e5m2)
+    layer.weight.data.mul_(2)
+    layer.quantize_weight_()
+    assert layer.weight_fp8.dtype == torch.float8_e5m2
+    assert torch.equal(layer(_x()), fo.block_scaled_linear(_x(), layer.weight, layer.bias, torch.float8_e5m2))
+    layer.quantize_weight_(torch.float8_e4m3fn)
+    assert layer.weight_fp8.dtype == torch.float8_e4m3fn and _is_current(layer)

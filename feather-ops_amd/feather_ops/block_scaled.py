@@ -155,11 +155,11 @@ def block_scaled_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     """`x @ weight^T + bias` in fp8 with a scale for each block of 128: x `[..., K]`, weight `[N, K]`, y `[..., N]` in x's
     dtype (bfloat16, float16 or float32).
 
-    Differentiable once, in reverse mode, in x, weight and bias: the gradients are products of fp8 operands too, each quantized along the axis it
-    is summed over (dx and dw are the exact gradients of the product but for that rounding, with the quantization itself
-    taken as the identity). Weight and activations are quantized on every call; `quantized_weight`, the result of
-    `quantize_blocks(weight, dtype, square=True)`, saves that for a weight that does not change. bias is taken in x's
-    dtype."""
+    Differentiable once, in reverse mode, in x, weight and bias: the gradients are products of fp8 operands too, each
+    quantized along the axis it is summed over (dx and dw are the exact gradients of the product but for that rounding, with
+    the quantization itself taken as the identity; dw over at most 2**22 rows of x). Weight and activations are quantized on
+    every call; `quantized_weight`, the result of `quantize_blocks(weight, dtype, square=True)`, saves that for a weight that
+    does not change. bias is taken in x's dtype."""
     return _checked_linear(x, weight, bias, dtype, quantized_weight, _UNKNOWN)
 
 

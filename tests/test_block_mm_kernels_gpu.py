@@ -65,3 +65,14 @@ def test_zeros(fo, m):
     weight = fo.quantize_blocks(_uneven(n, k, 6), square=True)
     zero = fo.quantize_blocks(torch.zeros((m, k), device="cuda"))
     assert (fo.block_scaled_mm(*zero, *weight, None, torch.float32) == 0).all()
+
+
+@pytest.mark.parametrize("by_row", [False, True])
+@pytest.mark.parametrize("m,n", [(2, 300), (20, 9000), (50, 70), (100, 300), (1400, 300), (300, 3300), (1312, 5426), (5551, 646), (1411, 5383)])
+def test_no_columns_to_sum_over(fo, m, n, by_row):
+    """K = 0: the bias alone, on whatever kernel."""
+    a, b = (torch.zeros((rows, 0), dtype=torch.float8_e4m3fn, device="cuda") for rows in (m, n))
+    sa, sb = torch.ones((m, 0), device="cuda"), torch.ones((n if by_row else ref.blocks(n), 0), device="cuda")
+    bias = _uneven(1, n, 7)[0].bfloat16()
+    assert torch.equal(fo.block_scaled_mm(a, sa, b, sb, bias), bias.expand(m, n))
+    assert (fo.block_scaled_mm(a, sa, b, sb) == 0).all()

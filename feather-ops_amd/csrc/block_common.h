@@ -209,25 +209,48 @@ __device__ __forceinline__ uint32_t max_bits(const float (&v)[kPiece]) {
     return m;
 }
 
-// A block's scale and the factor that takes its values to codes. A product with L / amax in place of the quotient by
-// amax / L: one division a block instead of one a value. The product of the largest value is at most L (1 + 2^-22), which
-// rounds to L, so codes need no clamp.
-__device__ __forceinline__ float block_scale(uint32_t amax_bits, bool e5m2, float& factor) {
+// What takes a block's values to codes: a product with L / amax in place of the quotient by amax / L, one division a block
+// instead of one a value. The product of the largest value is at most L (1 + 2^-22), which rounds to L, so codes need no
+// clamp. One term for values that were computed in fp32 and are off by as much themselves.
+struct Factor {
+    float hi;
+    __device__ __forceinline__ void set(float amax, float largest, float) { hi = largest / amax; }
+    __device__ __forceinline__ float operator()(float v) const { return v * hi; }
+};
+
+// L / amax as hi + lo, within 2^-46 of it, for values that are given: value * lo, then one multiply-add with hi, is the
+// quotient rounded once, so that a code is the nearest one, ties too: none of 34 million bf16 values takes another than by
+// 64 bits (with one term 5294 of 17 million, with 32-bit quotients 11118 of the 34: most at exact ties). Rows of 4096 x 4096
+// take 11.4 us for 11.1, 4096 x 12288 along both axes with sums 38.5 for 37.4.
+struct ExactFactor {
+    float hi, lo;
+    __device__ __forceinline__ void set(float amax, float largest, float inverse) {
+        hi = largest / amax;
+        const float rest = __builtin_fmaf(-hi, amax, largest) * (hi * inverse);   // the remainder, exact, over amax
+        lo = amax < __builtin_inff() ? rest : 0.0f;                               // of infinity: hi is zero, or NaN
+    }
+    __device__ __forceinline__ float operator()(float v) const { return __builtin_fmaf(v, hi, v * lo); }
+};
+
+// A block's scale and factor.
+template <typename F>
+__device__ __forceinline__ float block_scale(uint32_t amax_bits, bool e5m2, F& factor) {
     const float amax = __builtin_bit_cast(float, max(amax_bits, kLeastBits));
     const float largest = e5m2 ? 57344.0f : 448.0f;
-    factor = largest / amax;
+    factor.set(amax, largest, e5m2 ? 1.0f / 57344.0f : 1.0f / 448.0f);
     return amax / largest;
 }
 
 // Four values times factor -> four codes, the first one lowest.
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float factor, bool e5m2) {
+template <typename F>
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, F factor, bool e5m2) {
     int out = 0;
     if (e5m2) {
-        out = __builtin_amdgcn_cvt_pk_bf8_f32(a * factor, b * factor, out, false);
-        out = __builtin_amdgcn_cvt_pk_bf8_f32(c * factor, d * factor, out, true);
+        out = __builtin_amdgcn_cvt_pk_bf8_f32(factor(a), factor(b), out, false);
+        out = __builtin_amdgcn_cvt_pk_bf8_f32(factor(c), factor(d), out, true);
     } else {
-        out = __builtin_amdgcn_cvt_pk_fp8_f32(a * factor, b * factor, out, false);
-        out = __builtin_amdgcn_cvt_pk_fp8_f32(c * factor, d * factor, out, true);
+        out = __builtin_amdgcn_cvt_pk_fp8_f32(factor(a), factor(b), out, false);
+        out = __builtin_amdgcn_cvt_pk_fp8_f32(factor(c), factor(d), out, true);
     }
     return static_cast<uint32_t>(out);
 }
@@ -250,9 +273,9 @@ inline Quantized from_row(Quantized q, int64_t row) {
 }
 
 // One piece's codes. kVec: ld_codes and codes are multiples of 8, and valid is <= 0 or >= 8.
-template <bool kVec>
+template <bool kVec, typename F>
 __device__ __forceinline__ void write_codes(const Quantized& q, int64_t row, int at, int valid, const float (&v)[kPiece],
-                                            float factor) {
+                                            F factor) {
     const u32x2v codes{codes4(v[0], v[1], v[2], v[3], factor, q.e5m2), codes4(v[4], v[5], v[6], v[7], factor, q.e5m2)};
     uint8_t* out = q.codes + row * q.ld_codes + at;
     if (valid >= kPiece) {
@@ -269,10 +292,10 @@ __device__ __forceinline__ void write_codes(const Quantized& q, int64_t row, int
 
 // One piece of a row quantized with its block's 16 lanes, all of which call this together (with valid <= 0 past the row's
 // end): writes its codes, and the block's first lane the scale.
-template <bool kVec>
+template <bool kVec, typename F>
 __device__ __forceinline__ void quantize_piece(const Quantized& q, int64_t row, int at, int valid,
                                                const float (&v)[kPiece]) {
-    float factor;
+    F factor;
     const float scale = block_scale(max16(max_bits(v)), q.e5m2, factor);
     if (valid <= 0) return;
     write_codes<kVec>(q, row, at, valid, v, factor);

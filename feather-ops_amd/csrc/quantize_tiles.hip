@@ -74,10 +74,11 @@ __global__ __launch_bounds__(kThreads) void tiles_kernel(const TilesParams p) {
             most = max(most, max_bits(v));
         } else {
             // valid <= 0 past the last row: quantize_piece writes nothing there
-            if (p.q.codes) quantize_piece<kVec>(p.q, row0 + r, at, r < rows ? p.cols - at : 0, v);
+            if (p.q.codes) quantize_piece<kVec, ExactFactor>(p.q, row0 + r, at, r < rows ? p.cols - at : 0, v);
         }
     }
-    float factor = 0.0f, scale = 0.0f;
+    ExactFactor factor{};
+    float scale = 0.0f;
     if constexpr (kSquare) {
         most = max16(most);
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));

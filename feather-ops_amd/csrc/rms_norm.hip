@@ -106,7 +106,7 @@ __device__ __forceinline__ void write_piece(const NormParams& p, int64_t row, in
     if (p.y) {
         if (valid > 0) store_piece<kType, kVec>(row_at<kType>(p.y, row, p.ldy), at, valid, v);
     } else {
-        quantize_piece<kVec>(p.q, row, at, valid, v);
+        quantize_piece<kVec, Factor>(p.q, row, at, valid, v);
     }
 }
 

@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsParams p) {
             return;
         }
     }
-    quantize_piece<kVec>(p.q, row, at, valid, v);
+    quantize_piece<kVec, std::conditional_t<kOp == Op::kQuantize, ExactFactor, Factor>>(p.q, row, at, valid, v);
 }
 
 // p from row `row` on.

@@ -101,12 +101,14 @@ __device__ __forceinline__ void write_piece(const NormParams& p, int64_t row, in
     float w[kPiece];
     if (p.weight_fp32) load_piece<FEATHER_FP32, kVec>(p.weight, at, valid, w);
     else unpack(raw_w, w);
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) v[i] = v[i] * r * w[i];
     if (p.y) {
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) v[i] = v[i] * r * w[i];
         if (valid > 0) store_piece<kType, kVec>(row_at<kType>(p.y, row, p.ldy), at, valid, v);
     } else {
-        quantize_piece<kVec, Factor>(p.q, row, at, valid, v);
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) v[i] *= w[i];
+        quantize_piece<kVec, RowFactor>(p.q, row, at, valid, v, r);
     }
 }
 

@@ -9,8 +9,8 @@
  * Blocks: a block is 128 consecutive values of a row (the last of a row may be shorter) or, of a weight, 128 x 128.
  * With L the format's largest value (448 or 57344), a block has
  *   scale = max(largest |value|, 2^-100) / L     code = value / scale, rounded to nearest even,
- * computed in fp32: the quotient of a given value is rounded once, that of an output which is not stored (the norm's, the
- * gate's) is a product with L / max(...), within an ulp and a half. A NaN makes its whole block NaN; an
+ * computed in fp32: the quotient is rounded once (the norm's without its factor 1 / rms, which is in the scale; the gate's
+ * is a product with L / max(...), within an ulp and a half). A NaN makes its whole block NaN; an
  * infinity makes its block's scale infinite, its own code NaN and the others' zero, so that what is computed from the
  * block is NaN. The floor 2^-100 keeps both scales finite and non-zero for blocks of zeros and of values too small to
  * matter, which get codes near zero.

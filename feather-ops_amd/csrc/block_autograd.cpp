@@ -6,36 +6,15 @@
 //
 // Host code; unlike the ops themselves (block_extension.cpp) it needs torch's C++ interface and not only its stable one, and
 // is a library of its own for that.
-#include <ATen/core/LegacyTypeDispatch.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/inductor/aoti_torch/c/shim.h>
-#include <torch/library.h>
+#include "autograd_common.h"
 
-#include <hip/hip_runtime_api.h>
-
-#include <algorithm>
 #include <cstdint>
-#include <initializer_list>
-#include <memory>
 #include <optional>
 #include <tuple>
-#include <utility>
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Function;
-using torch::autograd::variable_list;
-
-template <typename Signature>
-c10::TypedOperatorHandle<Signature> op(const char* name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
-}
+using namespace feather;
 
 Tensor silu_mul(const Tensor& x) {
     static const auto call = op<Tensor(const Tensor&)>("feather_ops::silu_mul");
@@ -92,21 +71,6 @@ int64_t type_number(at::ScalarType type) {
     TORCH_CHECK_VALUE(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat,
                       "values must be bfloat16, float16 or float32");
     return type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : 2;
-}
-
-// A gradient as the kernels read it: each row's values side by side (a broadcast one is copied out).
-Tensor as_rows(const Tensor& t) {
-    return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous();
-}
-
-bool wants_grad(const Tensor& t) { return t.requires_grad(); }
-
-// Forward mode has no formulas here: an operand's tangent is refused, with and without a graph, and never dropped. (Under a
-// transform the op is called once more for each level, with that level's tangents.)
-void refuse_tangents(const char* name, std::initializer_list<std::optional<Tensor>> operands) {
-    for (const auto& t : operands)
-        TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "forward-mode derivatives of ", name,
-                                    " are not implemented");
 }
 
 struct SiluMul : public Function<SiluMul> {
@@ -170,36 +134,6 @@ Norm rms_norm_autograd(const Tensor& x, const Tensor& weight, const std::optiona
     return rms_norm(x, weight, residual, eps, need_rstd);
 }
 
-// The forward's workspace for the backward's products: both run on the forward's stream. A graph that captures the backward
-// gets one of its own, whose arrival counters each replay clears, as graphs may share the memory of what a capture frees.
-std::optional<Tensor> workspace_of(const c10::IValue& kept) {
-    if (!kept.isTensor()) return std::nullopt;
-    const Tensor& workspace = kept.toTensor();
-    if (workspace.key_set().has(c10::DispatchKey::Python)) return workspace;   // fake
-    void* stream = nullptr;
-    TORCH_CHECK(aoti_torch_get_current_cuda_stream(workspace.get_device(), &stream) == AOTI_TORCH_SUCCESS,
-                "no current stream");
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) == hipSuccess,
-                "the stream's capture status is unknown");
-    if (capture == hipStreamCaptureStatusNone) return workspace;
-    constexpr int64_t kCounterBytes = 64 * 1024;
-    Tensor own = at::empty_like(workspace);
-    own.narrow(0, 0, std::min(kCounterBytes, own.numel())).zero_();
-    return own;
-}
-
-// Makes `grad` depend on what it was computed from, by way of a node that refuses to go on: the gradient that came in and an
-// operand, by the edge that the layer's node has to it (the operand itself is not kept, its fp8 copies are).
-void refuse_second(Tensor& grad, const Tensor& grad_y, const torch::autograd::Edge& operand) {
-    torch::autograd::edge_list from;
-    if (grad_y.requires_grad()) from.push_back(torch::autograd::impl::gradient_edge(grad_y));
-    if (operand.is_valid()) from.push_back(operand);
-    if (!grad.defined() || from.empty()) return;
-    torch::autograd::set_history(grad, std::make_shared<torch::autograd::Error>(
-                                           "second derivatives of block_scaled_linear are not implemented", std::move(from)));
-}
-
 // y = x w^T + bias in fp8: x and w quantized by rows and by squares; dx = dy w and dw = dy^T x with dy, dy^T and x^T quantized
 // by rows, and w^T by the same squares. What is kept for the backward is fp8.
 struct Linear : public Function<Linear> {
@@ -260,9 +194,9 @@ struct Linear : public Function<Linear> {
         if (twice) {   // dx depends on the weight, dW on x, all three on dy
             const auto node = torch::autograd::get_current_node();
             TORCH_CHECK(node, "block_scaled_linear: its backward runs outside of its node");
-            refuse_second(grad_x, grads[0], node->next_edge(1));
-            refuse_second(grad_w, grads[0], node->next_edge(0));
-            refuse_second(grad_b, grads[0], {});
+            refuse_second("block_scaled_linear", grad_x, grads[0], {node->next_edge(1)});
+            refuse_second("block_scaled_linear", grad_w, grads[0], {node->next_edge(0)});
+            refuse_second("block_scaled_linear", grad_b, grads[0], {});
         }
         return {grad_x, grad_w, grad_b, Tensor(), Tensor(), Tensor(), Tensor()};
     }

@@ -18,6 +18,7 @@
 
 #include "block_common.h"
 #include "scaled_mm_kernels.h"
+#include "split_join.h"
 
 namespace feather {
 
@@ -116,42 +117,6 @@ __device__ __forceinline__ void add_scaled(f32x4& acc, const f32x4 t, float s) {
 __device__ __forceinline__ void add_scaled(f32x4& acc, const f32x4 t, const f32x4 s) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(t[i], s[i], acc[i]);
-}
-
-// A tile whose K is split over p.splits workgroups: parts of it (kSlots a tile, each one wave's fp32 sums) meet in the
-// workspace. A wave writes its sums through to the memory that all XCDs share, counts itself in, and the last of the part's
-// waves to come reads all of them back, adds them in order of the K ranges (so the result does not depend on who was last),
-// leaves the counter at zero and returns true: it stores the outputs. Nobody waits for another workgroup.
-template <int kSlots, int RM, int RN>
-__device__ __forceinline__ bool join_splits(const BlockMmParams& p, f32x4 (&acc)[RM][RN], int tile, int split, int slot,
-                                            int lane) {
-    constexpr uint32_t kPartBytes = RM * RN * kWave * 16;
-    const rsrc_t parts = make_rsrc(p.split_part, 0x7fffffffu);
-    const auto place = [&](int s) {
-        return (static_cast<uint32_t>(tile * p.splits + s) * kSlots + slot) * kPartBytes + lane * 16u;
-    };
-    uint32_t* const counter = p.split_ctr + tile * kSlots + slot;
-#pragma unroll
-    for (int f = 0; f < RM * RN; ++f)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[f / RN][f % RN]), parts,
-                                               place(split) + f * kWave * 16u, 0, kDeviceScope);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // written for every XCD before the count says so
-    uint32_t before = 0;
-    if (lane == 0) before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    before = __builtin_amdgcn_readfirstlane(before);
-    asm volatile("" ::: "memory");   // the reads below come after it
-    if (before + 1 != static_cast<uint32_t>(p.splits)) return false;
-    for (int s = 0; s < p.splits; ++s) {
-#pragma unroll
-        for (int f = 0; f < RM * RN; ++f) {
-            const u32x4 bits = __builtin_amdgcn_raw_buffer_load_b128(parts, place(s) + f * kWave * 16u, 0, kDeviceScope);
-            const f32x4 part = __builtin_bit_cast(f32x4, bits);
-            f32x4& sum = acc[f / RN][f % RN];
-            sum = s == 0 ? part : sum + part;
-        }
-    }
-    if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return true;
 }
 
 }  // namespace feather

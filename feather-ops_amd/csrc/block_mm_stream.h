@@ -144,7 +144,7 @@ __global__ __launch_bounds__(T::kThreads) void block_stream_kernel(const BlockMm
         for (int w = 1; w < T::kWaves; ++w) sum[0][0] += join[w][f][lane];
         if (p.splits > 1) {
             const int tile = static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x);
-            if (!join_splits<RM * RN, 1, 1>(p, sum, tile, split, f, lane)) continue;
+            if (!join_splits<RM * RN>(p, sum, tile, split, f, lane)) continue;
         }
         store_out(p, m0 + f / RN * 16 + r16, n0 + f % RN * 16 + 4 * g, sum[0][0]);
     }

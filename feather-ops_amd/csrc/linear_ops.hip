@@ -1,0 +1,337 @@
+// The feed-forward operators' host side (include/feather_linear_ops.h): the choice of a kernel, the contract's checks and the C
+// ABI, and the gated block's elementwise backward.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "feather_internal.h"
+#include "feather_linear_ops.h"
+#include "linear_launch.h"
+
+namespace feather {
+namespace {
+
+constexpr int64_t kCUs = 256;
+constexpr int64_t kCtrBytes = 64 * 1024;   // the workspace's arrival counters, as the other split launches'
+constexpr int64_t kMaxCounters = kCtrBytes / 4;
+constexpr int64_t kMaxPartBytes = kMaxSize - kCtrBytes;
+constexpr int64_t kMaxDepth = int64_t{1} << 21;   // K and row strides: 256 rows of a tile stay within 31-bit offsets
+
+int64_t ceil_div(int64_t x, int64_t y) { return (x + y - 1) / y; }
+
+bool splits_fit(const LinearPlan& plan) {
+    return plan.tiles * plan.slots <= kMaxCounters && plan.tiles * plan.splits * plan.tile_bytes <= kMaxPartBytes;
+}
+
+// A tile, and microseconds of a workgroup's start and end and of a stage of 64, with per_cu workgroups on a CU and with one.
+struct TileCost {
+    LinearKernel kernel;
+    int bm, bn, per_cu;
+    float fixed, full, alone;
+};
+constexpr TileCost kTiles[] = {
+    {kTile256, 256, 256, 1, 4.0f, 1.42f, 1.42f},
+    {kTile256x128, 256, 128, 1, 3.0f, 0.85f, 0.85f},
+    {kTile128, 128, 128, 2, 2.0f, 0.98f, 0.60f},
+};
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+
+// N: columns of b (gated: 2 F).
+LinearPlan tile_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t all = ceil_div(K, 64);
+    const float memory = static_cast<float>(N + M) * static_cast<float>(K) / 2.4e6f;   // us at 4.8 TB/s
+    LinearPlan best{};
+    for (const TileCost& t : kTiles) {
+        const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
+        for (const int splits : kSplits) {
+            LinearPlan plan{t.kernel, splits, tiles, 4, int64_t{4} * t.bm * t.bn, 0.0f};
+            if (splits > 1 && (splits > all || tiles * splits > 4 * kCUs || !splits_fit(plan))) break;
+            const auto stages = static_cast<float>(ceil_div(all, splits));
+            const int64_t groups = tiles * splits;
+            const int64_t rounds = groups / (kCUs * t.per_cu);
+            const int64_t rest = groups - rounds * kCUs * t.per_cu;
+            float cost = static_cast<float>(rounds) * (stages * t.full + t.fixed);
+            if (rest > 0) cost += stages * (rest > kCUs ? t.full : t.alone) + t.fixed;
+            cost = std::max(cost, memory);
+            // the last of a tile's workgroups reads all of its sums back
+            if (splits > 1) cost += 2.0f + 1.5f / 65536.0f * static_cast<float>(splits * plan.tile_bytes);
+            plan.cost = cost;
+            if (best.cost == 0.0f || cost < best.cost) best = plan;
+        }
+    }
+    return best;
+}
+
+constexpr int64_t kFewRows = 64;
+
+// At most 64 rows: N outputs (gated: of one half).
+LinearPlan few_rows_plan(int64_t M, int64_t N, int64_t K, bool gated) {
+    const int rm = M > 32 ? 4 : M > 16 ? 2 : 1;
+    const LinearKernel kernel = M > 32 ? kFewRows64 : M > 16 ? kFewRows32 : kFewRows16;
+    const int64_t tiles = ceil_div(N, few_rows_columns(gated));
+    LinearPlan plan{kernel, 1, tiles, gated ? rm : 2 * rm, int64_t{2048} * rm, 0.0f};
+    while (plan.splits < 8 && tiles * plan.splits * 2 <= 2 * kCUs && ceil_div(K, 128) / (plan.splits * 2) >= 8) plan.splits *= 2;
+    if (!splits_fit(plan)) plan.splits = 1;
+    return plan;
+}
+
+LinearPlan gated_plan(int64_t M, int64_t F, int64_t K) {
+    return M <= kFewRows ? few_rows_plan(M, F, K, true) : tile_plan(M, 2 * ceil_div(F, 64) * 64, K);
+}
+
+int64_t workspace_of(const LinearPlan& plan) {
+    return plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
+}
+
+// Whether a plan's launch has fewer than 2^32 threads.
+bool launchable(const LinearPlan& plan) {
+    return plan.tiles * plan.splits <= kMaxThreads / (plan.kernel >= kFewRows16 ? 512 : 256);
+}
+
+bool sizes_ok(int64_t M, int64_t N, int64_t K) {
+    return M >= 1 && M <= kMaxSize / 4 && N >= 1 && N <= kMaxSize / 8 && K >= 1 && K <= kMaxDepth &&
+           ceil_div(M, 128) * ceil_div(N, 128) <= kMaxSize / 16;
+}
+
+bool operand_ok(const void* p, int64_t ld, int64_t cols) {
+    return p && on_16(p) && ld % 8 == 0 && ld >= cols && ld <= kMaxDepth;
+}
+
+bool half_type(int type) { return type == FEATHER_BF16 || type == FEATHER_FP16; }
+
+bool output_ok(const void* p, int64_t ld, int64_t cols, int type) {
+    return p && ld >= cols && ld <= kMaxSize / 4 && aligned_to_type(p, type);
+}
+
+bool workspace_ok(const void* workspace, int64_t bytes, int64_t need) {
+    return need == 0 || (workspace && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0);
+}
+
+void use_workspace(LinearParams& p, void* workspace) {
+    p.split_ctr = static_cast<uint32_t*>(workspace);
+    p.split_part = workspace ? static_cast<uint8_t*>(workspace) + kCtrBytes : nullptr;
+}
+
+// ---- the gated block's elementwise backward ----
+//
+//   grad_gate = dy up act'(gate)     grad_up = dy act(gate)
+//
+// A lane takes 8 columns of both halves of kRows rows, one after the other, and keeps their sums. Memory bounds it.
+constexpr int kThreads = 256;
+constexpr int kRows = 32;
+
+struct BackwardParams {
+    const uint16_t* grad_y;
+    const float* kept;
+    uint16_t* grad;
+    float* sums;
+    int64_t ld_grad_y, ld_kept, ld_grad;
+    int32_t rows, cols, act;
+};
+
+template <int kType, int kAct>
+__device__ __forceinline__ void backward_rows(const BackwardParams& p, int at, int valid, int row0, int row1) {
+    const int half = (p.cols + 7) & ~7;
+    float sum_gate[kPiece] = {}, sum_up[kPiece] = {};
+    const bool last = at + kPiece >= p.cols;
+#pragma unroll 2
+    for (int row = row0; row < row1; ++row) {
+        const float* const kept = p.kept + row * p.ld_kept + at;
+        float dy[kPiece], gate[kPiece], up[kPiece];
+        load_piece<kType, false>(p.grad_y + row * p.ld_grad_y, at, valid, dy);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 g = *reinterpret_cast<const f32x4*>(kept + 4 * h);
+            const f32x4 u = *reinterpret_cast<const f32x4*>(kept + half + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                gate[4 * h + e] = g[e];
+                up[4 * h + e] = u[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) {
+            const Slope s = activate_with_slope<kAct>(gate[e]);
+            // the slope first: of a gate masked with the type's lowest value it is 0, and dy up may be infinite
+            gate[e] = dy[e] * s.slope * up[e];
+            up[e] = dy[e] * s.value;
+            sum_gate[e] += gate[e];
+            sum_up[e] += up[e];
+        }
+        uint16_t* const out = p.grad + row * p.ld_grad;
+        store_piece<kType, false>(out, at, valid, gate);
+        store_piece<kType, false>(out + p.cols, at, valid, up);
+        if (last)
+            for (int c = 2 * p.cols; c < ((2 * p.cols + 7) & ~7); ++c) out[c] = 0;
+    }
+    if (p.sums) {
+        float* const out = p.sums + static_cast<int64_t>(row0 / kRows) * 2 * p.cols;
+        store_piece<FEATHER_FP32, false>(out, at, valid, sum_gate);
+        store_piece<FEATHER_FP32, false>(out + p.cols, at, valid, sum_up);
+    }
+}
+
+template <int kType>
+__global__ __launch_bounds__(kThreads) void gated_backward_kernel(const BackwardParams p) {
+    const int at = static_cast<int>(blockIdx.x * kThreads + threadIdx.x) * kPiece;
+    const int valid = p.cols - at;
+    if (valid <= 0) return;
+    const int row0 = static_cast<int>(blockIdx.y) * kRows;
+    const int row1 = row0 + kRows < p.rows ? row0 + kRows : p.rows;
+    if (p.act == kSilu) backward_rows<kType, kSilu>(p, at, valid, row0, row1);
+    else if (p.act == kGelu) backward_rows<kType, kGelu>(p, at, valid, row0, row1);
+    else backward_rows<kType, kGeluTanh>(p, at, valid, row0, row1);
+}
+
+}  // namespace
+}  // namespace feather
+
+using namespace feather;
+
+extern "C" int64_t feather_gated_linear_workspace_bytes(int64_t M, int64_t F, int64_t K) {
+    return sizes_ok(M, 2 * F, K) ? workspace_of(gated_plan(M, F, K)) : -1;
+}
+
+extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* weight, int64_t ld_weight, const void* bias,
+                                     int type, int activation, void* y, int64_t ldy, float* kept, int64_t ld_kept, int64_t M,
+                                     int64_t F, int64_t K, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+    const int64_t F8 = (F + 7) / 8 * 8;
+    if (F < 1 || !sizes_ok(M, 2 * F, K) || K % 8 != 0 || !half_type(type) || activation < 0 || activation > 2 ||
+        !operand_ok(x, ldx, K) || !operand_ok(weight, ld_weight, K) || !output_ok(y, ldy, F, type) ||
+        (bias && !aligned_to_type(bias, type)))
+        return false;
+    if (kept && (!on_16(kept) || ld_kept % 4 != 0 || ld_kept < 2 * F8 || ld_kept >= int64_t{1} << 22)) return false;
+    const LinearPlan plan = gated_plan(M, F, K);
+    const int64_t need = workspace_of(plan);
+    if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
+    LinearParams p{};
+    p.a = static_cast<const uint16_t*>(x);
+    p.b = static_cast<const uint16_t*>(weight);
+    p.lda = ldx;
+    p.ldb = ld_weight;
+    p.M = static_cast<int32_t>(M);
+    p.N = static_cast<int32_t>(F);
+    p.K = static_cast<int32_t>(K);
+    p.splits = plan.splits;
+    p.bias = bias;
+    p.c = y;
+    p.ldc = ldy;
+    p.h = kept;
+    p.ldh = ld_kept;
+    p.act = activation;
+    use_workspace(p, need > 0 ? workspace : nullptr);
+    (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(p, plan, kept ? Operands::kGatedKeep : Operands::kGated, stream);
+    return true;
+}
+
+extern "C" int64_t feather_gated_backward_parts(int64_t M, int64_t F) {
+    return M >= 1 && F >= 1 ? ceil_div(M, kRows) : 0;
+}
+
+extern "C" bool feather_gated_backward(const void* grad_y, int64_t ld_grad_y, const float* kept, int64_t ld_kept, int type,
+                                       int activation, void* grad, int64_t ld_grad, float* sums, int64_t M, int64_t F,
+                                       hipStream_t stream) {
+    const int64_t F8 = (F + 7) / 8 * 8;
+    if (M < 1 || M > kMaxSize || F < 1 || F > kMaxSize / 8 || !half_type(type) || activation < 0 || activation > 2 ||
+        !matrix_ok(grad_y, ld_grad_y, M, F) || !aligned_to_type(grad_y, type) || !kept || !on_16(kept) || ld_kept % 4 != 0 ||
+        ld_kept < 2 * F8 || !grad || !on_16(grad) || ld_grad % 8 != 0 || ld_grad < 2 * F || ceil_div(M, kRows) > 65535 * int64_t{32})
+        return false;
+    constexpr int64_t kMost = 65535;   // groups of rows of a launch
+    for (int64_t row = 0; row < M; row += kMost * kRows) {
+        BackwardParams p{static_cast<const uint16_t*>(grad_y) + row * ld_grad_y, kept + row * ld_kept,
+                         static_cast<uint16_t*>(grad) + row * ld_grad,
+                         sums ? sums + row / kRows * 2 * F : nullptr, ld_grad_y, ld_kept, ld_grad,
+                         static_cast<int32_t>(std::min(M - row, kMost * kRows)), static_cast<int32_t>(F), activation};
+        const dim3 groups(static_cast<uint32_t>(ceil_div(F8 / 8, kThreads)), static_cast<uint32_t>(ceil_div(p.rows, kRows)));
+        if (type == FEATHER_BF16) gated_backward_kernel<FEATHER_BF16><<<groups, kThreads, 0, stream>>>(p);
+        else gated_backward_kernel<FEATHER_FP16><<<groups, kThreads, 0, stream>>>(p);
+    }
+    return true;
+}
+
+extern "C" int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return sizes_ok(M, N, K) ? workspace_of(tile_plan(M, N, K)) : -1;
+}
+
+extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const void* b, int64_t ldb, bool b_across,
+                                const void* bias, int type, void* c, int64_t ldc, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                                hipStream_t stream) {
+    if (!sizes_ok(M, N, K) || !half_type(type) || (a_across && !b_across) || !operand_ok(a, lda, a_across ? M : K) ||
+        !operand_ok(b, ldb, b_across ? N : K) || !output_ok(c, ldc, N, type) || (bias && !aligned_to_type(bias, type)))
+        return false;
+    const LinearPlan plan = tile_plan(M, N, K);
+    const int64_t need = workspace_of(plan);
+    if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
+    LinearParams p{};
+    p.a = static_cast<const uint16_t*>(a);
+    p.b = static_cast<const uint16_t*>(b);
+    p.lda = lda;
+    p.ldb = ldb;
+    p.M = static_cast<int32_t>(M);
+    p.N = static_cast<int32_t>(N);
+    p.K = static_cast<int32_t>(K);
+    p.splits = plan.splits;
+    p.bias = bias;
+    p.c = c;
+    p.ldc = ldc;
+    use_workspace(p, need > 0 ? workspace : nullptr);
+    const Operands operands = a_across ? Operands::kBothAcross : b_across ? Operands::kBAcross : Operands::kAlong;
+    (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(p, plan, operands, stream);
+    return true;
+}
+
+// ---- 4-bit weights ----
+
+namespace {
+
+bool int4_ok(const uint8_t* codes, int64_t ld_codes, const void* scale, int64_t ld_scale, const uint8_t* zero, int64_t ld_zero,
+             int group, int type, int64_t rows, int64_t K) {
+    return codes && (reinterpret_cast<uintptr_t>(codes) & 3) == 0 && ld_codes % 4 == 0 && ld_codes >= (K + 1) / 2 &&
+           ld_codes <= 2 * kMaxDepth && scale && aligned_to_type(scale, type) && ld_scale >= std::max<int64_t>(rows, 4) &&
+           ld_scale <= kMaxSize && (!zero || (ld_zero >= std::max<int64_t>(rows, 4) && ld_zero <= kMaxSize)) &&
+           (group == 32 || group == 64 || group == 128);
+}
+
+}  // namespace
+
+extern "C" int64_t feather_int4_linear_rows(void) { return kFewRows; }
+
+extern "C" int64_t feather_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated) {
+    return M <= kFewRows && sizes_ok(M, gated ? 2 * N : N, K) ? workspace_of(few_rows_plan(M, N, K, gated)) : -1;
+}
+
+extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64_t ld_codes, const void* scale,
+                                    int64_t ld_scale, const uint8_t* zero, int64_t ld_zero, int group, const void* bias, int type,
+                                    bool gated, int activation, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                                    void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+    const int64_t rows = gated ? 2 * N : N;
+    if (N < 1 || M > kFewRows || !sizes_ok(M, rows, K) || !half_type(type) || activation < 0 || activation > 2 ||
+        !operand_ok(x, ldx, K) || !output_ok(y, ldy, N, type) || (bias && !aligned_to_type(bias, type)) ||
+        !int4_ok(codes, ld_codes, scale, ld_scale, zero, ld_zero, group, type, rows, K))
+        return false;
+    const LinearPlan plan = few_rows_plan(M, N, K, gated);
+    const int64_t need = workspace_of(plan);
+    if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
+    Int4Params p{};
+    p.a = static_cast<const uint16_t*>(x);
+    p.lda = ldx;
+    p.M = static_cast<int32_t>(M);
+    p.N = static_cast<int32_t>(N);
+    p.K = static_cast<int32_t>(K);
+    p.splits = plan.splits;
+    p.bias = bias;
+    p.c = y;
+    p.ldc = ldy;
+    p.act = activation;
+    use_workspace(p, need > 0 ? workspace : nullptr);
+    p.codes = codes;
+    p.scale = static_cast<const uint16_t*>(scale);
+    p.zero = zero;
+    p.ld_codes = ld_codes;
+    p.ld_scale = ld_scale;
+    p.ld_zero = ld_zero;
+    p.group = group;
+    (type == FEATHER_BF16 ? int4_launch_bf16 : int4_launch_fp16)(p, plan, gated, stream);
+    return true;
+}

@@ -19,6 +19,15 @@ from .block_scaled import (  # noqa: E402
 )
 from .convert import bf16_to_fp16  # noqa: E402
 from .gate import silu_mul, silu_mul_quantized  # noqa: E402
+from .gated import gated_linear  # noqa: E402
+from .int4 import (  # noqa: E402
+    Int4Linear,
+    dequantize_int4,
+    int4_gated_linear,
+    int4_linear,
+    quantize_int4,
+    to_int4_linear,
+)
 from .modules import ScaledMMLinear, relabel_modules, relabelled_class, to_scaled_mm_linear  # noqa: E402
 from .norm import rms_norm, rms_norm_quantized  # noqa: E402
 from .scaled_mm import (  # noqa: E402
@@ -33,13 +42,19 @@ from .scaled_mm import (  # noqa: E402
 
 __all__ = [
     "BlockScaledLinear",
+    "Int4Linear",
     "ScaledMMLinear",
     "bf16_to_fp16",
     "block_scaled_linear",
     "block_scaled_mm",
+    "dequantize_int4",
+    "gated_linear",
+    "int4_gated_linear",
+    "int4_linear",
     "prepack_b_for_scaled_mm",
     "prepack_transpose",
     "quantize_blocks",
+    "quantize_int4",
     "relabel_modules",
     "relabelled_class",
     "rms_norm",
@@ -52,5 +67,6 @@ __all__ = [
     "silu_mul_quantized",
     "tile_shape",
     "to_block_scaled_linear",
+    "to_int4_linear",
     "to_scaled_mm_linear",
 ]

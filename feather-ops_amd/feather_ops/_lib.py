@@ -1,7 +1,7 @@
 """Loading of the native code: `_C` (the torch library), through it `libfeather_ops_gfx950.so`, and `_autograd.so` (the
 autograd nodes of its ops). The first keeps to torch's stable interface, the last cannot, and may fail to load beside another
-torch than it was built for: then the operators that need it (`rms_norm`, `silu_mul`, `block_scaled_linear`) raise, and
-everything else works.
+torch than it was built for: then the operators that need it (`rms_norm`, `silu_mul`, `block_scaled_linear`, `gated_linear`,
+`int4_linear`) raise, and everything else works.
 
 There is no fallback: if the extension is not built, importing `feather_ops` fails with the build
 command, and the ops only have a CUDA (HIP) dispatch key, so CPU tensors are rejected by the dispatcher.
@@ -56,7 +56,11 @@ def _refuse_autograd(error: OSError) -> None:
     define = torch.library.Library("feather_ops", "FRAGMENT")
     define.define("block_scaled_linear(Tensor x, Tensor weight, Tensor? bias, bool e5m2, Tensor? weight_codes, "
                   "Tensor? weight_scale, Tensor? workspace) -> Tensor")
-    define.impl("block_scaled_linear", require_autograd, "CompositeImplicitAutograd")
+    define.define("gated_linear(Tensor x, Tensor weight, Tensor? bias, int activation, Tensor? workspace) -> Tensor")
+    define.define("int4_linear(Tensor x, Tensor codes, Tensor scale, Tensor? zero, Tensor? bias, int k, Tensor? workspace) "
+                  "-> Tensor")
+    for name in ("block_scaled_linear", "gated_linear", "int4_linear"):
+        define.impl(name, require_autograd, "CompositeImplicitAutograd")
     nodes = torch.library.Library("feather_ops", "IMPL", "AutogradCUDA")
     for name in ("silu_mul", "rms_norm"):
         nodes.impl(name, require_autograd)
@@ -84,6 +88,12 @@ def c_library() -> ctypes.CDLL:
                                                             [ctypes.c_bool, ctypes.c_int])
         lib.feather_block_scaled_mm_workspace_bytes.restype = ctypes.c_int64
         lib.feather_block_scaled_mm_workspace_bytes.argtypes = [ctypes.c_int64] * 3
+        for name, flags in (("gated_linear", []), ("product", []), ("int4_linear", [ctypes.c_bool])):
+            bytes_of = getattr(lib, f"feather_{name}_workspace_bytes")
+            bytes_of.restype = ctypes.c_int64
+            bytes_of.argtypes = [ctypes.c_int64] * 3 + flags
+        lib.feather_int4_linear_rows.restype = ctypes.c_int64
+        lib.feather_int4_linear_rows.argtypes = []
         _c_library = lib
     return _c_library
 

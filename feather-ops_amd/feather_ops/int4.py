@@ -1,0 +1,308 @@
+"""Products with 4-bit weights that have one scale for each group of columns, their quantization, and the layers on them; not in
+the reference, whose weights have 8 bits. Kernels: `csrc/linear_stream.h` (few rows), `csrc/linear_tile.h`, `csrc/int4.hip`; autograd
+node: `csrc/linear_autograd.cpp`. C ABI: `include/feather_linear_ops.h`.
+
+A quantized weight is `(codes, scale, zero)`: value (n, k) is `(q - zero) * scale` with the code q, 0 .. 15, and the scale and zero
+point of its group of 32, 64 or 128 columns.
+
+- codes: uint8 `[N, ceil(K / 2)]`, two columns to a byte, the even one in the low half;
+- scale: `[N, ceil(K / group)]` in the activations' dtype, best stored group by group (`scale.t()` is contiguous);
+- zero: uint8 like scale, 0 .. 15; or None: 8.
+"""
+
+import functools
+from collections.abc import Callable
+
+import torch
+from torch import nn
+
+from . import _lib
+from .block_scaled import _plain, _workspace, as_rows
+from .gate import silu_mul
+from .gated import HALVES, _workspace_bytes as _gated_workspace_bytes, activate, activation_number, operand
+from .modules import relabel_modules
+
+GROUPS = (32, 64, 128)
+Int4Weight = tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]
+
+
+def quantize_int4(weight: torch.Tensor, group: int = 128, *, zeros: bool = False) -> Int4Weight:
+    """(codes, scale, zero) of a bfloat16 or float16 weight `[N, K]`. A group's scale is its largest magnitude / 7 (zero is then
+    None) or, with `zeros`, its range (extended to 0) / 15, rounded to the weight's dtype; codes are the nearest. Not
+    differentiable."""
+    if weight.dim() != 2 or weight.dtype not in HALVES:
+        raise ValueError(f"weight must be a bfloat16 or float16 matrix, got {tuple(weight.shape)} {weight.dtype}")
+    if group not in GROUPS:
+        raise ValueError(f"group must be one of {GROUPS}, got {group}")
+    n, k = weight.shape
+    w = as_rows(_plain(weight))
+    if w.numel() == 0:
+        shape = (n, -(-k // group))
+        return (w.new_empty((n, -(-k // 2)), dtype=torch.uint8), w.new_empty(shape),
+                w.new_empty(shape, dtype=torch.uint8) if zeros else None)
+    codes, scale, zero = torch.ops.feather_ops.int4_quantize.default(w, group, zeros)
+    return codes[:, : -(-k // 2)], scale[:, :n].t(), zero[:, :n].t() if zeros else None
+
+
+def _group_of(k: int, groups: int) -> int:
+    for group in GROUPS:
+        if -(-k // group) == groups:
+            return group
+    raise ValueError(f"scale must have one column for each group of 32, 64 or 128 columns of {k}, got {groups}")
+
+
+def _grouped(t: torch.Tensor) -> torch.Tensor:
+    """[N, groups] stored group by group, 4 values to a group at least (copied where it is not)."""
+    n, groups = t.shape
+    if (n <= 1 or t.stride(0) == 1) and (max(n, t.stride(1)) if groups <= 1 else t.stride(1)) >= max(n, 4):
+        return t
+    out = t.new_empty((groups, -(-n // 4) * 4))[:, :n].t()
+    return out.copy_(t)
+
+
+def _whole_bytes(codes: torch.Tensor) -> torch.Tensor:
+    """Codes with rows on 4-byte boundaries that can be read to the next one (copied where they cannot)."""
+    n, cols = codes.shape
+    pitch, step = codes.stride()
+    whole = -(-cols // 4) * 4
+    if (step == 1 or cols <= 1) and codes.storage_offset() % 4 == 0 and ((pitch % 4 == 0 and whole <= pitch <= 1 << 22) or n <= 1):
+        end = codes.storage_offset() + (n - 1) * pitch + whole
+        if whole == cols or end <= codes.untyped_storage().nbytes():
+            return codes
+    out = codes.new_empty((n, -(-cols // 16) * 16))[:, :cols]
+    return out.copy_(codes)
+
+
+def _check(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, k: int) -> None:
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] != -(-k // 2):
+        raise ValueError(f"codes must be uint8 [N, {-(-k // 2)}], two columns to a byte, got {tuple(codes.shape)} {codes.dtype}")
+    if scale.dim() != 2 or scale.shape[0] != codes.shape[0] or not scale.dtype.is_floating_point:
+        raise ValueError(f"scale must be [{codes.shape[0]}, groups], got {tuple(scale.shape)} {scale.dtype}")
+    _group_of(k, scale.shape[1])
+    if scale.requires_grad:
+        raise ValueError("a quantized weight takes no gradients")
+    if zero is not None:
+        if zero.dtype != torch.uint8 or zero.shape != scale.shape:
+            raise ValueError(f"zero must be uint8 {tuple(scale.shape)}, got {tuple(zero.shape)} {zero.dtype}")
+
+
+def _laid_out(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, dtype: torch.dtype) -> Int4Weight:
+    """A weight as the kernels read it, with scales in `dtype`: itself where it is."""
+    return _whole_bytes(codes), _grouped(scale.to(dtype)), None if zero is None else _grouped(zero)
+
+
+def dequantize_int4(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None,
+                    k: int | None = None) -> torch.Tensor:
+    """The weight `[N, K]` that codes stand for, in scale's dtype (bfloat16 or float16), each value rounded once. k: the columns,
+    where they are odd (None: twice the bytes of a row). Not differentiable."""
+    if codes.dim() != 2:
+        raise ValueError(f"codes must be a matrix, got {codes.dim()} dimensions")
+    k = 2 * codes.shape[1] if k is None else k
+    if scale.dtype not in HALVES:
+        raise ValueError(f"scale must be bfloat16 or float16, got {scale.dtype}")
+    if codes.shape[0] == 0 or k == 0:
+        return scale.new_empty((codes.shape[0], k))
+    scale = _plain(scale)
+    _check(codes, scale, zero, k)
+    return torch.ops.feather_ops.int4_dequantize.default(*_laid_out(codes, scale, zero, scale.dtype), k)[:, :k]
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(M: int, rows: int, K: int, gated: bool, trains: bool) -> int:
+    lib = _lib.c_library()
+    n, k8 = rows // 2 if gated else rows, -(-K // 8) * 8
+    if M <= lib.feather_int4_linear_rows():
+        need = lib.feather_int4_linear_workspace_bytes(M, n, K, gated)
+    elif gated:
+        need = _gated_workspace_bytes(M, n, k8, False)
+    else:
+        need = lib.feather_product_workspace_bytes(M, n, k8)
+    return max(0, need, lib.feather_product_workspace_bytes(M, K, rows) if trains else 0)
+
+
+def _prepared(x: torch.Tensor, codes: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor | None:
+    """Checks of x and bias; the bias as the kernels take it."""
+    if x.dtype not in HALVES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    if bias is None:
+        return None
+    if bias.shape != codes.shape[:1]:
+        raise ValueError(f"bias must have {codes.shape[0]} values, got {tuple(bias.shape)}")
+    return bias.to(x.dtype).contiguous()
+
+
+def int4_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None,
+                bias: torch.Tensor | None = None) -> torch.Tensor:
+    """`x @ W^T + bias` with a 4-bit weight W `[N, K]`: x `[..., K]`, the result `[..., N]`, both bfloat16 or float16; bias `[N]`.
+
+    Up to 64 rows take the codes as they are, each group's sum times its scale in fp32; more take W rounded to x's dtype. The
+    result is rounded once. Differentiable once, in reverse mode, in x and bias (the weight is frozen): dx = dy @ W with W rounded
+    to x's dtype. Scales in another dtype than x's, scales and zero points that are not stored group by group, codes whose rows do
+    not start on 4-byte boundaries, and rows of x off 16-byte boundaries or of no multiple of 8 values are copied on every call.
+    K is at most 2**21."""
+    bias = _prepared(x, codes, bias)
+    k = x.shape[-1]
+    _check(codes, scale, zero, k)
+    if x.numel() == 0 or codes.numel() == 0:
+        return nn.functional.linear(x, x.new_zeros((codes.shape[0], k)), bias)
+    if torch.compiler.is_compiling():
+        return _int4_linear_auto(x, codes, scale, zero, bias)
+    return _linear(x, codes, scale, zero, bias)
+
+
+def _linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
+            bias: torch.Tensor | None) -> torch.Tensor:
+    trains = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))
+    k = x.shape[-1]
+    rows = operand(as_rows(x))
+    codes, scale, zero = _laid_out(codes, scale, zero, x.dtype)
+    need = _workspace_bytes(int(rows.shape[0]), int(codes.shape[0]), int(k), False, trains)
+    y = torch.ops.feather_ops.int4_linear.default(rows, codes, scale, zero, bias, k, _workspace(rows, need) if need else None)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+def int4_gated_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None,
+                      bias: torch.Tensor | None = None, activation: str = "silu") -> torch.Tensor:
+    """`gated_linear` with a 4-bit weight of 2 F rows, the gates' first: x `[..., K]`, the result `[..., F]`, in one launch up to 64
+    rows. Where x or bias takes gradients it is `int4_linear` and the activation of its outputs, in x's dtype."""
+    act = activation_number(activation)
+    bias = _prepared(x, codes, bias)
+    if codes.dim() != 2 or codes.shape[0] % 2:
+        raise ValueError(f"codes must have an even number of rows, the gates' and the others', got {tuple(codes.shape)}")
+    trains = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))
+    if x.numel() == 0 or codes.numel() == 0 or trains:
+        h = int4_linear(x, codes, scale, zero, bias)
+        if act == 0:
+            return silu_mul(h)
+        gate, up = h.chunk(2, -1)
+        return activate(gate, act) * up
+    _check(codes, scale, zero, x.shape[-1])
+    if torch.compiler.is_compiling():
+        return _int4_gated_auto(x, codes, scale, zero, bias, act)
+    return _gated(x, codes, scale, zero, bias, act)
+
+
+def _gated(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, bias: torch.Tensor | None,
+           act: int) -> torch.Tensor:
+    k = x.shape[-1]
+    rows = operand(as_rows(_plain(x)))
+    codes, scale, zero = _laid_out(codes, scale, zero, x.dtype)
+    need = _workspace_bytes(int(rows.shape[0]), int(codes.shape[0]), int(k), True, False)
+    y = torch.ops.feather_ops.int4_forward.default(rows, codes, scale, zero, bias, k, True, act,
+                                                   _workspace(rows, need) if need else None)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+class Int4Linear:
+    """Mixin for `nn.Linear` (via `relabel_modules`): `forward` is `int4_linear` with the weight as it was when `quantize_weight_`
+    was called, 16-bit in and out. It is kept in three non-persistent buffers, `weight_int4`, `weight_scale` and `weight_zero`;
+    parameters and `state_dict` stay as they were. The weight is frozen; gradients reach the input and the bias, so the layer can
+    sit under trainable adapters."""
+
+    def quantize_weight_(self, group: int = 128, zeros: bool = False) -> None:
+        codes, scale, zero = quantize_int4(self.weight, group, zeros=zeros)
+        self.register_buffer("weight_int4", codes, persistent=False)
+        self.register_buffer("weight_scale", scale, persistent=False)
+        self.register_buffer("weight_zero", zero, persistent=False)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int4_linear(x, self.weight_int4, self.weight_scale, self.weight_zero, self.bias)
+
+
+def to_int4_linear(root: nn.Module, group: int = 128, zeros: bool = False,
+                   accept: Callable[[nn.Module], bool] | None = None) -> int:
+    """Relabel the `nn.Linear` modules under `root` (those `accept` approves, by default every one with a bfloat16 or float16
+    weight) as `Int4Linear`, quantize their weights and return how many changed."""
+    def default_accept(module: nn.Module) -> bool:
+        return isinstance(module, nn.Linear) and module.weight.dtype in HALVES
+
+    count = relabel_modules(root, Int4Linear, accept or default_accept)
+    for module in root.modules():
+        if isinstance(module, Int4Linear) and not hasattr(module, "weight_int4"):
+            module.quantize_weight_(group, zeros)
+    return count
+
+
+# ---- one node each under torch.compile ----
+
+
+@torch.library.custom_op("feather_ops::int4_linear_auto", mutates_args=())
+def _int4_linear_auto(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
+                      bias: torch.Tensor | None) -> torch.Tensor:
+    """int4_linear as one opaque op."""
+    return _linear(x, codes, scale, zero, bias)
+
+
+@_int4_linear_auto.register_fake
+def _(x, codes, scale, zero, bias):
+    return x.new_empty((*x.shape[:-1], codes.shape[0]))
+
+
+@torch.library.custom_op("feather_ops::int4_linear_auto_backward", mutates_args=())
+def _int4_linear_auto_backward(grad: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
+                               k: int) -> torch.Tensor:
+    rows = operand(as_rows(grad))
+    codes, scale, zero = _laid_out(codes, scale, zero, grad.dtype)
+    need = max(0, _lib.c_library().feather_product_workspace_bytes(rows.shape[0], k, codes.shape[0]))
+    dx = torch.ops.feather_ops.int4_backward.default(rows, codes, scale, zero, k, _workspace(rows, need) if need else None)
+    return dx.reshape(*grad.shape[:-1], k)
+
+
+@_int4_linear_auto_backward.register_fake
+def _(grad, codes, scale, zero, k):
+    return grad.new_empty((*grad.shape[:-1], k))
+
+
+def _linear_auto_context(ctx, inputs, output) -> None:
+    x, codes, scale, zero, _ = inputs
+    ctx.save_for_backward(codes, scale, zero)
+    ctx.k = x.shape[-1]
+
+
+def _linear_auto_backward(ctx, grad: torch.Tensor) -> tuple:
+    need_x, _, _, _, need_bias = ctx.needs_input_grad
+    dx = _int4_linear_auto_backward(grad, *ctx.saved_tensors, ctx.k) if need_x else None
+    return dx, None, None, None, grad.float().sum(tuple(range(grad.dim() - 1))).to(grad.dtype) if need_bias else None
+
+
+_int4_linear_auto.register_autograd(_linear_auto_backward, setup_context=_linear_auto_context)
+
+
+@torch.library.custom_op("feather_ops::int4_gated_auto", mutates_args=())
+def _int4_gated_auto(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
+                     bias: torch.Tensor | None, act: int) -> torch.Tensor:
+    """int4_gated_linear as one opaque op."""
+    return _gated(x, codes, scale, zero, bias, act)
+
+
+@_int4_gated_auto.register_fake
+def _(x, codes, scale, zero, bias, act):
+    return x.new_empty((*x.shape[:-1], codes.shape[0] // 2))
+
+
+# ---- shapes, for tracing ----
+
+
+@torch.library.register_fake("feather_ops::int4_forward")
+def _(x, codes, scale, zero, bias, k, gated, activation, workspace):
+    return x.new_empty((x.shape[0], codes.shape[0] // 2 if gated else codes.shape[0]))
+
+
+@torch.library.register_fake("feather_ops::int4_backward")
+def _(grad_y, codes, scale, zero, k, workspace):
+    return grad_y.new_empty((grad_y.shape[0], k))
+
+
+@torch.library.register_fake("feather_ops::int4_quantize")
+def _(weight, group, zeros):
+    n, k = weight.shape
+    ld, groups = (n + 3) // 4 * 4, (k + group - 1) // group
+    return (weight.new_empty((n, ((k + 1) // 2 + 15) // 16 * 16), dtype=torch.uint8), weight.new_empty((groups, ld)),
+            weight.new_empty((groups, ld) if zeros else (0, 0), dtype=torch.uint8))
+
+
+@torch.library.register_fake("feather_ops::int4_dequantize")
+def _(codes, scale, zero, k):
+    return scale.new_empty((codes.shape[0], (k + 7) // 8 * 8))

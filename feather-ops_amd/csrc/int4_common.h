@@ -2,7 +2,7 @@
 // 0 .. 15 two to a byte, the even k in the low half.
 //
 // A dword holds 8 codes of consecutive k. They become 16-bit values two at a time, in the order 0 4 1 5 2 6 3 7, by putting a
-// code's bits into the mantissa of a power of two: fp16 1024 + q, whose 1024 + 8 is taken off again, exactly; bf16 128 + q, which
+// code's bits into the mantissa of a power of two: fp16 1024 + q, whose 1024 + z is taken off again, exactly; bf16 128 + q, which
 // stays (there is no packed bf16 arithmetic): its 128 + z, times the sum of x, is taken off the group's sum in fp32.
 // Activations are put into the same order.
 #pragma once
@@ -19,41 +19,44 @@ struct Int4Params : LinearParams {   // b: unused
     int32_t group;              // 32, 64 or 128
 };
 
-// The constant that a group's codes are off their value by, as the matrix cores see them: z - kCodeBias.
+// What decode8 keeps in registers: the powers of two that codes are put into and, fp16, what is taken off again: of the low
+// nibbles 1024 + z, of the high ones, which stay in their place, 64 + z.
 template <bool kBf16>
-constexpr float kCodeBias = kBf16 ? -128.0f : 8.0f;
+struct Decode {
+    uint32_t one, low, high;
 
-// What decode8 keeps in a register. (The compiler would rather spend two instructions on literals.)
-template <bool kBf16>
-__device__ __forceinline__ uint32_t code_one() {
-    uint32_t one = kBf16 ? 0x43004300u : 0x64006400u;   // 128, 1024
-    asm volatile("" : "+v"(one));
-    return one;
-}
-
-// 8 codes -> 8 values code - 8 (fp16) or code + 128 (bf16), in the order 0 4 1 5 2 6 3 7.
-template <bool kBf16>
-__device__ __forceinline__ half8 decode8(uint32_t w, uint32_t one) {
-    constexpr uint32_t kLow = 0x000f000fu;
-    const auto insert = [&](uint32_t v, uint32_t mask) { return (v & mask) | one; };
-    if constexpr (kBf16) {
-        return __builtin_bit_cast(half8, u32x4{insert(w, kLow), insert(w >> 4, kLow), insert(w >> 8, kLow), insert(w >> 12, kLow)});
-    } else {
-        // The high nibbles stay in their place: 1024 + 16 q, divided and shifted by one multiply-add.
-        const uint32_t u = w >> 8;
-        const half2v less{static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
-        const half2v part{static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-        const half2v less16{static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
-        const auto low = [&](uint32_t v) {
-            return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, insert(v, kLow)) + less);
-        };
-        const auto high = [&](uint32_t v) {
-            return __builtin_bit_cast(uint32_t,
-                                      __builtin_elementwise_fma(__builtin_bit_cast(half2v, insert(v, kLow << 4)), part, less16));
-        };
-        return __builtin_bit_cast(half8, u32x4{low(w), high(w), low(u), high(u)});
+    __device__ __forceinline__ void init() {
+        one = kBf16 ? 0x43004300u : 0x64006400u;   // 128, 1024
+        asm volatile("" : "+v"(one));              // (the compiler would rather spend two instructions on literals)
+        low = 0x64086408u;                         // 1032
+        high = 0x54805480u;                        // 72
     }
-}
+    // fp16: codes of a row with zero point z.
+    __device__ __forceinline__ void set_zero(uint32_t z) {
+        z |= z << 16;
+        low = 0x64006400u | z;
+        high = 0x54005400u | z << 4;
+    }
+    // 8 codes -> 8 values code - z (fp16) or code + 128 (bf16), in the order 0 4 1 5 2 6 3 7.
+    __device__ __forceinline__ half8 operator()(uint32_t w) const {
+        constexpr uint32_t kLow = 0x000f000fu;
+        const auto insert = [&](uint32_t v, uint32_t mask) { return (v & mask) | one; };
+        if constexpr (kBf16) {
+            return __builtin_bit_cast(half8, u32x4{insert(w, kLow), insert(w >> 4, kLow), insert(w >> 8, kLow), insert(w >> 12, kLow)});
+        } else {
+            const uint32_t u = w >> 8;
+            const half2v part{static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+            const auto at_low = [&](uint32_t v) {
+                return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, insert(v, kLow)) - __builtin_bit_cast(half2v, low));
+            };
+            const auto at_high = [&](uint32_t v) {   // 1024 + 16 q
+                return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, insert(v, kLow << 4)), part,
+                                                                              -__builtin_bit_cast(half2v, high)));
+            };
+            return __builtin_bit_cast(half8, u32x4{at_low(w), at_high(w), at_low(u), at_high(u)});
+        }
+    }
+};
 
 // 8 activations into the codes' order.
 __device__ __forceinline__ half8 order8(u32x4 v) {
@@ -62,10 +65,10 @@ __device__ __forceinline__ half8 order8(u32x4 v) {
                                            __builtin_amdgcn_perm(v[3], v[1], kLow), __builtin_amdgcn_perm(v[3], v[1], kHigh)});
 }
 
-// 8 times 1, or (bf16) -136, what takes a code + 128 to code - 8.
-template <bool kBf16, bool kOffset>
+// bf16: 8 times -136, what takes a code + 128 to code - 8, or 1.
+template <bool kOffset>
 __device__ __forceinline__ half8 constant8() {
-    constexpr uint32_t k = kOffset ? 0xc308c308u : kBf16 ? 0x3f803f80u : 0x3c003c00u;
+    constexpr uint32_t k = kOffset ? 0xc308c308u : 0x3f803f80u;
     return __builtin_bit_cast(half8, u32x4{k, k, k, k});
 }
 
@@ -92,26 +95,19 @@ __device__ __forceinline__ ScaleAt scale_at(int n, int N) {
 }
 
 template <bool kBf16>
-__device__ __forceinline__ f32x4 scales4(u32x2 raw, bool edge, uint32_t shift) {
-    if (edge) {
-        asm volatile("");   // a branch, and not selects for every other workgroup
-        const uint64_t v = (static_cast<uint64_t>(raw[1]) << 32 | raw[0]) >> (16 * shift & 63);
-        raw = u32x2{static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32)};
-    }
+__device__ __forceinline__ f32x4 scales4(u32x2 raw, uint32_t shift) {
+    const uint64_t v = (static_cast<uint64_t>(raw[1]) << 32 | raw[0]) >> (16 * shift & 63);
+    const auto lo = static_cast<uint32_t>(v), hi = static_cast<uint32_t>(v >> 32);
     constexpr int kType = kTypeOf<kBf16>;
     if constexpr (kBf16) {
-        return f32x4{to_float<kType>(raw[0] & 0xffffu), __builtin_bit_cast(float, raw[0] & 0xffff0000u),
-                     to_float<kType>(raw[1] & 0xffffu), __builtin_bit_cast(float, raw[1] & 0xffff0000u)};
+        return f32x4{to_float<kType>(lo & 0xffffu), __builtin_bit_cast(float, lo & 0xffff0000u), to_float<kType>(hi & 0xffffu),
+                     __builtin_bit_cast(float, hi & 0xffff0000u)};
     }
-    return f32x4{to_float<kType>(raw[0] & 0xffffu), to_float<kType>(raw[0] >> 16), to_float<kType>(raw[1] & 0xffffu),
-                 to_float<kType>(raw[1] >> 16)};
+    return f32x4{to_float<kType>(lo & 0xffffu), to_float<kType>(lo >> 16), to_float<kType>(hi & 0xffffu), to_float<kType>(hi >> 16)};
 }
 
-__device__ __forceinline__ f32x4 zeros4(uint32_t raw, bool edge, uint32_t shift) {
-    if (edge) {
-        asm volatile("");
-        raw >>= 8 * shift & 31;
-    }
+__device__ __forceinline__ f32x4 zeros4(uint32_t raw, uint32_t shift) {
+    raw >>= 8 * shift & 31;
     return f32x4{static_cast<float>(raw & 255u), static_cast<float>(raw >> 8 & 255u), static_cast<float>(raw >> 16 & 255u),
                  static_cast<float>(raw >> 24)};
 }

@@ -1,35 +1,43 @@
 // The 4-bit products' kernels of one activation type: compiled with FEATHER_LINEAR_BF16 set to 0 (fp16) or 1 (bf16).
+#include "linear_few.h"
 #include "linear_launch.h"
-#include "linear_stream.h"
 
 namespace feather {
 namespace {
 
 constexpr bool kBf16 = FEATHER_LINEAR_BF16 != 0;
 
-template <int RM, int kGroups, bool kZeros, Form kForm>
+template <typename T, int kGroups, bool kZeros, Form kForm>
 void few(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
-    using T = LinearStream<RM, 2, 8, 2>;
-    linear_stream_kernel<T, kGroups, kZeros, kForm, kBf16>
+    few_rows_kernel<T, kGroups, kZeros, kForm, kBf16>
         <<<dim3(static_cast<uint32_t>(plan.tiles), plan.splits), T::kThreads, 0, stream>>>(p);
 }
 
-template <int kGroups, bool kZeros, Form kForm>
-void by_rows(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
-    if (plan.kernel == kFewRows16) few<1, kGroups, kZeros, kForm>(p, plan, stream);
-    else if (plan.kernel == kFewRows32) few<2, kGroups, kZeros, kForm>(p, plan, stream);
-    else few<4, kGroups, kZeros, kForm>(p, plan, stream);
+template <int kGroups, bool kZeros>
+void plain(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
+    constexpr Form kForm = Form::kPlain;
+    if (plan.kernel == kFew16_1_16_1) few<FewRows<1, 1, 16, 1>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew16_1_8_2) few<FewRows<1, 1, 8, 2>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew16_2_8_1) few<FewRows<1, 2, 8, 1>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew32_1_4_4) few<FewRows<2, 1, 4, 4>, kGroups, kZeros, kForm>(p, plan, stream);
+    else few<FewRows<4, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
+}
+
+template <int kGroups, bool kZeros>
+void gated(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
+    constexpr Form kForm = Form::kGated;
+    if (plan.kernel == kFew16_2_4_2) few<FewRows<1, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew16_2_8_1) few<FewRows<1, 2, 8, 1>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew16_2_16_1) few<FewRows<1, 2, 16, 1>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew32_2_4_4) few<FewRows<2, 2, 4, 4>, kGroups, kZeros, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew32_2_4_2) few<FewRows<2, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
+    else few<FewRows<4, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
 }
 
 template <int kGroups>
-void by_group(const Int4Params& p, const LinearPlan& plan, bool gated, hipStream_t stream) {
-    if (p.zero) {
-        if (gated) by_rows<kGroups, true, Form::kGated>(p, plan, stream);
-        else by_rows<kGroups, true, Form::kPlain>(p, plan, stream);
-    } else {
-        if (gated) by_rows<kGroups, false, Form::kGated>(p, plan, stream);
-        else by_rows<kGroups, false, Form::kPlain>(p, plan, stream);
-    }
+void by_group(const Int4Params& p, const LinearPlan& plan, bool gate, hipStream_t stream) {
+    if (p.zero) (gate ? gated<kGroups, true> : plain<kGroups, true>)(p, plan, stream);
+    else (gate ? gated<kGroups, false> : plain<kGroups, false>)(p, plan, stream);
 }
 
 }  // namespace

@@ -1,6 +1,6 @@
 // The 16-bit products' kernels of one operand type: compiled with FEATHER_LINEAR_BF16 set to 0 (fp16) or 1 (bf16).
+#include "linear_few.h"
 #include "linear_launch.h"
-#include "linear_stream.h"
 #include "linear_tile.h"
 
 namespace feather {
@@ -21,18 +21,18 @@ void tiles(const LinearParams& p, const LinearPlan& plan, hipStream_t stream) {
     else tile<LinearTile<128, 128>, kAAcross, kBAcross, kForm>(p, plan, stream);
 }
 
-template <int RM, int kWaves, int kDepth, Form kForm>
+template <typename T, Form kForm>
 void few(const LinearParams& p, const LinearPlan& plan, hipStream_t stream) {
-    using T = LinearStream<RM, 2, kWaves, kDepth>;
-    linear_stream_kernel<T, 0, false, kForm, kBf16>
+    few_rows_kernel<T, 0, false, kForm, kBf16>
         <<<dim3(static_cast<uint32_t>(plan.tiles), plan.splits), T::kThreads, 0, stream>>>(p);
 }
 
 template <Form kForm>
 void gated(const LinearParams& p, const LinearPlan& plan, hipStream_t stream) {
-    if (plan.kernel == kFewRows16) few<1, 8, 2, kForm>(p, plan, stream);
-    else if (plan.kernel == kFewRows32) few<2, 8, 2, kForm>(p, plan, stream);
-    else if (plan.kernel == kFewRows64) few<4, 8, 2, kForm>(p, plan, stream);
+    if (plan.kernel == kFew16_2_8_1) few<FewRows<1, 2, 8, 1>, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew32_4_4_2) few<FewRows<2, 4, 4, 2>, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew32_2_4_2) few<FewRows<2, 2, 4, 2>, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew64_2_4_2) few<FewRows<4, 2, 4, 2>, kForm>(p, plan, stream);
     else tiles<false, false, kForm>(p, plan, stream);
 }
 

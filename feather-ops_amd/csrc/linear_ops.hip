@@ -45,7 +45,7 @@ LinearPlan tile_plan(int64_t M, int64_t N, int64_t K) {
     for (const TileCost& t : kTiles) {
         const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
         for (const int splits : kSplits) {
-            LinearPlan plan{t.kernel, splits, tiles, 4, int64_t{4} * t.bm * t.bn, 0.0f};
+            LinearPlan plan{t.kernel, splits, tiles, 256, 4, int64_t{4} * t.bm * t.bn, 0.0f};
             if (splits > 1 && (splits > all || tiles * splits > 4 * kCUs || !splits_fit(plan))) break;
             const auto stages = static_cast<float>(ceil_div(all, splits));
             const int64_t groups = tiles * splits;
@@ -65,19 +65,50 @@ LinearPlan tile_plan(int64_t M, int64_t N, int64_t K) {
 
 constexpr int64_t kFewRows = 64;
 
-// At most 64 rows: N outputs (gated: of one half).
-LinearPlan few_rows_plan(int64_t M, int64_t N, int64_t K, bool gated) {
-    const int rm = M > 32 ? 4 : M > 16 ? 2 : 1;
-    const LinearKernel kernel = M > 32 ? kFewRows64 : M > 16 ? kFewRows32 : kFewRows16;
-    const int64_t tiles = ceil_div(N, few_rows_columns(gated));
-    LinearPlan plan{kernel, 1, tiles, gated ? rm : 2 * rm, int64_t{2048} * rm, 0.0f};
-    while (plan.splits < 8 && tiles * plan.splits * 2 <= 2 * kCUs && ceil_div(K, 128) / (plan.splits * 2) >= 8) plan.splits *= 2;
+// At most 64 rows, N outputs (gated: of one half). Workgroups by their columns of output; K is split over more of them where that
+// still leaves `least` steps of 128 to each and no more than 256 in all.
+LinearPlan few_plan(LinearKernel kernel, int rm, int rn, int wk, int wn, int64_t N, int64_t K, bool gated, int least) {
+    const int64_t tiles = ceil_div(N, 16 * (gated ? rn / 2 : rn) * wn);
+    LinearPlan plan{kernel, 1, tiles, 64 * wk * wn, rm * rn * wn / (gated ? 2 : 1), int64_t{1024} * rm * rn * wn, 0.0f};
+    while (plan.splits < 8 && tiles * plan.splits * 2 <= kCUs && ceil_div(K, 128) / (plan.splits * 2) >= least) plan.splits *= 2;
     if (!splits_fit(plan)) plan.splits = 1;
     return plan;
 }
 
+// Measured in us, groups of 128, weights from HBM; RN_WK_WN, "/s" K splits.
+//   4 bits, 1 row: 4096 x 4096 1_16_1 6.2, 1_8_1 6.9, 2_8_1 7.8; 4096 x 14336 1_16_1 11.3, 1_8_1/2 12.5; 8192 x 8192 1_8_2 12.0, 2_8_1
+//   13.2, 1_16_1 16.6; 14336 x 4096 2_8_1 10.4, 2_4_2 11.5, 1_8_2 13.0. Gated, 1 row: 14336 x 4096 2_4_2 16.4, 2_8_1 19.6; 8192 x
+//   8192 2_8_1 19.1, 2_4_2 20.4; 2048 x 16384 2_16_1 15.7, 2_8_1 19.8.
+//   24 rows: 13824 x 5120 1_4_4 17.9, 2_4_4/2 19.3, 2_4_2 19.4; 5120 x 13824 1_4_4/2 22.2, /4 25.4, 1_8_2 26.1. Gated: 13824 x 5120
+//   2_4_4 31.3, 4_4_2 31.9, 2_4_2 37.2; 4096 x 4096 2_4_2/2 11.4, 2_4_4/2 15.1.
+LinearPlan int4_plan(int64_t M, int64_t N, int64_t K, bool gated) {
+    if (M > 32) return few_plan(kFew64_2_4_2, 4, 2, 4, 2, N, K, gated, 8);
+    if (M > 16) {
+        if (!gated) return few_plan(kFew32_1_4_4, 2, 1, 4, 4, N, K, gated, 8);
+        if (N > 64 * 160) return few_plan(kFew32_2_4_4, 2, 2, 4, 4, N, K, gated, 8);
+        return few_plan(kFew32_2_4_2, 2, 2, 4, 2, N, K, gated, 8);
+    }
+    if (gated) {
+        if (N > 8192) return few_plan(kFew16_2_4_2, 1, 2, 4, 2, N, K, gated, 16);
+        if (N > 2048 || K <= 8192) return few_plan(kFew16_2_8_1, 1, 2, 8, 1, N, K, gated, 32);
+        return few_plan(kFew16_2_16_1, 1, 2, 16, 1, N, K, gated, 64);
+    }
+    if (N > 8192) return few_plan(kFew16_2_8_1, 1, 2, 8, 1, N, K, gated, 32);
+    if (N > 4096) return few_plan(kFew16_1_8_2, 1, 1, 8, 2, N, K, gated, 32);
+    return few_plan(kFew16_1_16_1, 1, 1, 16, 1, N, K, gated, 64);
+}
+
+// 16-bit weights, measured alike: 1 row of 4096 -> 14336 2_8_1 42.5, 2_4_1 48.7; 24 rows of 5120 -> 13824 4_4_2 57.7, 2_4_2 60.4,
+// 2_8_1 74.7.
+LinearPlan gated_few_plan(int64_t M, int64_t F, int64_t K) {
+    if (M > 32) return few_plan(kFew64_2_4_2, 4, 2, 4, 2, F, K, true, 8);
+    if (M > 16 && F > 64 * 160) return few_plan(kFew32_4_4_2, 2, 4, 4, 2, F, K, true, 8);
+    if (M > 16) return few_plan(kFew32_2_4_2, 2, 2, 4, 2, F, K, true, 8);
+    return few_plan(kFew16_2_8_1, 1, 2, 8, 1, F, K, true, 16);
+}
+
 LinearPlan gated_plan(int64_t M, int64_t F, int64_t K) {
-    return M <= kFewRows ? few_rows_plan(M, F, K, true) : tile_plan(M, 2 * ceil_div(F, 64) * 64, K);
+    return M <= kFewRows ? gated_few_plan(M, F, K) : tile_plan(M, 2 * ceil_div(F, 64) * 64, K);
 }
 
 int64_t workspace_of(const LinearPlan& plan) {
@@ -86,7 +117,7 @@ int64_t workspace_of(const LinearPlan& plan) {
 
 // Whether a plan's launch has fewer than 2^32 threads.
 bool launchable(const LinearPlan& plan) {
-    return plan.tiles * plan.splits <= kMaxThreads / (plan.kernel >= kFewRows16 ? 512 : 256);
+    return plan.tiles * plan.splits <= kMaxThreads / plan.threads;
 }
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
@@ -298,7 +329,7 @@ bool int4_ok(const uint8_t* codes, int64_t ld_codes, const void* scale, int64_t 
 extern "C" int64_t feather_int4_linear_rows(void) { return kFewRows; }
 
 extern "C" int64_t feather_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated) {
-    return M <= kFewRows && sizes_ok(M, gated ? 2 * N : N, K) ? workspace_of(few_rows_plan(M, N, K, gated)) : -1;
+    return M <= kFewRows && sizes_ok(M, gated ? 2 * N : N, K) ? workspace_of(int4_plan(M, N, K, gated)) : -1;
 }
 
 extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64_t ld_codes, const void* scale,
@@ -310,7 +341,7 @@ extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* c
         !operand_ok(x, ldx, K) || !output_ok(y, ldy, N, type) || (bias && !aligned_to_type(bias, type)) ||
         !int4_ok(codes, ld_codes, scale, ld_scale, zero, ld_zero, group, type, rows, K))
         return false;
-    const LinearPlan plan = few_rows_plan(M, N, K, gated);
+    const LinearPlan plan = int4_plan(M, N, K, gated);
     const int64_t need = workspace_of(plan);
     if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
     Int4Params p{};

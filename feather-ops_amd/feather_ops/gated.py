@@ -1,5 +1,5 @@
 """The gated feed-forward block's first half in one kernel, `act(x Wg^T + bg) * (x Wu^T + bu)`, in 16 bits, with gradients; not in
-the reference. Kernels: `csrc/linear_tile.h` (and the products of the backward), `csrc/linear_stream.h` (few rows),
+the reference. Kernels: `csrc/linear_tile.h` (and the products of the backward), `csrc/linear_few.h` (few rows),
 `csrc/linear_ops.hip`; autograd node: `csrc/linear_autograd.cpp`. C ABI: `include/feather_linear_ops.h`.
 
 The weight holds both projections, `[2 F, K]`: the gates' rows first, as `silu_mul` takes their outputs.

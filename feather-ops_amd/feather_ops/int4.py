@@ -1,5 +1,5 @@
 """Products with 4-bit weights that have one scale for each group of columns, their quantization, and the layers on them; not in
-the reference, whose weights have 8 bits. Kernels: `csrc/linear_stream.h` (few rows), `csrc/linear_tile.h`, `csrc/int4.hip`; autograd
+the reference, whose weights have 8 bits. Kernels: `csrc/linear_few.h` (few rows), `csrc/linear_tile.h`, `csrc/int4.hip`; autograd
 node: `csrc/linear_autograd.cpp`. C ABI: `include/feather_linear_ops.h`.
 
 A quantized weight is `(codes, scale, zero)`: value (n, k) is `(q - zero) * scale` with the code q, 0 .. 15, and the scale and zero

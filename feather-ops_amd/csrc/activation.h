@@ -4,7 +4,9 @@
 //   gelu       g P(g)                              P the normal distribution's function, (1 + erf(g / sqrt 2)) / 2
 //   gelu_tanh  g s(z),  z = sqrt(8 / pi) (g + 0.044715 g^3), since (1 + tanh(z / 2)) / 2 = s(z)
 //
-// In fp32 with the exponential and reciprocal instructions, within a few ulp: results are rounded to 16 bits.
+// In fp32 with the exponential and reciprocal instructions, within a few ulp (gelu 2^-19): results are rounded to 16 bits. At the
+// end of a 256 x 256 tile one wave a SIMD does this for 128 values a lane, with nothing beside it: by the library's erfc, some 60
+// instructions, 5000 x 2576 gelu took 40 us more than silu at 4097 rows.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -30,21 +32,39 @@ __device__ __forceinline__ Logistic logistic(float z) {
     return z < 0.0f ? Logistic{tq, q} : Logistic{q, tq};
 }
 
-// a * s for a factor s that may be 0 where a is infinite or the type's lowest value: 0 and not NaN.
-__device__ __forceinline__ float faded(float a, float s) { return s == 0.0f ? 0.0f * s : a * s; }
+// a * s for a factor s that may be 0 where a is infinite: 0 and not NaN.
+__device__ __forceinline__ float faded(float a, float s) { return (s == 0.0f ? 0.0f : a) * s; }
 
 constexpr float kTanhSlope = 1.5957691216057308f;   // sqrt(8 / pi)
 constexpr float kTanhCube = 0.044715f;
-constexpr float kRootHalf = 0.70710678118654752f;
 constexpr float kNormalDensity = 0.39894228040143268f;   // 1 / sqrt(2 pi)
 
-// P(g), without the cancellation of 1 + erf at negative g.
-__device__ __forceinline__ float normal_function(float g) { return 0.5f * erfcf(-g * kRootHalf); }
+struct Normal {
+    float p, density;   // P(g) and P'(g)
+};
+
+// With t = |g|, P(-t) exp(t^2 / 2) is smooth and falls from 1 / 2 like 1 / t: a polynomial in u = 1 / (1 + 0.36 t) without a
+// constant, fitted to the least relative error over t up to 14.5 (1e-6), where the exponential ends.
+__device__ __forceinline__ Normal normal(float g) {
+    const float t = fabsf(g);
+    const float root = __expf(-0.25f * t * t);
+    const float e = root * root;
+    const float u = __builtin_amdgcn_rcpf(__builtin_fmaf(0.36f, t, 1.0f));
+    float r = 0.04678545892238617f;
+    r = __builtin_fmaf(r, u, -0.1788369119167328f);
+    r = __builtin_fmaf(r, u, 0.17969179153442383f);
+    r = __builtin_fmaf(r, u, 0.02741684578359127f);
+    r = __builtin_fmaf(r, u, 0.13940362632274628f);
+    r = __builtin_fmaf(r, u, 0.1418297439813614f);
+    r = __builtin_fmaf(r, u, 0.14370901882648468f);
+    const float tail = r * u * e;
+    return {g < 0.0f ? tail : 1.0f - tail, kNormalDensity * e};
+}
 
 template <int kAct>
 __device__ __forceinline__ float activate(float g) {
     if constexpr (kAct == kSilu) return faded(g, logistic(g).s);
-    if constexpr (kAct == kGelu) return faded(g, normal_function(g));
+    if constexpr (kAct == kGelu) return faded(g, normal(g).p);
     const float z = kTanhSlope * (g + kTanhCube * g * g * g);
     return faded(g, logistic(z).s);
 }
@@ -57,8 +77,8 @@ __device__ __forceinline__ Slope activate_with_slope(float g) {
         return {value, l.s + faded(value, l.c)};
     }
     if constexpr (kAct == kGelu) {
-        const float p = normal_function(g);
-        return {faded(g, p), p + faded(g, kNormalDensity * __expf(-0.5f * g * g))};
+        const Normal n = normal(g);
+        return {faded(g, n.p), n.p + faded(g, n.density)};
     }
     const float z = kTanhSlope * (g + kTanhCube * g * g * g);
     const Logistic l = logistic(z);

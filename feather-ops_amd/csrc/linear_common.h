@@ -25,6 +25,8 @@ struct LinearParams {
     const uint16_t* b;      // [N, K] ([2 N, K] gated: the gates' rows, then the ups'), or [K, N] where transposed
     int64_t lda, ldb;       // elements
     int32_t M, N, K;
+    int32_t m_first, n_first;   // tiles: the outputs where this launch starts, and how many tiles there are
+    int32_t tiles_m, tiles_n;
     int32_t splits;
     const void* bias;       // N values ([2 N] gated) of the operands' type, or null
     void* c;                // [M, N]

@@ -10,6 +10,7 @@
 #include <tuple>
 
 #include "extension_common.h"
+#include "feather_internal.h"
 #include "feather_linear_ops.h"
 
 namespace {
@@ -100,6 +101,26 @@ Workspace check_workspace(std::optional<Tensor>& workspace, int64_t need, const 
 
 float* floats(Tensor& t) { return static_cast<float*>(t.mutable_data_ptr()); }
 
+// Rows of x as a large product reads them: where neither operand's rows start on half lines of memory, each stage of each row
+// costs a line more, and x is copied to whole lines first (4096 x 2576 -> 8192 in 256 x 256 tiles 171 us, with either operand
+// copied 138; the copy 9).
+constexpr int64_t kHalfLine = 32;   // values
+
+struct Rows {
+    Tensor own;
+    const void* data;
+    int64_t ld;
+};
+
+Rows on_lines(const Tensor& x, int64_t ldx, int64_t other_ld, int64_t n, hipStream_t stream) {
+    const int64_t m = x.size(0), k = x.size(1);
+    if (ldx % kHalfLine == 0 || other_ld % kHalfLine == 0 || m < 512 || n < 2048 || k < 256) return {x, x.const_data_ptr(), ldx};
+    const int64_t ld = up_to(k, 2 * kHalfLine);
+    Tensor own = new_rows(x, m, ld, torch_dtype(half_type(x, "x")));
+    check_launch(feather_copy_rows(x.const_data_ptr(), ldx, own.mutable_data_ptr(), ld, m, k, stream), "copy of rows");
+    return {own, own.const_data_ptr(), ld};
+}
+
 // feather_ops::gated_forward (feather_gated_linear): (y, what the backward needs), the latter empty unless `keep`.
 std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
                                          const int64_t activation, const bool keep, std::optional<Tensor> workspace) {
@@ -120,9 +141,11 @@ std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& weight, 
     Tensor y = new_rows(x, M, F, torch_dtype(type));
     Tensor kept = keep ? new_rows(x, M, ld_kept, aoti_torch_dtype_float32()) : new_rows(x, 0, 0, aoti_torch_dtype_float32());
     torch::stable::accelerator::DeviceGuard guard(x.get_device_index());
-    check_launch(feather_gated_linear(x.const_data_ptr(), ldx, weight.const_data_ptr(), ldw, bias_data, type,
+    const hipStream_t stream = current_stream(x.get_device_index());
+    const Rows rows = on_lines(x, ldx, ldw, 2 * F, stream);
+    check_launch(feather_gated_linear(rows.data, rows.ld, weight.const_data_ptr(), ldw, bias_data, type,
                                       static_cast<int>(activation), y.mutable_data_ptr(), F, keep ? floats(kept) : nullptr, ld_kept,
-                                      M, F, K, ws.data, ws.bytes, current_stream(x.get_device_index())),
+                                      M, F, K, ws.data, ws.bytes, stream),
                  "gated_linear");
     return {y, kept};
 }
@@ -150,7 +173,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& grad_y, const Te
                     "kept must be what the forward kept");
     STD_TORCH_CHECK(activation >= 0 && activation <= 2, "unknown activation");
     const int32_t dtype = torch_dtype(type);
-    const int64_t ld_grad = up_to(2 * F, 8);
+    const int64_t ld_grad = up_to(2 * F, 2 * kHalfLine);
     Tensor grad = new_rows(x, M, ld_grad, dtype);
     const int64_t parts = feather_gated_backward_parts(M, F);
     Tensor sums = new_rows(x, need_bias ? parts : 0, need_bias ? 2 * F : 0, aoti_torch_dtype_float32());
@@ -234,11 +257,12 @@ Int4 check_int4(const Tensor& codes, const Tensor& scale, const std::optional<Te
     return w;
 }
 
-Tensor new_dequantized(const Int4& w, const Tensor& like, int64_t K, int type, hipStream_t stream) {
-    const int64_t K8 = up_to(K, 8);
-    Tensor out = new_rows(like, w.rows, K8, torch_dtype(type));
+// The weight [N, K] in 16 bits, rows a multiple of `pitch` (of 8) values apart.
+Tensor new_dequantized(const Int4& w, const Tensor& like, int64_t K, int64_t pitch, int type, hipStream_t stream) {
+    const int64_t ld = up_to(K, pitch);
+    Tensor out = new_rows(like, w.rows, ld, torch_dtype(type));
     check_launch(feather_int4_dequantize(w.codes, w.ld_codes, w.scale, w.ld_scale, w.zero, w.ld_zero, w.group, type,
-                                         out.mutable_data_ptr(), K8, w.rows, K, stream),
+                                         out.mutable_data_ptr(), ld, w.rows, K, stream),
                  "dequantize_int4");
     return out;
 }
@@ -270,16 +294,17 @@ Tensor int4_forward(const Tensor& x, const Tensor& codes, const Tensor& scale, c
         return y;
     }
     const int64_t K8 = up_to(K, 8);
-    const Tensor full = new_dequantized(w, x, K, type, stream);
+    const int64_t ldw = up_to(K, 2 * kHalfLine);
+    const Tensor full = new_dequantized(w, x, K, 2 * kHalfLine, type, stream);
     if (gated) {
         const Workspace ws = check_workspace(workspace, feather_gated_linear_workspace_bytes(M, N, K8), x);
-        check_launch(feather_gated_linear(x.const_data_ptr(), ldx, full.const_data_ptr(), K8, bias_data, type,
+        check_launch(feather_gated_linear(x.const_data_ptr(), ldx, full.const_data_ptr(), ldw, bias_data, type,
                                           static_cast<int>(activation), y.mutable_data_ptr(), N, nullptr, 0, M, N, K8, ws.data,
                                           ws.bytes, stream),
                      "int4_linear");
     } else {
         const Workspace ws = check_workspace(workspace, feather_product_workspace_bytes(M, N, K8), x);
-        check_launch(feather_product(x.const_data_ptr(), ldx, false, full.const_data_ptr(), K8, false, bias_data, type,
+        check_launch(feather_product(x.const_data_ptr(), ldx, false, full.const_data_ptr(), ldw, false, bias_data, type,
                                      y.mutable_data_ptr(), N, M, N, K8, ws.data, ws.bytes, stream),
                      "int4_linear");
     }
@@ -300,8 +325,8 @@ Tensor int4_backward(const Tensor& grad_y, const Tensor& codes, const Tensor& sc
     Tensor grad_x = new_rows(grad_y, M, K, torch_dtype(type));
     torch::stable::accelerator::DeviceGuard guard(grad_y.get_device_index());
     const hipStream_t stream = current_stream(grad_y.get_device_index());
-    const Tensor full = new_dequantized(w, grad_y, K, type, stream);
-    check_launch(feather_product(grad_y.const_data_ptr(), ld, false, full.const_data_ptr(), up_to(K, 8), true, nullptr, type,
+    const Tensor full = new_dequantized(w, grad_y, K, 2 * kHalfLine, type, stream);
+    check_launch(feather_product(grad_y.const_data_ptr(), ld, false, full.const_data_ptr(), up_to(K, 2 * kHalfLine), true, nullptr, type,
                                  grad_x.mutable_data_ptr(), K, M, K, w.rows, ws.data, ws.bytes, stream),
                  "int4_linear's backward");
     return grad_x;
@@ -339,7 +364,7 @@ Tensor int4_dequantize(const Tensor& codes, const Tensor& scale, const std::opti
     const Int4 w = check_int4(codes, scale, zero, K, codes);
     STD_TORCH_CHECK(w.rows > 0 && K > 0, "the weight must not be empty");
     torch::stable::accelerator::DeviceGuard guard(codes.get_device_index());
-    return new_dequantized(w, codes, K, type, current_stream(codes.get_device_index()));
+    return new_dequantized(w, codes, K, 8, type, current_stream(codes.get_device_index()));
 }
 
 }  // namespace

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <iterator>
 
 #include "feather_internal.h"
 #include "feather_linear_ops.h"
@@ -24,40 +25,47 @@ bool splits_fit(const LinearPlan& plan) {
     return plan.tiles * plan.slots <= kMaxCounters && plan.tiles * plan.splits * plan.tile_bytes <= kMaxPartBytes;
 }
 
-// A tile, and microseconds of a workgroup's start and end and of a stage of 64, with per_cu workgroups on a CU and with one.
+// A tile, and microseconds: of a workgroup's start and end, and of a stage of 64 where workgroups fill the chip (per_cu on each CU)
+// and where there is one alone, with what lies between in proportion. The figures minimise what the pick of tile and K splits
+// loses against the best pair in 2900 timings of 178 shapes (100 to 4096 rows, 1024 to 28672 columns, K 512 to 14336): 1.4% in
+// geometric mean, 23% at most.
 struct TileCost {
     LinearKernel kernel;
     int bm, bn, per_cu;
-    float fixed, full, alone;
+    float fixed, full, lone;
 };
 constexpr TileCost kTiles[] = {
-    {kTile256, 256, 256, 1, 4.0f, 1.42f, 1.42f},
-    {kTile256x128, 256, 128, 1, 3.0f, 0.85f, 0.85f},
-    {kTile128, 128, 128, 2, 2.0f, 0.98f, 0.60f},
+    {kTile256, 256, 256, 1, 9.8f, 1.30f, 1.28f},
+    {kTile256x128, 256, 128, 1, 5.9f, 0.77f, 0.47f},
+    {kTile128, 128, 128, 2, 3.8f, 0.82f, 0.48f},
 };
-constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8};
+constexpr float kLaunchCost = 2.0f;   // us from the end of one launch to the next one's work
 
 // N: columns of b (gated: 2 F).
 LinearPlan tile_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t all = ceil_div(K, 64);
-    const float memory = static_cast<float>(N + M) * static_cast<float>(K) / 2.4e6f;   // us at 4.8 TB/s
+    const float memory = static_cast<float>(N + M) * static_cast<float>(K) / 2.2e6f;   // us at 4.4 TB/s
     LinearPlan best{};
     for (const TileCost& t : kTiles) {
         const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
+        const int64_t cap = kCUs * t.per_cu;
         for (const int splits : kSplits) {
             LinearPlan plan{t.kernel, splits, tiles, 256, 4, int64_t{4} * t.bm * t.bn, 0.0f};
             if (splits > 1 && (splits > all || tiles * splits > 4 * kCUs || !splits_fit(plan))) break;
             const auto stages = static_cast<float>(ceil_div(all, splits));
             const int64_t groups = tiles * splits;
-            const int64_t rounds = groups / (kCUs * t.per_cu);
-            const int64_t rest = groups - rounds * kCUs * t.per_cu;
+            const int64_t rounds = groups / cap;
+            const int64_t rest = groups - rounds * cap;
             float cost = static_cast<float>(rounds) * (stages * t.full + t.fixed);
-            if (rest > 0) cost += stages * (rest > kCUs ? t.full : t.alone) + t.fixed;
+            if (rest > 0) cost += stages * (t.lone + (t.full - t.lone) * static_cast<float>(rest) / static_cast<float>(cap)) + t.fixed;
             cost = std::max(cost, memory);
-            // the last of a tile's workgroups reads all of its sums back
-            if (splits > 1) cost += 2.0f + 1.5f / 65536.0f * static_cast<float>(splits * plan.tile_bytes);
-            plan.cost = cost;
-            if (best.cost == 0.0f || cost < best.cost) best = plan;
+            // sums are written, and the last of a tile's workgroups reads all of its back
+            if (splits > 1)
+                cost += 1.8f + static_cast<float>(t.bm * t.bn) * static_cast<float>(splits) *
+                                    (3.9f / 65536.0f + static_cast<float>(tiles) * (4.4f / 16777216.0f));
+            plan.cost = cost + kLaunchCost;
+            if (best.cost == 0.0f || plan.cost < best.cost) best = plan;
         }
     }
     return best;
@@ -107,17 +115,125 @@ LinearPlan gated_few_plan(int64_t M, int64_t F, int64_t K) {
     return few_plan(kFew16_2_8_1, 1, 2, 8, 1, F, K, true, 16);
 }
 
-LinearPlan gated_plan(int64_t M, int64_t F, int64_t K) {
-    return M <= kFewRows ? gated_few_plan(M, F, K) : tile_plan(M, 2 * ceil_div(F, 64) * 64, K);
+// A part of a product: rows m0 .. + M, b's columns n0 .. + N (gated: gates and ups together).
+struct Part {
+    int64_t m0, n0, M, N;
+    LinearPlan plan;
+};
+
+struct Parts {
+    Part part[4];
+    int count;
+    float cost;
+};
+
+// One launch for a part. Few rows of a gated block, all of its columns, go to a kernel of their own.
+LinearPlan whole_plan(int64_t M, int64_t N, int64_t K, bool all_gated) {
+    if (!all_gated || M > kFewRows) return tile_plan(M, N, K);
+    LinearPlan plan = gated_few_plan(M, N / 2, K);
+    plan.cost = kLaunchCost + 2.0f + static_cast<float>(N) * static_cast<float>(K) / (M > 32 ? 1.6e6f : 2.4e6f);
+    return plan;
 }
+
+// Large products go in up to four launches where whole rounds of tiles end at a column or row and the rest does better on
+// other tiles. Cuts fall on multiples of 256 and are tried where a number of whole rounds of each tile ends, along either axis; a
+// part may be cut once more.
+Parts cut(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bool all_gated, int depth) {
+    const LinearPlan whole = whole_plan(M, N, K, all_gated);
+    Parts best{{{m0, n0, M, N, whole}}, 1, whole.cost};
+    if (depth == 0 || whole.cost < 20.0f) return best;
+    const auto attempt = [&](bool rows, int64_t at) {
+        const int64_t total = rows ? M : N;
+        if (at <= 0 || at >= total) return;
+        const LinearPlan first = rows ? whole_plan(at, N, K, all_gated) : whole_plan(M, at, K, false);
+        if (first.cost >= best.cost) return;
+        const Parts heads = depth > 1 ? (rows ? cut(m0, n0, at, N, K, all_gated, depth - 1) : cut(m0, n0, M, at, K, false, depth - 1))
+                                      : Parts{{{m0, n0, rows ? at : M, rows ? N : at, first}}, 1, first.cost};
+        const Parts rest = rows ? cut(m0 + at, n0, M - at, N, K, all_gated, depth - 1)
+                                : cut(m0, n0 + at, M, N - at, K, false, depth - 1);
+        const float cost = heads.cost + rest.cost;
+        if (cost >= best.cost || heads.count + rest.count > 4) return;
+        best.count = 0;
+        for (int i = 0; i < heads.count; ++i) best.part[best.count++] = heads.part[i];
+        for (int i = 0; i < rest.count; ++i) best.part[best.count++] = rest.part[i];
+        best.cost = cost;
+    };
+    for (const TileCost& t : kTiles) {
+        const int64_t round = kCUs * t.per_cu;
+        const int64_t tiles_m = ceil_div(M, t.bm), tiles_n = ceil_div(N, t.bn);
+        const int64_t rounds = tiles_m * tiles_n / round;
+        if (rounds == 0) continue;
+        attempt(false, rounds * round / tiles_m * t.bn / 256 * 256);
+        attempt(true, rounds * round / tiles_n * t.bm / 256 * 256);
+    }
+    attempt(true, M / 256 * 256);
+    return best;
+}
+
+// The launches of a product: the same ones for every call of a shape. A search of large shapes takes up to 0.1 ms of the
+// host, so each thread keeps the last ones by shape.
+const Parts& parts_of(int64_t M, int64_t N, int64_t K, bool gated) {
+    struct Entry {
+        int64_t M, N, K;
+        bool gated;
+        Parts parts;
+    };
+    constexpr uint64_t kEntries = 64;
+    thread_local Entry table[kEntries];
+    const auto hash = static_cast<uint64_t>(M) * 0x9e3779b97f4a7c15u + static_cast<uint64_t>(N) * 0xc2b2ae3d27d4eb4fu +
+                      static_cast<uint64_t>(K) * 0x165667b19e3779f9u + (gated ? 1u << 31 : 0u);
+    Entry& e = table[(hash >> 32) % kEntries];
+    if (e.M != M || e.N != N || e.K != K || e.gated != gated || e.parts.count == 0)
+        e = Entry{M, N, K, gated, cut(0, 0, M, N, K, gated, 2)};
+    return e.parts;
+}
+
+// Gated: columns of whole pairs of fragments, F rounded up to them.
+const Parts& gated_parts(int64_t M, int64_t F, int64_t K) { return parts_of(M, 2 * ceil_div(F, 16) * 16, K, true); }
 
 int64_t workspace_of(const LinearPlan& plan) {
     return plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
 }
 
-// Whether a plan's launch has fewer than 2^32 threads.
+int64_t workspace_of(const Parts& parts) {
+    int64_t most = 0;
+    for (int i = 0; i < parts.count; ++i) most = std::max(most, workspace_of(parts.part[i].plan));
+    return most;
+}
+
+// Whether each launch has fewer than 2^32 threads.
 bool launchable(const LinearPlan& plan) {
     return plan.tiles * plan.splits <= kMaxThreads / plan.threads;
+}
+
+bool launchable(const Parts& parts) {
+    for (int i = 0; i < parts.count; ++i)
+        if (!launchable(parts.part[i].plan)) return false;
+    return true;
+}
+
+// The launches of a product, one after the other.
+void launch(const LinearParams& whole, const Parts& parts, int type, Operands operands, hipStream_t stream) {
+    const bool gated = operands == Operands::kGated || operands == Operands::kGatedKeep;
+    for (int i = 0; i < parts.count; ++i) {
+        const Part& part = parts.part[i];
+        LinearParams p = whole;
+        p.splits = part.plan.splits;
+        if (part.plan.kernel > kTile128) {   // all columns of the rows
+            p.a += part.m0 * p.lda;
+            p.c = static_cast<uint16_t*>(p.c) + part.m0 * p.ldc;
+            if (p.h) p.h += part.m0 * p.ldh;
+            p.M = static_cast<int32_t>(part.M);
+        } else {
+            const auto tile = *std::find_if(std::begin(kTiles), std::end(kTiles),
+                                            [&](const TileCost& t) { return t.kernel == part.plan.kernel; });
+            p.m_first = static_cast<int32_t>(part.m0);
+            p.n_first = static_cast<int32_t>(gated ? part.n0 / 2 : part.n0);
+            p.tiles_m = static_cast<int32_t>(ceil_div(part.M, tile.bm));
+            p.tiles_n = static_cast<int32_t>(ceil_div(part.N, tile.bn));
+        }
+        (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(p, part.plan, operands, stream);
+    }
 }
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
@@ -150,7 +266,7 @@ void use_workspace(LinearParams& p, void* workspace) {
 //
 // A lane takes 8 columns of both halves of kRows rows, one after the other, and keeps their sums. Memory bounds it.
 constexpr int kThreads = 256;
-constexpr int kRows = 32;
+constexpr int kRows = 16;
 
 struct BackwardParams {
     const uint16_t* grad_y;
@@ -166,35 +282,42 @@ __device__ __forceinline__ void backward_rows(const BackwardParams& p, int at, i
     const int half = (p.cols + 7) & ~7;
     float sum_gate[kPiece] = {}, sum_up[kPiece] = {};
     const bool last = at + kPiece >= p.cols;
-#pragma unroll 2
-    for (int row = row0; row < row1; ++row) {
-        const float* const kept = p.kept + row * p.ld_kept + at;
-        float dy[kPiece], gate[kPiece], up[kPiece];
-        load_piece<kType, false>(p.grad_y + row * p.ld_grad_y, at, valid, dy);
+    constexpr int kAhead = 4;   // rows whose loads are in flight together
+    for (int first = row0; first < row1; first += kAhead) {
+        RawPiece<kType> raw[kAhead];
+        f32x4 gates[kAhead][2], ups[kAhead][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const f32x4 g = *reinterpret_cast<const f32x4*>(kept + 4 * h);
-            const f32x4 u = *reinterpret_cast<const f32x4*>(kept + half + 4 * h);
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t row = first + i < row1 ? first + i : row1 - 1;
+            const float* const kept = p.kept + row * p.ld_kept + at;
+            raw[i] = load_raw<kType, false>(p.grad_y + row * p.ld_grad_y, at, valid);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                gate[4 * h + e] = g[e];
-                up[4 * h + e] = u[e];
+            for (int h = 0; h < 2; ++h) {
+                gates[i][h] = *reinterpret_cast<const f32x4*>(kept + 4 * h);
+                ups[i][h] = *reinterpret_cast<const f32x4*>(kept + half + 4 * h);
             }
         }
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) {
-            const Slope s = activate_with_slope<kAct>(gate[e]);
-            // the slope first: of a gate masked with the type's lowest value it is 0, and dy up may be infinite
-            gate[e] = dy[e] * s.slope * up[e];
-            up[e] = dy[e] * s.value;
-            sum_gate[e] += gate[e];
-            sum_up[e] += up[e];
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t row = first + i;
+            if (row >= row1) break;
+            float dy[kPiece], gate[kPiece], up[kPiece];
+            unpack(raw[i], dy);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                const Slope s = activate_with_slope<kAct>(gates[i][e / 4][e % 4]);
+                // the slope first: of a gate masked with the type's lowest value it is 0, and dy up may be infinite
+                gate[e] = dy[e] * s.slope * ups[i][e / 4][e % 4];
+                up[e] = dy[e] * s.value;
+                sum_gate[e] += gate[e];
+                sum_up[e] += up[e];
+            }
+            uint16_t* const out = p.grad + row * p.ld_grad;
+            store_piece<kType, false>(out, at, valid, gate);
+            store_piece<kType, false>(out + p.cols, at, valid, up);
+            if (last)
+                for (int c = 2 * p.cols; c < ((2 * p.cols + 7) & ~7); ++c) out[c] = 0;
         }
-        uint16_t* const out = p.grad + row * p.ld_grad;
-        store_piece<kType, false>(out, at, valid, gate);
-        store_piece<kType, false>(out + p.cols, at, valid, up);
-        if (last)
-            for (int c = 2 * p.cols; c < ((2 * p.cols + 7) & ~7); ++c) out[c] = 0;
     }
     if (p.sums) {
         float* const out = p.sums + static_cast<int64_t>(row0 / kRows) * 2 * p.cols;
@@ -215,13 +338,45 @@ __global__ __launch_bounds__(kThreads) void gated_backward_kernel(const Backward
     else backward_rows<kType, kGeluTanh>(p, at, valid, row0, row1);
 }
 
+// ---- rows put on whole lines ----
+
+struct CopyParams {
+    const uint16_t* from;
+    uint16_t* to;
+    int64_t ld_from, ld_to, rows;
+    int32_t pieces;   // of a row
+};
+
+__global__ __launch_bounds__(kThreads) void copy_rows_kernel(const CopyParams p) {
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    const int64_t row = index / p.pieces;
+    if (row >= p.rows) return;
+    const int at = static_cast<int>(index - row * p.pieces) * kPiece;
+    *reinterpret_cast<u32x4*>(p.to + row * p.ld_to + at) = *reinterpret_cast<const u32x4*>(p.from + row * p.ld_from + at);
+}
+
 }  // namespace
 }  // namespace feather
 
 using namespace feather;
 
+extern "C" bool feather_copy_rows(const void* from, int64_t ld_from, void* to, int64_t ld_to, int64_t rows, int64_t cols,
+                                  hipStream_t stream) {
+    if (!matrix_ok(from, ld_from, rows, cols) || !matrix_ok(to, ld_to, rows, cols) || cols % 8 != 0 || ld_from % 8 != 0 ||
+        ld_to % 8 != 0 || !on_16(from) || !on_16(to))
+        return false;
+    const auto pieces = static_cast<int32_t>(cols / 8);
+    const int64_t most = (kMaxThreads - kThreads) / pieces;   // rows of a launch
+    for (int64_t row = 0; row < rows; row += most) {
+        const CopyParams p{static_cast<const uint16_t*>(from) + row * ld_from, static_cast<uint16_t*>(to) + row * ld_to, ld_from, ld_to,
+                           std::min(rows - row, most), pieces};
+        copy_rows_kernel<<<static_cast<uint32_t>(ceil_div(p.rows * pieces, kThreads)), kThreads, 0, stream>>>(p);
+    }
+    return true;
+}
+
 extern "C" int64_t feather_gated_linear_workspace_bytes(int64_t M, int64_t F, int64_t K) {
-    return sizes_ok(M, 2 * F, K) ? workspace_of(gated_plan(M, F, K)) : -1;
+    return sizes_ok(M, 2 * F, K) ? workspace_of(gated_parts(M, F, K)) : -1;
 }
 
 extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* weight, int64_t ld_weight, const void* bias,
@@ -233,9 +388,9 @@ extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* wei
         (bias && !aligned_to_type(bias, type)))
         return false;
     if (kept && (!on_16(kept) || ld_kept % 4 != 0 || ld_kept < 2 * F8 || ld_kept >= int64_t{1} << 22)) return false;
-    const LinearPlan plan = gated_plan(M, F, K);
-    const int64_t need = workspace_of(plan);
-    if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
+    const Parts& parts = gated_parts(M, F, K);
+    const int64_t need = workspace_of(parts);
+    if (!launchable(parts) || !workspace_ok(workspace, workspace_bytes, need)) return false;
     LinearParams p{};
     p.a = static_cast<const uint16_t*>(x);
     p.b = static_cast<const uint16_t*>(weight);
@@ -244,7 +399,6 @@ extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* wei
     p.M = static_cast<int32_t>(M);
     p.N = static_cast<int32_t>(F);
     p.K = static_cast<int32_t>(K);
-    p.splits = plan.splits;
     p.bias = bias;
     p.c = y;
     p.ldc = ldy;
@@ -252,7 +406,7 @@ extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* wei
     p.ldh = ld_kept;
     p.act = activation;
     use_workspace(p, need > 0 ? workspace : nullptr);
-    (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(p, plan, kept ? Operands::kGatedKeep : Operands::kGated, stream);
+    launch(p, parts, type, kept ? Operands::kGatedKeep : Operands::kGated, stream);
     return true;
 }
 
@@ -282,7 +436,7 @@ extern "C" bool feather_gated_backward(const void* grad_y, int64_t ld_grad_y, co
 }
 
 extern "C" int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return sizes_ok(M, N, K) ? workspace_of(tile_plan(M, N, K)) : -1;
+    return sizes_ok(M, N, K) ? workspace_of(parts_of(M, N, K, false)) : -1;
 }
 
 extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const void* b, int64_t ldb, bool b_across,
@@ -291,9 +445,9 @@ extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const
     if (!sizes_ok(M, N, K) || !half_type(type) || (a_across && !b_across) || !operand_ok(a, lda, a_across ? M : K) ||
         !operand_ok(b, ldb, b_across ? N : K) || !output_ok(c, ldc, N, type) || (bias && !aligned_to_type(bias, type)))
         return false;
-    const LinearPlan plan = tile_plan(M, N, K);
-    const int64_t need = workspace_of(plan);
-    if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
+    const Parts& parts = parts_of(M, N, K, false);
+    const int64_t need = workspace_of(parts);
+    if (!launchable(parts) || !workspace_ok(workspace, workspace_bytes, need)) return false;
     LinearParams p{};
     p.a = static_cast<const uint16_t*>(a);
     p.b = static_cast<const uint16_t*>(b);
@@ -302,17 +456,32 @@ extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const
     p.M = static_cast<int32_t>(M);
     p.N = static_cast<int32_t>(N);
     p.K = static_cast<int32_t>(K);
-    p.splits = plan.splits;
     p.bias = bias;
     p.c = c;
     p.ldc = ldc;
     use_workspace(p, need > 0 ? workspace : nullptr);
-    const Operands operands = a_across ? Operands::kBothAcross : b_across ? Operands::kBAcross : Operands::kAlong;
-    (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(p, plan, operands, stream);
+    launch(p, parts, type, a_across ? Operands::kBothAcross : b_across ? Operands::kBAcross : Operands::kAlong, stream);
     return true;
 }
 
+extern "C" int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, int64_t out[16]) {
+    if (!sizes_ok(M, gated ? 2 * N : N, K)) return 0;
+    const Parts& parts = gated ? gated_parts(M, N, K) : parts_of(M, N, K, false);
+    for (int i = 0; i < parts.count; ++i) {
+        const Part& part = parts.part[i];
+        const int64_t launch[4] = {part.plan.kernel, part.plan.splits, part.M, part.N};
+        std::copy(launch, launch + 4, out + 4 * i);
+    }
+    return parts.count;
+}
+
 // ---- 4-bit weights ----
+
+extern "C" void feather_int4_launch(int64_t M, int64_t N, int64_t K, bool gated, int64_t out[2]) {
+    const LinearPlan plan = int4_plan(M, N, K, gated);
+    out[0] = plan.kernel;
+    out[1] = plan.splits;
+}
 
 namespace {
 

@@ -140,21 +140,21 @@ void linear_tile_kernel(const LinearParams p) {
     const int wave_m = wave / 2;
     const int wave_n = wave % 2;
     constexpr int kCols = kGated ? T::BN / 2 : T::BN;   // outputs of a tile's row
-    const int tiles_m = (p.M + T::BM - 1) / T::BM;
-    const int tiles_n = (p.N + kCols - 1) / kCols;
-    const int tiles = tiles_m * tiles_n;
+    const int tiles = p.tiles_m * p.tiles_n;
     const int split = p.splits > 1 ? static_cast<int>(blockIdx.x) / tiles : 0;
     const int tile = static_cast<int>(blockIdx.x) - split * tiles;
     int tm, tn;
-    tile_of_block(tile, tiles, tiles_m, tiles_n, tm, tn);
+    tile_of_block(tile, tiles, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = p.m_first + tm * T::BM;
+    const int n0 = p.n_first + tn * kCols;
     const int all = (p.K + 63) / 64;
     const int first = static_cast<int>(static_cast<int64_t>(split) * all / p.splits);
     const int stages = static_cast<int>(static_cast<int64_t>(split + 1) * all / p.splits) - first;
 
     Operand<T::BM, kAAcross, false> a;
     Operand<T::BN, kBAcross, kGated> b;
-    a.init(p.a, p.lda, tm * T::BM, p.M, p.K, wave, lane, wave_m);
-    b.init(p.b, p.ldb, tn * kCols, p.N, p.K, wave, lane, wave_n);
+    a.init(p.a, p.lda, m0, p.M, p.K, wave, lane, wave_m);
+    b.init(p.b, p.ldb, n0, p.N, p.K, wave, lane, wave_n);
 
     f32x4 acc[RM][RN];
 #pragma unroll
@@ -235,7 +235,7 @@ void linear_tile_kernel(const LinearParams p) {
     if (p.splits > 1 && !join_splits<T::kWaves>(p, acc, tile, split, wave, lane)) return;
     constexpr int kOut = OutStage<RM, kGated ? RN / 2 : RN>::kBytes;
     static_assert(T::kWaves * kOut <= T::kLdsBytes, "the epilogue's rows fit");
-    finish<kForm, kBf16>(p, acc, tm * T::BM + wave_m * 16 * RM, tn * kCols + wave_n * (kGated ? 8 : 16) * RN, lane,
+    finish<kForm, kBf16>(p, acc, m0 + wave_m * 16 * RM, n0 + wave_n * (kGated ? 8 : 16) * RN, lane,
                          lds + wave * kOut);
 }
 

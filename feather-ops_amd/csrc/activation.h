@@ -5,8 +5,8 @@
 //   gelu_tanh  g s(z),  z = sqrt(8 / pi) (g + 0.044715 g^3), since (1 + tanh(z / 2)) / 2 = s(z)
 //
 // In fp32 with the exponential and reciprocal instructions, within a few ulp (gelu 2^-19): results are rounded to 16 bits. At the
-// end of a 256 x 256 tile one wave a SIMD does this for 128 values a lane, with nothing beside it: by the library's erfc, some 60
-// instructions, 5000 x 2576 gelu took 40 us more than silu at 4097 rows.
+// end of a 256 x 256 tile one wave a SIMD does this for 128 values a lane, with nothing beside it. gelu by the library's erfc, some
+// 60 instructions: 4097 x 2576 -> 5000 242 us, by the polynomial below 230.
 #pragma once
 
 #include <hip/hip_runtime.h>

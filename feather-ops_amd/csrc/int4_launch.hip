@@ -1,4 +1,5 @@
 // The 4-bit products' kernels of one activation type: compiled with FEATHER_LINEAR_BF16 set to 0 (fp16) or 1 (bf16).
+#include "int4_tile.h"
 #include "linear_few.h"
 #include "linear_launch.h"
 
@@ -34,6 +35,13 @@ void gated(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
     else few<FewRows<4, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
 }
 
+template <Form kForm>
+void tile(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
+    const dim3 groups(static_cast<uint32_t>(plan.tiles * plan.splits));
+    if (plan.kernel == kInt4Tile256) int4_tile_kernel<Int4Tile<256>, kForm, kBf16><<<groups, Int4Tile<256>::kThreads, 0, stream>>>(p);
+    else int4_tile_kernel<Int4Tile<128>, kForm, kBf16><<<groups, Int4Tile<128>::kThreads, 0, stream>>>(p);
+}
+
 template <int kGroups>
 void by_group(const Int4Params& p, const LinearPlan& plan, bool gate, hipStream_t stream) {
     if (p.zero) (gate ? gated<kGroups, true> : plain<kGroups, true>)(p, plan, stream);
@@ -49,7 +57,8 @@ void by_group(const Int4Params& p, const LinearPlan& plan, bool gate, hipStream_
 #endif
 
 void FEATHER_LAUNCH(const Int4Params& p, const LinearPlan& plan, bool gated, hipStream_t stream) {
-    if (p.group == 32) by_group<4>(p, plan, gated, stream);
+    if (plan.kernel <= kInt4Tile128) (gated ? tile<Form::kGated> : tile<Form::kPlain>)(p, plan, stream);
+    else if (p.group == 32) by_group<4>(p, plan, gated, stream);
     else if (p.group == 64) by_group<2>(p, plan, gated, stream);
     else by_group<1>(p, plan, gated, stream);
 }

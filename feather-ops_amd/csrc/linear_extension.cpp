@@ -285,7 +285,7 @@ Tensor int4_forward(const Tensor& x, const Tensor& codes, const Tensor& scale, c
     Tensor y = new_rows(x, M, N, torch_dtype(type));
     torch::stable::accelerator::DeviceGuard guard(x.get_device_index());
     const hipStream_t stream = current_stream(x.get_device_index());
-    if (M <= feather_int4_linear_rows()) {
+    if (feather_int4_linear_direct(w.codes, w.ld_codes, M, N, K, gated)) {
         const Workspace ws = check_workspace(workspace, feather_int4_linear_workspace_bytes(M, N, K, gated), x);
         check_launch(feather_int4_linear(x.const_data_ptr(), ldx, w.codes, w.ld_codes, w.scale, w.ld_scale, w.zero, w.ld_zero,
                                          w.group, bias_data, type, gated, static_cast<int>(activation), y.mutable_data_ptr(), N, M,

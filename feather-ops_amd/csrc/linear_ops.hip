@@ -39,15 +39,28 @@ constexpr TileCost kTiles[] = {
     {kTile256x128, 256, 128, 1, 5.9f, 0.77f, 0.47f},
     {kTile128, 128, 128, 2, 3.8f, 0.82f, 0.48f},
 };
+// The same of 4-bit weights, from 360 timings of 31 shapes (100 to 2048 rows): 2.2% in geometric mean, 38% at most.
+constexpr TileCost kInt4Tiles[] = {
+    {kInt4Tile256, 256, 256, 1, 5.1f, 1.65f, 1.18f},
+    {kInt4Tile128, 128, 256, 2, 2.9f, 1.92f, 0.85f},
+};
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8};
 constexpr float kLaunchCost = 2.0f;   // us from the end of one launch to the next one's work
 
+enum class Kind { kPlain, kGated, kInt4, kInt4Gated };
+
+constexpr bool is_int4(Kind kind) { return kind == Kind::kInt4 || kind == Kind::kInt4Gated; }
+
+const TileCost* tiles_begin(bool int4) { return int4 ? std::begin(kInt4Tiles) : std::begin(kTiles); }
+const TileCost* tiles_end(bool int4) { return int4 ? std::end(kInt4Tiles) : std::end(kTiles); }
+
 // N: columns of b (gated: 2 F).
-LinearPlan tile_plan(int64_t M, int64_t N, int64_t K) {
+LinearPlan tile_plan(int64_t M, int64_t N, int64_t K, bool int4) {
     const int64_t all = ceil_div(K, 64);
-    const float memory = static_cast<float>(N + M) * static_cast<float>(K) / 2.2e6f;   // us at 4.4 TB/s
+    const float memory = (static_cast<float>(N) * (int4 ? 0.25f : 1.0f) + static_cast<float>(M)) * static_cast<float>(K) / 2.2e6f;   // us at 4.4 TB/s
     LinearPlan best{};
-    for (const TileCost& t : kTiles) {
+    for (const TileCost* at = tiles_begin(int4); at != tiles_end(int4); ++at) {
+        const TileCost& t = *at;
         const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
         const int64_t cap = kCUs * t.per_cu;
         for (const int splits : kSplits) {
@@ -127,30 +140,32 @@ struct Parts {
     float cost;
 };
 
-// One launch for a part. Few rows of a gated block, all of its columns, go to a kernel of their own.
-LinearPlan whole_plan(int64_t M, int64_t N, int64_t K, bool all_gated) {
-    if (!all_gated || M > kFewRows) return tile_plan(M, N, K);
-    LinearPlan plan = gated_few_plan(M, N / 2, K);
-    plan.cost = kLaunchCost + 2.0f + static_cast<float>(N) * static_cast<float>(K) / (M > 32 ? 1.6e6f : 2.4e6f);
+// One launch for a part. Few rows of a gated block or of 4-bit weights, all of the columns, go to a kernel of their own.
+LinearPlan whole_plan(Kind kind, int64_t M, int64_t N, int64_t K, bool all_columns) {
+    if (kind == Kind::kPlain || !all_columns || M > kFewRows) return tile_plan(M, N, K, is_int4(kind));
+    const bool gated = kind != Kind::kInt4;
+    LinearPlan plan = is_int4(kind) ? int4_plan(M, gated ? N / 2 : N, K, gated) : gated_few_plan(M, N / 2, K);
+    const float rate = (is_int4(kind) ? 2.0f : 1.0f) * (M > 32 ? 1.6e6f : 2.4e6f);   // weights a us
+    plan.cost = kLaunchCost + 2.0f + static_cast<float>(N) * static_cast<float>(K) / rate;
     return plan;
 }
 
 // Large products go in up to four launches where whole rounds of tiles end at a column or row and the rest does better on
 // other tiles. Cuts fall on multiples of 256 and are tried where a number of whole rounds of each tile ends, along either axis; a
 // part may be cut once more.
-Parts cut(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bool all_gated, int depth) {
-    const LinearPlan whole = whole_plan(M, N, K, all_gated);
+Parts cut(Kind kind, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bool all_columns, int depth) {
+    const LinearPlan whole = whole_plan(kind, M, N, K, all_columns);
     Parts best{{{m0, n0, M, N, whole}}, 1, whole.cost};
     if (depth == 0 || whole.cost < 20.0f) return best;
     const auto attempt = [&](bool rows, int64_t at) {
         const int64_t total = rows ? M : N;
         if (at <= 0 || at >= total) return;
-        const LinearPlan first = rows ? whole_plan(at, N, K, all_gated) : whole_plan(M, at, K, false);
+        const LinearPlan first = rows ? whole_plan(kind, at, N, K, all_columns) : whole_plan(kind, M, at, K, false);
         if (first.cost >= best.cost) return;
-        const Parts heads = depth > 1 ? (rows ? cut(m0, n0, at, N, K, all_gated, depth - 1) : cut(m0, n0, M, at, K, false, depth - 1))
+        const Parts heads = depth > 1 ? (rows ? cut(kind, m0, n0, at, N, K, all_columns, depth - 1) : cut(kind, m0, n0, M, at, K, false, depth - 1))
                                       : Parts{{{m0, n0, rows ? at : M, rows ? N : at, first}}, 1, first.cost};
-        const Parts rest = rows ? cut(m0 + at, n0, M - at, N, K, all_gated, depth - 1)
-                                : cut(m0, n0 + at, M, N - at, K, false, depth - 1);
+        const Parts rest = rows ? cut(kind, m0 + at, n0, M - at, N, K, all_columns, depth - 1)
+                                : cut(kind, m0, n0 + at, M, N - at, K, false, depth - 1);
         const float cost = heads.cost + rest.cost;
         if (cost >= best.cost || heads.count + rest.count > 4) return;
         best.count = 0;
@@ -158,38 +173,37 @@ Parts cut(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bool all_gate
         for (int i = 0; i < rest.count; ++i) best.part[best.count++] = rest.part[i];
         best.cost = cost;
     };
-    for (const TileCost& t : kTiles) {
-        const int64_t round = kCUs * t.per_cu;
-        const int64_t tiles_m = ceil_div(M, t.bm), tiles_n = ceil_div(N, t.bn);
+    for (const TileCost* t = tiles_begin(is_int4(kind)); t != tiles_end(is_int4(kind)); ++t) {
+        const int64_t round = kCUs * t->per_cu;
+        const int64_t tiles_m = ceil_div(M, t->bm), tiles_n = ceil_div(N, t->bn);
         const int64_t rounds = tiles_m * tiles_n / round;
         if (rounds == 0) continue;
-        attempt(false, rounds * round / tiles_m * t.bn / 256 * 256);
-        attempt(true, rounds * round / tiles_n * t.bm / 256 * 256);
+        attempt(false, rounds * round / tiles_m * t->bn / 256 * 256);
+        attempt(true, rounds * round / tiles_n * t->bm / 256 * 256);
     }
     attempt(true, M / 256 * 256);
     return best;
 }
 
 // The launches of a product: the same ones for every call of a shape. A search of large shapes takes up to 0.1 ms of the
-// host, so each thread keeps the last ones by shape.
-const Parts& parts_of(int64_t M, int64_t N, int64_t K, bool gated) {
+// host, so each thread keeps the last ones by shape. Gated: N outputs, whose columns of b are whole pairs of fragments.
+const Parts& parts_of(Kind kind, int64_t M, int64_t N, int64_t K) {
     struct Entry {
+        Kind kind;
         int64_t M, N, K;
-        bool gated;
         Parts parts;
     };
     constexpr uint64_t kEntries = 64;
-    thread_local Entry table[kEntries];
+    thread_local Entry table[kEntries] = {};
     const auto hash = static_cast<uint64_t>(M) * 0x9e3779b97f4a7c15u + static_cast<uint64_t>(N) * 0xc2b2ae3d27d4eb4fu +
-                      static_cast<uint64_t>(K) * 0x165667b19e3779f9u + (gated ? 1u << 31 : 0u);
+                      static_cast<uint64_t>(K) * 0x165667b19e3779f9u + (static_cast<uint64_t>(kind) << 36);
     Entry& e = table[(hash >> 32) % kEntries];
-    if (e.M != M || e.N != N || e.K != K || e.gated != gated || e.parts.count == 0)
-        e = Entry{M, N, K, gated, cut(0, 0, M, N, K, gated, 2)};
+    if (e.M != M || e.N != N || e.K != K || e.kind != kind || e.parts.count == 0) {
+        const bool gated = kind == Kind::kGated || kind == Kind::kInt4Gated;
+        e = Entry{kind, M, N, K, cut(kind, 0, 0, M, gated ? 2 * ceil_div(N, 16) * 16 : N, K, true, 2)};
+    }
     return e.parts;
 }
-
-// Gated: columns of whole pairs of fragments, F rounded up to them.
-const Parts& gated_parts(int64_t M, int64_t F, int64_t K) { return parts_of(M, 2 * ceil_div(F, 16) * 16, K, true); }
 
 int64_t workspace_of(const LinearPlan& plan) {
     return plan.splits > 1 ? kCtrBytes + plan.tiles * plan.splits * plan.tile_bytes : 0;
@@ -213,27 +227,35 @@ bool launchable(const Parts& parts) {
 }
 
 // The launches of a product, one after the other.
-void launch(const LinearParams& whole, const Parts& parts, int type, Operands operands, hipStream_t stream) {
-    const bool gated = operands == Operands::kGated || operands == Operands::kGatedKeep;
+template <typename P, typename Launch>
+void launch(const P& whole, const Parts& parts, Kind kind, Launch&& go) {
+    const bool gated = kind == Kind::kGated || kind == Kind::kInt4Gated;
     for (int i = 0; i < parts.count; ++i) {
         const Part& part = parts.part[i];
-        LinearParams p = whole;
+        P p = whole;
         p.splits = part.plan.splits;
-        if (part.plan.kernel > kTile128) {   // all columns of the rows
+        if (part.plan.kernel > kInt4Tile128) {   // all columns of the rows
             p.a += part.m0 * p.lda;
             p.c = static_cast<uint16_t*>(p.c) + part.m0 * p.ldc;
             if (p.h) p.h += part.m0 * p.ldh;
             p.M = static_cast<int32_t>(part.M);
         } else {
-            const auto tile = *std::find_if(std::begin(kTiles), std::end(kTiles),
-                                            [&](const TileCost& t) { return t.kernel == part.plan.kernel; });
+            const bool int4 = is_int4(kind);
+            const auto tile = *std::find_if(tiles_begin(int4), tiles_end(int4), [&](const TileCost& t) { return t.kernel == part.plan.kernel; });
             p.m_first = static_cast<int32_t>(part.m0);
             p.n_first = static_cast<int32_t>(gated ? part.n0 / 2 : part.n0);
             p.tiles_m = static_cast<int32_t>(ceil_div(part.M, tile.bm));
             p.tiles_n = static_cast<int32_t>(ceil_div(part.N, tile.bn));
         }
-        (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(p, part.plan, operands, stream);
+        go(p, part.plan);
     }
+}
+
+void launch(const LinearParams& p, const Parts& parts, int type, Operands operands, hipStream_t stream) {
+    const bool gated = operands == Operands::kGated || operands == Operands::kGatedKeep;
+    launch(p, parts, gated ? Kind::kGated : Kind::kPlain, [&](const LinearParams& part, const LinearPlan& plan) {
+        (type == FEATHER_BF16 ? linear_launch_bf16 : linear_launch_fp16)(part, plan, operands, stream);
+    });
 }
 
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
@@ -376,7 +398,7 @@ extern "C" bool feather_copy_rows(const void* from, int64_t ld_from, void* to, i
 }
 
 extern "C" int64_t feather_gated_linear_workspace_bytes(int64_t M, int64_t F, int64_t K) {
-    return sizes_ok(M, 2 * F, K) ? workspace_of(gated_parts(M, F, K)) : -1;
+    return sizes_ok(M, 2 * F, K) ? workspace_of(parts_of(Kind::kGated, M, F, K)) : -1;
 }
 
 extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* weight, int64_t ld_weight, const void* bias,
@@ -388,7 +410,7 @@ extern "C" bool feather_gated_linear(const void* x, int64_t ldx, const void* wei
         (bias && !aligned_to_type(bias, type)))
         return false;
     if (kept && (!on_16(kept) || ld_kept % 4 != 0 || ld_kept < 2 * F8 || ld_kept >= int64_t{1} << 22)) return false;
-    const Parts& parts = gated_parts(M, F, K);
+    const Parts& parts = parts_of(Kind::kGated, M, F, K);
     const int64_t need = workspace_of(parts);
     if (!launchable(parts) || !workspace_ok(workspace, workspace_bytes, need)) return false;
     LinearParams p{};
@@ -436,7 +458,7 @@ extern "C" bool feather_gated_backward(const void* grad_y, int64_t ld_grad_y, co
 }
 
 extern "C" int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return sizes_ok(M, N, K) ? workspace_of(parts_of(M, N, K, false)) : -1;
+    return sizes_ok(M, N, K) ? workspace_of(parts_of(Kind::kPlain, M, N, K)) : -1;
 }
 
 extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const void* b, int64_t ldb, bool b_across,
@@ -445,7 +467,7 @@ extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const
     if (!sizes_ok(M, N, K) || !half_type(type) || (a_across && !b_across) || !operand_ok(a, lda, a_across ? M : K) ||
         !operand_ok(b, ldb, b_across ? N : K) || !output_ok(c, ldc, N, type) || (bias && !aligned_to_type(bias, type)))
         return false;
-    const Parts& parts = parts_of(M, N, K, false);
+    const Parts& parts = parts_of(Kind::kPlain, M, N, K);
     const int64_t need = workspace_of(parts);
     if (!launchable(parts) || !workspace_ok(workspace, workspace_bytes, need)) return false;
     LinearParams p{};
@@ -464,9 +486,9 @@ extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const
     return true;
 }
 
-extern "C" int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, int64_t out[16]) {
+extern "C" int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, bool int4, int64_t out[16]) {
     if (!sizes_ok(M, gated ? 2 * N : N, K)) return 0;
-    const Parts& parts = gated ? gated_parts(M, N, K) : parts_of(M, N, K, false);
+    const Parts& parts = parts_of(int4 ? (gated ? Kind::kInt4Gated : Kind::kInt4) : gated ? Kind::kGated : Kind::kPlain, M, N, K);
     for (int i = 0; i < parts.count; ++i) {
         const Part& part = parts.part[i];
         const int64_t launch[4] = {part.plan.kernel, part.plan.splits, part.M, part.N};
@@ -476,12 +498,6 @@ extern "C" int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gat
 }
 
 // ---- 4-bit weights ----
-
-extern "C" void feather_int4_launch(int64_t M, int64_t N, int64_t K, bool gated, int64_t out[2]) {
-    const LinearPlan plan = int4_plan(M, N, K, gated);
-    out[0] = plan.kernel;
-    out[1] = plan.splits;
-}
 
 namespace {
 
@@ -495,10 +511,17 @@ bool int4_ok(const uint8_t* codes, int64_t ld_codes, const void* scale, int64_t 
 
 }  // namespace
 
-extern "C" int64_t feather_int4_linear_rows(void) { return kFewRows; }
-
 extern "C" int64_t feather_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated) {
-    return M <= kFewRows && sizes_ok(M, gated ? 2 * N : N, K) ? workspace_of(int4_plan(M, N, K, gated)) : -1;
+    return sizes_ok(M, gated ? 2 * N : N, K) ? workspace_of(parts_of(gated ? Kind::kInt4Gated : Kind::kInt4, M, N, K)) : -1;
+}
+
+extern "C" bool feather_int4_linear_direct(const uint8_t* codes, int64_t ld_codes, int64_t M, int64_t N, int64_t K, bool gated) {
+    const int64_t rows = gated ? 2 * N : N;
+    if (M <= kFewRows || !sizes_ok(M, rows, K)) return true;
+    if (!on_16(codes) || ld_codes % 16 != 0) return false;
+    // Dequantized, codes are read and values written, and read again (us at 4.4 TB/s).
+    const float before = kLaunchCost + static_cast<float>(rows) * static_cast<float>(K) * (2.5f / 4.4e6f);
+    return parts_of(gated ? Kind::kInt4Gated : Kind::kInt4, M, N, K).cost <= before + parts_of(gated ? Kind::kGated : Kind::kPlain, M, N, K).cost;
 }
 
 extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64_t ld_codes, const void* scale,
@@ -506,20 +529,21 @@ extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* c
                                     bool gated, int activation, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
                                     void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     const int64_t rows = gated ? 2 * N : N;
-    if (N < 1 || M > kFewRows || !sizes_ok(M, rows, K) || !half_type(type) || activation < 0 || activation > 2 ||
+    if (N < 1 || !sizes_ok(M, rows, K) || !half_type(type) || activation < 0 || activation > 2 ||
         !operand_ok(x, ldx, K) || !output_ok(y, ldy, N, type) || (bias && !aligned_to_type(bias, type)) ||
-        !int4_ok(codes, ld_codes, scale, ld_scale, zero, ld_zero, group, type, rows, K))
+        !int4_ok(codes, ld_codes, scale, ld_scale, zero, ld_zero, group, type, rows, K) ||
+        (M > kFewRows && (!on_16(codes) || ld_codes % 16 != 0)))
         return false;
-    const LinearPlan plan = int4_plan(M, N, K, gated);
-    const int64_t need = workspace_of(plan);
-    if (!launchable(plan) || !workspace_ok(workspace, workspace_bytes, need)) return false;
+    const Kind kind = gated ? Kind::kInt4Gated : Kind::kInt4;
+    const Parts& parts = parts_of(kind, M, N, K);
+    const int64_t need = workspace_of(parts);
+    if (!launchable(parts) || !workspace_ok(workspace, workspace_bytes, need)) return false;
     Int4Params p{};
     p.a = static_cast<const uint16_t*>(x);
     p.lda = ldx;
     p.M = static_cast<int32_t>(M);
     p.N = static_cast<int32_t>(N);
     p.K = static_cast<int32_t>(K);
-    p.splits = plan.splits;
     p.bias = bias;
     p.c = y;
     p.ldc = ldy;
@@ -532,6 +556,8 @@ extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* c
     p.ld_scale = ld_scale;
     p.ld_zero = ld_zero;
     p.group = group;
-    (type == FEATHER_BF16 ? int4_launch_bf16 : int4_launch_fp16)(p, plan, gated, stream);
+    launch(p, parts, kind, [&](const Int4Params& part, const LinearPlan& plan) {
+        (type == FEATHER_BF16 ? int4_launch_bf16 : int4_launch_fp16)(part, plan, gated, stream);
+    });
     return true;
 }

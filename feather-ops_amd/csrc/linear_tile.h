@@ -59,9 +59,10 @@ struct Operand {
     const uint16_t* base;      // of the workgroup's first row (or column)
     int64_t ld;
     int32_t rows, K;           // rows (columns, in whole pieces of 8) of the operand from there on, and its depth
-    rsrc_t rsrc;               // along: the whole of the workgroup's rows
-    uint32_t off[kKeys];
-    uint32_t step;
+    static constexpr int kOffsets = kAcross ? kKeys : kSize / 32;
+    uint32_t off[kOffsets];    // along: of each load
+    uint32_t step;             // across: between loads
+    uint32_t bytes;            // along
     int32_t piece;             // along: the k of this lane's piece in a stage
     uint32_t read_at;
 
@@ -92,27 +93,31 @@ struct Operand {
             const int most = kGated ? kSize / 2 : kSize;
             base = p + mine * ld;
             rows = total - first < most ? total - first : most;
-            rsrc = make_rsrc(base, static_cast<uint32_t>(rows - 1) * pitch + static_cast<uint32_t>((K + 7) & ~7) * 2u);
+            bytes = static_cast<uint32_t>(rows - 1) * pitch + static_cast<uint32_t>((K + 7) & ~7) * 2u;
             const int row = (kGated ? 8 * (wave & 1) : 8 * wave) + lane / 8;
             const int at = (lane % 8) ^ (lane / 8);
             piece = at * 8;
-            off[0] = static_cast<uint32_t>(row) * pitch + static_cast<uint32_t>(at) * 16u;
-            step = (kGated ? 16u : 32u) * pitch;
+#pragma unroll
+            for (int d = 0; d < kOffsets; ++d)
+                off[d] = static_cast<uint32_t>(row + d * (kGated ? 16 : 32)) * pitch + static_cast<uint32_t>(at) * 16u;
             const int r16 = lane % 16, g = lane / 16;
             read_at = static_cast<uint32_t>((part * 16 * R + r16) * 128 + ((g ^ (r16 % 8)) << 4));
         }
     }
 
-    // Load d of a stage into a unit (zeros, into a unit that nobody reads, where the stage is past the end).
+    // Load d of a stage into a unit (zeros, into a unit that nobody reads, where the stage is past the end). kLast: the stage may
+    // be K's last, which may have less than 64.
+    template <bool kLast>
     __device__ __forceinline__ void load(int d, int stage, bool live, uint8_t* unit, int wave) const {
         uint8_t* const to = unit + (wave + d * kWaves) * 1024;
         if constexpr (kAcross) {
             const int left = K - stage * 64;
             const int here = left < 64 ? left : 64;
-            const uint32_t bytes = live ? static_cast<uint32_t>(here - 1) * static_cast<uint32_t>(ld * 2) + static_cast<uint32_t>(rows) * 2u : 0u;
-            dma16(make_rsrc(base + static_cast<int64_t>(stage) * 64 * ld, bytes), to, off[d % kKeys] + d * step);
+            const uint32_t size = live ? static_cast<uint32_t>(here - 1) * static_cast<uint32_t>(ld * 2) + static_cast<uint32_t>(rows) * 2u : 0u;
+            dma16(make_rsrc(base + static_cast<int64_t>(stage) * 64 * ld, size), to, off[d % kKeys] + d * step);
         } else {
-            dma16(rsrc, to, (live && piece < K - stage * 64 ? off[0] : kOob) + d * step, static_cast<uint32_t>(stage) * 128u);
+            const bool in = !kLast || piece < K - stage * 64;
+            dma16(make_rsrc(base, live ? bytes : 0u), to, in ? off[d] : kOob, static_cast<uint32_t>(stage) * 128u);
         }
     }
 
@@ -149,7 +154,9 @@ void linear_tile_kernel(const LinearParams p) {
     const int n0 = p.n_first + tn * kCols;
     const int all = (p.K + 63) / 64;
     const int first = static_cast<int>(static_cast<int64_t>(split) * all / p.splits);
-    const int stages = static_cast<int>(static_cast<int64_t>(split + 1) * all / p.splits) - first;
+    // The last stage comes first: the loop's loads need not look for K's end.
+    const int last = static_cast<int>(static_cast<int64_t>(split + 1) * all / p.splits) - 1;
+    const int stages = last + 1 - first;
 
     Operand<T::BM, kAAcross, false> a;
     Operand<T::BN, kBAcross, kGated> b;
@@ -168,9 +175,9 @@ void linear_tile_kernel(const LinearParams p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int d = 0; d < T::kALoads; ++d) a.load(d, first + t, t < stages, lds + (t ? na : ua), wave);
+        for (int d = 0; d < T::kALoads; ++d) a.template load<true>(d, t ? first : last, t < stages, lds + (t ? na : ua), wave);
 #pragma unroll
-        for (int d = 0; d < T::kBLoads; ++d) b.load(d, first + t, t < stages, lds + (t ? nb : ub), wave);
+        for (int d = 0; d < T::kBLoads; ++d) b.template load<true>(d, t ? first : last, t < stages, lds + (t ? nb : ub), wave);
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::kALoads + T::kBLoads));
     barrier_only();
@@ -184,8 +191,7 @@ void linear_tile_kernel(const LinearParams p) {
     for (int r = 0; r < RM + RN; ++r) read(r, 0, ua, ub);
 
     const auto multiply = [&](int m, int s) {
-        const int i = m / RN;
-        const int j = i % 2 ? RN - 1 - m % RN : m % RN;
+        const int i = m / RN, j = m % RN;
         acc[i][j] = mfma16<kBf16>(__builtin_bit_cast(half8, w[s][j]), __builtin_bit_cast(half8, x[s][i]), acc[i][j]);
     };
     for (int t = 0; t < stages; ++t) {
@@ -195,7 +201,7 @@ void linear_tile_kernel(const LinearParams p) {
             multiply(m, 0);
             if (m % T::kReadStep == 0) read(m / T::kReadStep, 1, ua, ub);
             if (m % T::kALoadStep == 1 && m / T::kALoadStep < T::kALoads)
-                a.load(m / T::kALoadStep, first + t + 2, t + 2 < stages, lds + fa, wave);
+                a.template load<false>(m / T::kALoadStep, first + t + 1, t + 2 < stages, lds + fa, wave);
             __builtin_amdgcn_sched_barrier(0);
         }
         // Second half: past the barrier stage t is read and stage t + 1 has landed, for every wave.
@@ -211,7 +217,7 @@ void linear_tile_kernel(const LinearParams p) {
                 const int n = m - T::kBarrier;
                 if (n % T::kReadStep == 0) read(n / T::kReadStep, 0, na, nb);
                 if (n % T::kBLoadStep == 1 && n / T::kBLoadStep < T::kBLoads)
-                    b.load(n / T::kBLoadStep, first + t + 2, t + 2 < stages, lds + ub, wave);
+                    b.template load<false>(n / T::kBLoadStep, first + t + 1, t + 2 < stages, lds + ub, wave);
             }
             __builtin_amdgcn_sched_barrier(0);
         }

@@ -92,8 +92,6 @@ def c_library() -> ctypes.CDLL:
             bytes_of = getattr(lib, f"feather_{name}_workspace_bytes")
             bytes_of.restype = ctypes.c_int64
             bytes_of.argtypes = [ctypes.c_int64] * 3 + flags
-        lib.feather_int4_linear_rows.restype = ctypes.c_int64
-        lib.feather_int4_linear_rows.argtypes = []
         _c_library = lib
     return _c_library
 

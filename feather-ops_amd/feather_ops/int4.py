@@ -111,12 +111,9 @@ def dequantize_int4(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor
 def _workspace_bytes(M: int, rows: int, K: int, gated: bool, trains: bool) -> int:
     lib = _lib.c_library()
     n, k8 = rows // 2 if gated else rows, -(-K // 8) * 8
-    if M <= lib.feather_int4_linear_rows():
-        need = lib.feather_int4_linear_workspace_bytes(M, n, K, gated)
-    elif gated:
-        need = _gated_workspace_bytes(M, n, k8, False)
-    else:
-        need = lib.feather_product_workspace_bytes(M, n, k8)
+    need = lib.feather_int4_linear_workspace_bytes(M, n, K, gated)
+    if M > 64:   # some go through the product in 16 bits, by their sizes and the codes' alignment
+        need = max(need, _gated_workspace_bytes(M, n, k8, False) if gated else lib.feather_product_workspace_bytes(M, n, k8))
     return max(0, need, lib.feather_product_workspace_bytes(M, K, rows) if trains else 0)
 
 

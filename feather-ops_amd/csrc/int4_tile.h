@@ -220,10 +220,11 @@ void int4_tile_kernel(const Int4Params p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int d = 0; d < T::kALoads; ++d) a.template load<true>(d, t ? first : last, t < stages, lds + (t ? na : ua), wave);
+        for (int d = 0; d < T::kALoads; ++d) a.load(d, t ? first : last, t < stages, lds + (t ? na : ua), wave);
 #pragma unroll
         for (int d = 0; d < T::kBLoads; ++d) load_b(d, t ? first : last, t < stages, t ? nb : ub);
     }
+    a.start(first + 1);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::kALoads + T::kBLoads));
     barrier_only();
 #pragma unroll
@@ -258,7 +259,7 @@ void int4_tile_kernel(const Int4Params p) {
             multiply(m, 0);
             if constexpr (m % RN == RN - 1) x[m / RN] = a.read(lds, ua, m / RN, 1);
             static_assert(T::kMfmas == 8 * T::kALoads, "a's loads fill the half");
-            if constexpr (m % 8 == 1) a.template load<false>(m / 8, first + t + 1, t + 2 < stages, lds + fa, wave);
+            if constexpr (m % 8 == 1) a.load_next(m / 8, t + 2 < stages, lds, fa, wave);
             decode_at(m, std::integral_constant<int, 0>{}, 1);
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -284,6 +285,7 @@ void int4_tile_kernel(const Int4Params p) {
             }
             __builtin_amdgcn_sched_barrier(0);
         });
+        a.advance();
         const uint32_t freed = ua;
         ua = na;
         na = fa;

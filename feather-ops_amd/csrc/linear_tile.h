@@ -62,7 +62,8 @@ struct Operand {
     static constexpr int kOffsets = kAcross ? kKeys : kSize / 32;
     uint32_t off[kOffsets];    // along: of each load
     uint32_t step;             // across: between loads
-    uint32_t bytes;            // along
+    uint32_t bytes;            // along: of the workgroup's rows; across: of a stage's
+    uint32_t at;               // along: of the next stage in a row
     int32_t piece;             // along: the k of this lane's piece in a stage
     uint32_t read_at;
 
@@ -105,9 +106,8 @@ struct Operand {
         }
     }
 
-    // Load d of a stage into a unit (zeros, into a unit that nobody reads, where the stage is past the end). kLast: the stage may
-    // be K's last, which may have less than 64.
-    template <bool kLast>
+    // Load d of a stage into a unit (zeros, into a unit that nobody reads, where the stage is past the end). The stage may be K's
+    // last, which may have less than 64.
     __device__ __forceinline__ void load(int d, int stage, bool live, uint8_t* unit, int wave) const {
         uint8_t* const to = unit + (wave + d * kWaves) * 1024;
         if constexpr (kAcross) {
@@ -116,9 +116,28 @@ struct Operand {
             const uint32_t size = live ? static_cast<uint32_t>(here - 1) * static_cast<uint32_t>(ld * 2) + static_cast<uint32_t>(rows) * 2u : 0u;
             dma16(make_rsrc(base + static_cast<int64_t>(stage) * 64 * ld, size), to, off[d % kKeys] + d * step);
         } else {
-            const bool in = !kLast || piece < K - stage * 64;
-            dma16(make_rsrc(base, live ? bytes : 0u), to, in ? off[d] : kOob, static_cast<uint32_t>(stage) * 128u);
+            dma16(make_rsrc(base, live ? bytes : 0u), to, piece < K - stage * 64 ? off[d] : kOob, static_cast<uint32_t>(stage) * 128u);
         }
+    }
+
+    // The same of whole stages, one after the other from `stage` on.
+    __device__ __forceinline__ void start(int stage) {
+        if constexpr (kAcross) {
+            base += static_cast<int64_t>(stage) * 64 * ld;
+            bytes = 63u * static_cast<uint32_t>(ld * 2) + static_cast<uint32_t>(rows) * 2u;
+        } else {
+            at = static_cast<uint32_t>(stage) * 128u;
+        }
+    }
+    __device__ __forceinline__ void load_next(int d, bool live, uint8_t* lds, uint32_t unit, int wave) const {
+        uint8_t* const to = lds + unit + (wave + d * kWaves) * 1024;
+        const rsrc_t rsrc = make_rsrc(base, live ? bytes : 0u);
+        if constexpr (kAcross) dma16(rsrc, to, off[d % kKeys] + d * step);
+        else dma16(rsrc, to, off[d], at);
+    }
+    __device__ __forceinline__ void advance() {
+        if constexpr (kAcross) base += 64 * ld;
+        else at += 128;
     }
 
     // Fragment i of half s of a stage.
@@ -175,10 +194,12 @@ void linear_tile_kernel(const LinearParams p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int d = 0; d < T::kALoads; ++d) a.template load<true>(d, t ? first : last, t < stages, lds + (t ? na : ua), wave);
+        for (int d = 0; d < T::kALoads; ++d) a.load(d, t ? first : last, t < stages, lds + (t ? na : ua), wave);
 #pragma unroll
-        for (int d = 0; d < T::kBLoads; ++d) b.template load<true>(d, t ? first : last, t < stages, lds + (t ? nb : ub), wave);
+        for (int d = 0; d < T::kBLoads; ++d) b.load(d, t ? first : last, t < stages, lds + (t ? nb : ub), wave);
     }
+    a.start(first + 1);
+    b.start(first + 1);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::kALoads + T::kBLoads));
     barrier_only();
     // Read r of a half: the first row of a, the rows of b, the other rows of a, the order of their use.
@@ -201,7 +222,7 @@ void linear_tile_kernel(const LinearParams p) {
             multiply(m, 0);
             if (m % T::kReadStep == 0) read(m / T::kReadStep, 1, ua, ub);
             if (m % T::kALoadStep == 1 && m / T::kALoadStep < T::kALoads)
-                a.template load<false>(m / T::kALoadStep, first + t + 1, t + 2 < stages, lds + fa, wave);
+                a.load_next(m / T::kALoadStep, t + 2 < stages, lds, fa, wave);
             __builtin_amdgcn_sched_barrier(0);
         }
         // Second half: past the barrier stage t is read and stage t + 1 has landed, for every wave.
@@ -217,10 +238,12 @@ void linear_tile_kernel(const LinearParams p) {
                 const int n = m - T::kBarrier;
                 if (n % T::kReadStep == 0) read(n / T::kReadStep, 0, na, nb);
                 if (n % T::kBLoadStep == 1 && n / T::kBLoadStep < T::kBLoads)
-                    b.template load<false>(n / T::kBLoadStep, first + t + 1, t + 2 < stages, lds + ub, wave);
+                    b.load_next(n / T::kBLoadStep, t + 2 < stages, lds, ub, wave);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        a.advance();
+        b.advance();
         const uint32_t freed = ua;
         ua = na;
         na = fa;

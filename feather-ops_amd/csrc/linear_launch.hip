@@ -30,6 +30,7 @@ void few(const LinearParams& p, const LinearPlan& plan, hipStream_t stream) {
 template <Form kForm>
 void gated(const LinearParams& p, const LinearPlan& plan, hipStream_t stream) {
     if (plan.kernel == kFew16_2_8_1) few<FewRows<1, 2, 8, 1>, kForm>(p, plan, stream);
+    else if (plan.kernel == kFew16_2_4_2) few<FewRows<1, 2, 4, 2>, kForm>(p, plan, stream);
     else if (plan.kernel == kFew32_4_4_2) few<FewRows<2, 4, 4, 2>, kForm>(p, plan, stream);
     else if (plan.kernel == kFew32_2_4_2) few<FewRows<2, 2, 4, 2>, kForm>(p, plan, stream);
     else if (plan.kernel == kFew64_2_4_2) few<FewRows<4, 2, 4, 2>, kForm>(p, plan, stream);

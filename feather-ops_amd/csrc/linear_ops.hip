@@ -119,12 +119,13 @@ LinearPlan int4_plan(int64_t M, int64_t N, int64_t K, bool gated) {
     return few_plan(kFew16_1_16_1, 1, 1, 16, 1, N, K, gated, 64);
 }
 
-// 16-bit weights, measured alike: 1 row of 4096 -> 14336 2_8_1 42.5, 2_4_1 48.7; 24 rows of 5120 -> 13824 4_4_2 57.7, 2_4_2 60.4,
-// 2_8_1 74.7.
+// 16-bit weights, measured alike: 1 row of 4096 -> 14336 2_8_1 42.5, 2_4_1 48.7; of 2048 -> 2048 7.5, 2_4_2 10.2; of 14336 -> 4096
+// 51.4, 2_4_2 48.1. 24 rows of 5120 -> 13824 4_4_2 57.7, 2_4_2 60.4, 2_8_1 74.7.
 LinearPlan gated_few_plan(int64_t M, int64_t F, int64_t K) {
     if (M > 32) return few_plan(kFew64_2_4_2, 4, 2, 4, 2, F, K, true, 8);
     if (M > 16 && F > 64 * 160) return few_plan(kFew32_4_4_2, 2, 4, 4, 2, F, K, true, 8);
     if (M > 16) return few_plan(kFew32_2_4_2, 2, 2, 4, 2, F, K, true, 8);
+    if (K > 8192) return few_plan(kFew16_2_4_2, 1, 2, 4, 2, F, K, true, 8);
     return few_plan(kFew16_2_8_1, 1, 2, 8, 1, F, K, true, 16);
 }
 
@@ -140,18 +141,27 @@ struct Parts {
     float cost;
 };
 
+// Microseconds of a launch for few rows: by its K, a workgroup's own time, or by its weights, whichever is more.
+struct FewCost {
+    int rows;
+    float fixed, by_k, rate;
+};
+constexpr FewCost kInt4Few[] = {{16, 4.2f, 0.0004f, 7.1e6f}, {32, 6.9f, 0.0005f, 4.75e6f}, {64, 10.2f, 0.00066f, 2.86e6f}};
+constexpr FewCost kGatedFew[] = {{16, 5.3f, 0.0011f, 2.4e6f}, {32, 9.5f, 0.00075f, 2.4e6f}, {64, 11.0f, 0.0008f, 2.05e6f}};
+
 // One launch for a part. Few rows of a gated block or of 4-bit weights, all of the columns, go to a kernel of their own.
 LinearPlan whole_plan(Kind kind, int64_t M, int64_t N, int64_t K, bool all_columns) {
     if (kind == Kind::kPlain || !all_columns || M > kFewRows) return tile_plan(M, N, K, is_int4(kind));
     const bool gated = kind != Kind::kInt4;
     LinearPlan plan = is_int4(kind) ? int4_plan(M, gated ? N / 2 : N, K, gated) : gated_few_plan(M, N / 2, K);
-    const float rate = (is_int4(kind) ? 2.0f : 1.0f) * (M > 32 ? 1.6e6f : 2.4e6f);   // weights a us
-    plan.cost = kLaunchCost + 2.0f + static_cast<float>(N) * static_cast<float>(K) / rate;
+    const FewCost* cost = is_int4(kind) ? kInt4Few : kGatedFew;
+    while (M > cost->rows) ++cost;
+    plan.cost = std::max(cost->fixed + cost->by_k * static_cast<float>(K), 2.0f + static_cast<float>(N) * static_cast<float>(K) / cost->rate);
     return plan;
 }
 
 // Large products go in up to four launches where whole rounds of tiles end at a column or row and the rest does better on
-// other tiles. Cuts fall on multiples of 256 and are tried where a number of whole rounds of each tile ends, along either axis; a
+// other tiles. Cuts fall on multiples of 256 (or on 64 rows) and are tried where a number of whole rounds of each tile ends, along either axis; a
 // part may be cut once more.
 Parts cut(Kind kind, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bool all_columns, int depth) {
     const LinearPlan whole = whole_plan(kind, M, N, K, all_columns);
@@ -182,6 +192,7 @@ Parts cut(Kind kind, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bo
         attempt(true, rounds * round / tiles_n * t->bm / 256 * 256);
     }
     attempt(true, M / 256 * 256);
+    if (is_int4(kind) && M <= 2 * kFewRows) attempt(true, kFewRows);   // two launches for few rows: 96 x 4096 -> 4096 22.7 us, a tile's 27.6
     return best;
 }
 

@@ -19,6 +19,8 @@ PRODUCT = {
 GATED = {
     (1, 33, 40): [("few 16 2/8/1", False)],
     (3, 35, 4104): [("few 16 2/8/1", True)],
+    (3, 4203, 8200): [("few 16 2/4/2", False)],
+    (5, 45, 8200): [("few 16 2/4/2", True)],
     (19, 10301, 72): [("few 32 4/4/2", False)],
     (17, 33, 136): [("few 32 2/4/2", False)],
     (23, 45, 2056): [("few 32 2/4/2", True)],
@@ -30,7 +32,7 @@ GATED = {
     (501, 5205, 8200): [("tile 256x256", True)],
     (701, 3101, 4104): [("tile 256x128", False)],
     (703, 2101, 16392): [("tile 256x128", True)],
-    (1303, 3101, 520): [("tile 128x128", False), ("few 32 2/4/2", False)],
+    (1303, 3101, 520): [("tile 128x128", False)],
     (1301, 2101, 16392): [("tile 256x256", True), ("few 32 2/4/2", True)],
     (1001, 8301, 1032): [("tile 256x256", False), ("tile 128x128", True)],
 }
@@ -45,6 +47,7 @@ INT4 = {
     (61, 45, 2055): [("few 64 2/4/2", True)],
     (65, 33, 39): [("int4 128x256", False)],
     (67, 45, 1031): [("int4 128x256", True)],
+    (70, 45, 4103): [("few 64 2/4/2", True), ("few 16 1/16/1", False)],
     (701, 21005, 519): [("int4 256x256", False)],
     (703, 10301, 4103): [("int4 256x256", True)],
     (1001, 16501, 1031): [("int4 256x256", False), ("int4 128x256", True)],
@@ -63,9 +66,10 @@ INT4_GATED = {
     (61, 45, 2055): [("few 64 2/4/2", True)],
     (65, 33, 39): [("int4 128x256", False)],
     (67, 45, 1031): [("int4 128x256", True)],
+    (99, 45, 4103): [("few 64 2/4/2", True), ("few 64 2/4/2", True)],
     (701, 5205, 4103): [("int4 256x256", True)],
     (1001, 8301, 1031): [("int4 256x256", False), ("int4 128x256", True)],
     (1301, 3101, 4103): [("int4 256x256", True), ("few 32 2/4/2", True)],
 }
 # Which of the kernels have no K split in any plan.
-NEVER_SPLIT = {"few 16 1/8/2", "few 32 4/4/2", "few 16 2/4/2", "few 32 2/4/4"}
+NEVER_SPLIT = {"few 16 1/8/2", "few 32 4/4/2", "few 32 2/4/4"}

@@ -1,4 +1,5 @@
-// 4-bit weights: their quantization, and back to 16 bits (include/feather_linear_ops.h). Streams through memory, which bounds both.
+// 4-bit weights: their quantization, and back to 16 bits (include/feather_linear_ops.h). Streams through memory, which bounds both:
+// 14336 x 4096 to 16 bits 28-34 us, 4.3-5.2 TB/s, of which the values written are four fifths.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -2,6 +2,10 @@
 // codes. Each wave takes them to 16 bits in registers, (q - z) s rounded once, between its matrix instructions. So that no value
 // is taken twice in a workgroup its 4 waves lie side by side, each with all of the tile's rows and 64 of its 256 columns: 128 KB
 // of LDS reads a stage either way, of 256 rows.
+//
+// What bounds it are instructions: a stage of 256 rows has 128 MFMAs and some 500 others of a wave, which issues one in four
+// clocks. A stage takes 1.4 us on one CU (linear_tile.h's 1.0), and 1000 x 4096 -> 14336 100-115 us, where dequantizing takes 37
+// and the product 86. From about 2000 rows on the other way is faster (4096 x 4096 -> 14336 411 us, 366).
 #pragma once
 
 #include <utility>

@@ -64,8 +64,9 @@ Tensor as_operand(const Tensor& t) {
     return out;
 }
 
-// y = act(x Wg^T + bg) * (x Wu^T + bu). Both sums are kept in fp32: rounded to 16 bits they cost the gradients more than the
-// gradients' own rounding (from bf16 2.9e-3 of them, of 2.3e-3).
+// y = act(x Wg^T + bg) * (x Wu^T + bu). Both sums are kept in fp32: rounded to bf16 they make the gradients' error, 2.34e-3 of
+// their norm, 2.96e-3 (512 x 512 -> 512, computed in 64 bits). They cost 80 us forward and as much backward of the 1920 of 4096 x
+// 4096 -> 12288.
 struct GatedLinear : public Function<GatedLinear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
                           int64_t activation, const std::optional<Tensor>& workspace) {

@@ -1,5 +1,7 @@
 // The kernel for few rows, with 16-bit or 4-bit weights. The weight is read once, straight into registers, and that is what
-// bounds it; the rows of x, which every workgroup reads, go through LDS.
+// bounds it; the rows of x, which every workgroup reads, go through LDS. One row of 4096 -> 14336 gated takes 44 us in 16 bits (5.3
+// TB/s) and 16.0 with 4-bit weights (3.7; the loads alone 14.5), 24 rows of 5120 -> 13824 57 and 32.5 (5.0 and 2.3; the loads alone
+// 25: codes become 16 bits between them).
 //
 // A workgroup's waves are WK parts of K by WN parts of its columns. An iteration takes WK steps of 128 k's, one to each part: its
 // rows of x are in one of two LDS buffers, in the order in which the matrix instructions take them, the next iteration's on

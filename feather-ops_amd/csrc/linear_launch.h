@@ -5,8 +5,8 @@
 
 namespace feather {
 
-// Tiles by their rows and columns (kInt4Tile...: of 4-bit weights, 256 columns); kernels for few rows by their rows (kFew...), with RN fragments of columns a wave, WK parts of K
-// and WN of the columns (...RN_WK_WN).
+// Tiles by their rows and columns (kInt4Tile...: of 4-bit weights, 256 columns); kernels for few rows by their rows (kFew...), with
+// RN fragments of columns a wave, WK parts of K and WN of the columns (...RN_WK_WN).
 enum LinearKernel : int {
     kTile256, kTile256x128, kTile128, kInt4Tile256, kInt4Tile128,
     kFew16_1_16_1, kFew16_1_8_2, kFew16_2_8_1, kFew16_2_4_2, kFew16_2_16_1, kFew32_1_4_4, kFew32_2_4_4, kFew32_2_4_2, kFew32_4_4_2,

@@ -26,23 +26,25 @@ bool splits_fit(const LinearPlan& plan) {
 }
 
 // A tile, and microseconds: of a workgroup's start and end, and of a stage of 64 where workgroups fill the chip (per_cu on each CU)
-// and where there is one alone, with what lies between in proportion. The figures minimise what the pick of tile and K splits
-// loses against the best pair in 2900 timings of 178 shapes (100 to 4096 rows, 1024 to 28672 columns, K 512 to 14336): 1.4% in
-// geometric mean, 23% at most.
+// and where there is one alone, with what lies between in proportion; and of the join of a split K: once, of each 64 K sums that
+// a tile's workgroups write and read back, and of 16 M sums in all.
 struct TileCost {
     LinearKernel kernel;
     int bm, bn, per_cu;
     float fixed, full, lone;
+    float join, each, all;
 };
+// They minimise what the pick of tile and K splits loses against the best pair, and the error of the times, in 2900 timings of 233
+// shapes (100 to 4096 rows, 1024 to 28672 columns, K 512 to 14336): 1.3% in geometric mean, 31% at most; times are 10% off.
 constexpr TileCost kTiles[] = {
-    {kTile256, 256, 256, 1, 9.8f, 1.30f, 1.28f},
-    {kTile256x128, 256, 128, 1, 5.9f, 0.77f, 0.47f},
-    {kTile128, 128, 128, 2, 3.8f, 0.82f, 0.48f},
+    {kTile256, 256, 256, 1, 8.2f, 1.29f, 0.82f, 2.1f, 2.2f, 7.8f},
+    {kTile256x128, 256, 128, 1, 4.4f, 0.77f, 0.41f, 2.1f, 2.2f, 7.8f},
+    {kTile128, 128, 128, 2, 2.2f, 0.84f, 0.36f, 2.1f, 2.2f, 7.8f},
 };
-// The same of 4-bit weights, from 360 timings of 31 shapes (100 to 2048 rows): 2.2% in geometric mean, 38% at most.
+// The same of 4-bit weights, from 844 timings of 86 shapes (70 to 4096 rows): 1.1%, 14% at most; times are 8% off.
 constexpr TileCost kInt4Tiles[] = {
-    {kInt4Tile256, 256, 256, 1, 5.1f, 1.65f, 1.18f},
-    {kInt4Tile128, 128, 256, 2, 2.9f, 1.92f, 0.85f},
+    {kInt4Tile256, 256, 256, 1, 8.3f, 1.51f, 1.17f, 4.0f, 2.2f, 8.0f},
+    {kInt4Tile128, 128, 256, 2, 4.5f, 1.88f, 0.68f, 4.0f, 2.2f, 8.0f},
 };
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8};
 constexpr float kLaunchCost = 2.0f;   // us from the end of one launch to the next one's work
@@ -57,7 +59,8 @@ const TileCost* tiles_end(bool int4) { return int4 ? std::end(kInt4Tiles) : std:
 // N: columns of b (gated: 2 F).
 LinearPlan tile_plan(int64_t M, int64_t N, int64_t K, bool int4) {
     const int64_t all = ceil_div(K, 64);
-    const float memory = (static_cast<float>(N) * (int4 ? 0.25f : 1.0f) + static_cast<float>(M)) * static_cast<float>(K) / 2.2e6f;   // us at 4.4 TB/s
+    // us at 4.4 TB/s
+    const float memory = (static_cast<float>(N) * (int4 ? 0.25f : 1.0f) + static_cast<float>(M)) * static_cast<float>(K) / 2.2e6f;
     LinearPlan best{};
     for (const TileCost* at = tiles_begin(int4); at != tiles_end(int4); ++at) {
         const TileCost& t = *at;
@@ -75,8 +78,8 @@ LinearPlan tile_plan(int64_t M, int64_t N, int64_t K, bool int4) {
             cost = std::max(cost, memory);
             // sums are written, and the last of a tile's workgroups reads all of its back
             if (splits > 1)
-                cost += 1.8f + static_cast<float>(t.bm * t.bn) * static_cast<float>(splits) *
-                                    (3.9f / 65536.0f + static_cast<float>(tiles) * (4.4f / 16777216.0f));
+                cost += t.join + static_cast<float>(t.bm * t.bn) * static_cast<float>(splits) *
+                                     (t.each / 65536.0f + static_cast<float>(tiles) * (t.all / 16777216.0f));
             plan.cost = cost + kLaunchCost;
             if (best.cost == 0.0f || plan.cost < best.cost) best = plan;
         }
@@ -156,7 +159,8 @@ LinearPlan whole_plan(Kind kind, int64_t M, int64_t N, int64_t K, bool all_colum
     LinearPlan plan = is_int4(kind) ? int4_plan(M, gated ? N / 2 : N, K, gated) : gated_few_plan(M, N / 2, K);
     const FewCost* cost = is_int4(kind) ? kInt4Few : kGatedFew;
     while (M > cost->rows) ++cost;
-    plan.cost = std::max(cost->fixed + cost->by_k * static_cast<float>(K), 2.0f + static_cast<float>(N) * static_cast<float>(K) / cost->rate);
+    const float weights = static_cast<float>(N) * static_cast<float>(K);
+    plan.cost = std::max(cost->fixed + cost->by_k * static_cast<float>(K), 2.0f + weights / cost->rate);
     return plan;
 }
 
@@ -172,8 +176,10 @@ Parts cut(Kind kind, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bo
         if (at <= 0 || at >= total) return;
         const LinearPlan first = rows ? whole_plan(kind, at, N, K, all_columns) : whole_plan(kind, M, at, K, false);
         if (first.cost >= best.cost) return;
-        const Parts heads = depth > 1 ? (rows ? cut(kind, m0, n0, at, N, K, all_columns, depth - 1) : cut(kind, m0, n0, M, at, K, false, depth - 1))
-                                      : Parts{{{m0, n0, rows ? at : M, rows ? N : at, first}}, 1, first.cost};
+        const Parts whole_heads{{{m0, n0, rows ? at : M, rows ? N : at, first}}, 1, first.cost};
+        const Parts heads = depth == 1 ? whole_heads
+                            : rows     ? cut(kind, m0, n0, at, N, K, all_columns, depth - 1)
+                                       : cut(kind, m0, n0, M, at, K, false, depth - 1);
         const Parts rest = rows ? cut(kind, m0 + at, n0, M - at, N, K, all_columns, depth - 1)
                                 : cut(kind, m0, n0 + at, M, N - at, K, false, depth - 1);
         const float cost = heads.cost + rest.cost;
@@ -192,7 +198,8 @@ Parts cut(Kind kind, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bo
         attempt(true, rounds * round / tiles_n * t->bm / 256 * 256);
     }
     attempt(true, M / 256 * 256);
-    if (is_int4(kind) && M <= 2 * kFewRows) attempt(true, kFewRows);   // two launches for few rows: 96 x 4096 -> 4096 22.7 us, a tile's 27.6
+    // two launches for few rows: 96 x 4096 -> 4096 22.7 us, a tile's 27.6
+    if (is_int4(kind) && M <= 2 * kFewRows) attempt(true, kFewRows);
     return best;
 }
 
@@ -252,7 +259,8 @@ void launch(const P& whole, const Parts& parts, Kind kind, Launch&& go) {
             p.M = static_cast<int32_t>(part.M);
         } else {
             const bool int4 = is_int4(kind);
-            const auto tile = *std::find_if(tiles_begin(int4), tiles_end(int4), [&](const TileCost& t) { return t.kernel == part.plan.kernel; });
+            const auto tile = *std::find_if(tiles_begin(int4), tiles_end(int4),
+                                            [&](const TileCost& t) { return t.kernel == part.plan.kernel; });
             p.m_first = static_cast<int32_t>(part.m0);
             p.n_first = static_cast<int32_t>(gated ? part.n0 / 2 : part.n0);
             p.tiles_m = static_cast<int32_t>(ceil_div(part.M, tile.bm));
@@ -477,8 +485,8 @@ extern "C" int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t
 }
 
 extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const void* b, int64_t ldb, bool b_across,
-                                const void* bias, int type, void* c, int64_t ldc, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
-                                hipStream_t stream) {
+                                const void* bias, int type, void* c, int64_t ldc, int64_t M, int64_t N, int64_t K,
+                                void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     if (!sizes_ok(M, N, K) || !half_type(type) || (a_across && !b_across) || !operand_ok(a, lda, a_across ? M : K) ||
         !operand_ok(b, ldb, b_across ? N : K) || !output_ok(c, ldc, N, type) || (bias && !aligned_to_type(bias, type)))
         return false;
@@ -534,9 +542,11 @@ extern "C" bool feather_int4_linear_direct(const uint8_t* codes, int64_t ld_code
     const int64_t rows = gated ? 2 * N : N;
     if (M <= kFewRows || !sizes_ok(M, rows, K)) return true;
     if (!on_16(codes) || ld_codes % 16 != 0) return false;
-    // Dequantized, codes are read and values written, and read again (us at 4.4 TB/s).
-    const float before = kLaunchCost + static_cast<float>(rows) * static_cast<float>(K) * (2.5f / 4.4e6f);
-    return parts_of(gated ? Kind::kInt4Gated : Kind::kInt4, M, N, K).cost <= before + parts_of(gated ? Kind::kGated : Kind::kPlain, M, N, K).cost;
+    // Dequantized, codes are read and values written (us at 4.4 TB/s). Of 84 shapes, 65 to 4096 rows, this picks the slower way by more
+    // than 4% for four, 10% at most.
+    const float before = 2.0f * kLaunchCost + static_cast<float>(rows) * static_cast<float>(K) * (2.5f / 4.4e6f);
+    const float direct = parts_of(gated ? Kind::kInt4Gated : Kind::kInt4, M, N, K).cost;
+    return direct <= before + parts_of(gated ? Kind::kGated : Kind::kPlain, M, N, K).cost;
 }
 
 extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64_t ld_codes, const void* scale,

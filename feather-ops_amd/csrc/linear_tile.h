@@ -1,6 +1,15 @@
 // The tile kernel of the 16-bit products, c = a b^T with either operand stored along its sum (rows of k) or across it (transposed):
 // a workgroup of 4 waves owns BM x BN outputs, two waves each way, and K streams through LDS in stages of 64 that direct
 // global-to-LDS loads fill.
+//
+// One wave a SIMD, with 256 accumulators and two halves of a stage in registers: of 256 x 256 outputs a stage takes 128 MFMAs, 32
+// fragment reads and 16 loads of each wave, 223 instructions in all, laid between the MFMAs by hand. 4096 x 16384 x 4096 runs 365
+// us, 1.46 PFLOP/s (the library 1.50). The matrix units are busy 79% of the clocks, at 1.94 GHz: power bounds it (operands of zeros:
+// the same clocks at 2.44 GHz, 286 us). Between the loops of two tiles there are 10 us, 6 of them the outputs' way out, most of
+// that memory's: all workgroups store at once.
+//
+// Measured, not taken: 32 x 32 x 16 MFMAs (4096 x 8192 x 4096 187 -> 215 us), outputs straight from the fragments (the same),
+// non-temporal stores (27648 x 5120 x 1024 248 -> 261), starts staggered over 8 us (248 -> 246).
 #pragma once
 
 #include "linear_common.h"

@@ -9,8 +9,8 @@
  * launch errors are left to the caller (hipGetLastError). No function allocates, synchronizes or keeps anything between calls.
  * Results are deterministic. Strides are in elements (of codes: bytes). Operands of products have rows on 16-byte boundaries
  * (strides are multiples of 8, at most 2^21) and, where a comment says padded, rows that can be read up to the next multiple of 8
- * values; outputs may have any alignment. Sizes: 1 <= M, N, K < 2^31 with K at most 2^21, and few enough outputs for a launch to
- * have under 2^32 threads.
+ * values; outputs may have any alignment. Sizes: M < 2^29, N (rows of a weight) < 2^28, K at most 2^21, and few enough outputs for
+ * a launch to have under 2^32 threads.
  *
  * Workspaces: the function's ..._workspace_bytes (0: none), 256-byte aligned. Its first 64 KiB are all zero before its first use
  * and left zero by every call; calls that share one must be ordered.
@@ -59,7 +59,8 @@ int64_t feather_gated_backward_parts(int64_t M, int64_t F);
  *      operand's rows are padded; stored along, they are padded with zeros.
  */
 bool feather_product(const void* a, int64_t lda, bool a_across, const void* b, int64_t ldb, bool b_across, const void* bias,
-                     int type, void* c, int64_t ldc, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+                     int type, void* c, int64_t ldc, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
 int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /*

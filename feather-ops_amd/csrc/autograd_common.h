@@ -3,10 +3,12 @@
 
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/inductor/aoti_torch/c/shim.h>
 #include <torch/library.h>
 
@@ -65,6 +67,48 @@ inline std::optional<Tensor> workspace_of(const c10::IValue& kept) {
     Tensor own = at::empty_like(workspace);
     own.narrow(0, 0, std::min(kCounterBytes, own.numel())).zero_();
     return own;
+}
+
+// Whether a stream is being captured. (The default one cannot be.)
+inline bool is_capturing(const c10::Stream& stream) {
+    if (stream.id() == 0) return false;
+    const c10::impl::VirtualGuardImpl guard(c10::DeviceType::CUDA);
+    const c10::Stream before = guard.exchangeStream(stream);
+    void* handle = nullptr;
+    const bool known = aoti_torch_get_current_cuda_stream(stream.device_index(), &handle) == AOTI_TORCH_SUCCESS;
+    guard.exchangeStream(before);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    return known && hipStreamIsCapturing(static_cast<hipStream_t>(handle), &capture) == hipSuccess &&
+           capture == hipStreamCaptureStatusActive;
+}
+
+// What runs after `node` in this backward, up to `depth` nodes on, on a stream that is neither `current` nor captured itself.
+inline bool leads_astray(const torch::autograd::Node& node, const c10::Stream& current, int depth) {
+    const auto* const runs = torch::autograd::get_current_graph_task_exec_info();
+    for (const torch::autograd::Edge& edge : node.next_edges()) {
+        if (!edge.is_valid()) continue;
+        if (runs && !runs->empty()) {
+            const auto found = runs->find(edge.function.get());
+            if (found == runs->end() || !found->second.should_execute()) continue;
+        }
+        const std::optional<c10::Stream> stream = edge.function->stream();
+        if (stream && *stream != current && !is_capturing(*stream)) return true;
+        if (depth > 1 && leads_astray(*edge.function, current, depth - 1)) return true;
+    }
+    return false;
+}
+
+// A backward that is being captured hands its gradients to the nodes before it on their streams. A leaf's node lives as long as
+// any graph on it, on the stream where that graph began: where that is not being captured, the wait between the two would end
+// the capture, and with it the process. It is refused instead. (Between the operator and a leaf there are the package's own views,
+// casts and copies: three at most.)
+inline void refuse_foreign_streams(const char* name, const Tensor& grad_y) {
+    const auto node = torch::autograd::get_current_node();
+    if (!node || !grad_y.is_cuda() || grad_y.key_set().has(c10::DispatchKey::Python)) return;
+    const c10::Stream current = c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getStream(grad_y.device());
+    TORCH_CHECK(!is_capturing(current) || !leads_astray(*node, current, 4), name,
+                ": its backward is being captured, and an operand belongs to a graph that lives on another stream, such as an "
+                "earlier pass's loss. Release that graph, or run that pass on the capturing stream");
 }
 
 // Makes `grad` depend on what it was computed from, by way of a node that refuses to go on: the gradient that came in and

@@ -61,8 +61,9 @@ __device__ __forceinline__ void spread_rows(uint32_t v, uint32_t (&out)[4]) {
 }
 
 // 8 codes of a column to 16 bits in steps of about an instruction that go between the MFMAs. bf16: q s - z s in fp32, exact,
-// rounded as it is packed; a code's byte, read as a float of 8 bits (e4m3), is q / 512, and two are converted at a time. fp16: codes
-// in the mantissas of 1024 + q and 1024 + 16 q, from where a multiplication and addition takes them to q - z, exactly.
+// rounded as it is packed; a code's byte, read as a float of 8 bits (e4m3), is q / 512, and two at a time are converted and multiplied
+// by 512. fp16: codes in the mantissas of 1024 + q and 1024 + 16 q, from where a multiplication and addition takes them to q - z,
+// exactly.
 template <bool kBf16>
 struct Decoder {
     static constexpr int kSetup = 4;
@@ -91,9 +92,8 @@ struct Decoder {
                 scale = __builtin_bit_cast(float, word << 16);
             } else if constexpr (kStep == 3) {
                 offset *= -scale;
-                scale *= 512.0f;
             } else if constexpr (e < 2) {
-                const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(e == 0 ? even : odd), kTop);
+                const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(e == 0 ? even : odd, 512.0f, kTop);
                 (e == 0 ? lo : hi)[0] = v[0];
                 (e == 0 ? lo : hi)[1] = v[1];
             } else if constexpr (e < 4) {

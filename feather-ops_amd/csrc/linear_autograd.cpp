@@ -86,6 +86,7 @@ struct GatedLinear : public Function<GatedLinear> {
         const bool need_b = bias && ctx->needs_input_grad(2);
         const variable_list saved = ctx->get_saved_variables();
         refuse_tangents("gated_linear", {grads[0]});
+        refuse_foreign_streams("gated_linear", grads[0]);
         const bool twice = at::GradMode::is_enabled();
         const at::NoGradGuard once;
         auto [grad_x, grad_w, grad_b] =
@@ -137,6 +138,7 @@ struct Int4Linear : public Function<Int4Linear> {
         // operands that are not there are not counted
         const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(saved[2].defined() ? 4 : 3);
         refuse_tangents("int4_linear", {grads[0]});
+        refuse_foreign_streams("int4_linear", grads[0]);
         const bool twice = at::GradMode::is_enabled();
         const at::NoGradGuard once;
         Tensor grad_x, grad_b;

@@ -131,6 +131,92 @@ def test_steps_in_a_graph(fo, example):
             assert all(torch.equal(p, q) for p, q in zip(out, want))
 
 
+@pytest.mark.parametrize("k", [2048, 2045])
+@pytest.mark.parametrize("kind", ["gated", "int4"])
+def test_forward_and_backward_in_two_graphs(fo, kind, k):
+    """They share their memory; products are split. Replays with new inputs, eager passes of the same leaves between them. While an
+    eager graph of the leaves lives on another stream, a captured backward is refused."""
+    m, f = 96, 64
+    g = torch.Generator("cuda").manual_seed(2)
+    x = torch.randn((m, k), generator=g, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn((2 * f, k), generator=g, device="cuda") * k**-0.5).bfloat16().requires_grad_()
+    codes = fo.quantize_int4(w.detach(), 32)
+    leaves = (x, w) if kind == "gated" else (x,)
+
+    def forward():
+        return fo.gated_linear(x, w, None, "gelu") if kind == "gated" else fo.int4_linear(x, *codes)
+
+    gy = torch.randn((m, f if kind == "gated" else 2 * f), generator=g, device="cuda").bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(forward(), leaves, gy)
+    torch.cuda.synchronize()
+    alive = forward()
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused, stream=side):
+        y = forward()
+        with pytest.raises(RuntimeError, match="lives on another stream"):
+            torch.autograd.grad(y, leaves, gy)
+    torch.autograd.grad(alive, leaves, gy)
+    del alive, y
+    pool, graphs = torch.cuda.graph_pool_handle(), [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0], pool=pool, stream=side):
+        y = forward()
+    with torch.cuda.graph(graphs[1], pool=pool, stream=side):
+        grads = torch.autograd.grad(y, leaves, gy)
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(x * 0.5)
+        eager = forward()
+        want = (eager.detach(), *torch.autograd.grad(eager, leaves, gy))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip((y.detach(), *grads), want))
+
+
+def test_vectors_batches_and_inference_mode(fo):
+    x, w = torch.randn(2, 3, 72, device="cuda").half(), torch.randn(80, 72, device="cuda").half() * 0.1
+    int4 = fo.quantize_int4(w, 32, zeros=True)
+    for call in (lambda t: fo.gated_linear(t, w), lambda t: fo.int4_linear(t, *int4), lambda t: fo.int4_gated_linear(t, *int4)):
+        rows = call(x.view(6, 72))
+        assert torch.equal(call(x), rows.view(2, 3, -1)) and torch.equal(call(x[1, 2]), call(x[1, 2:])[0])
+        with torch.inference_mode():
+            assert torch.equal(call(x.clone()), rows.view(2, 3, -1))
+        assert not call(x).requires_grad
+    vector = x[0, 0].clone().requires_grad_()
+    for call in (lambda t: fo.gated_linear(t, w), lambda t: fo.int4_linear(t, *int4)):
+        (grad,) = torch.autograd.grad(call(vector).sum(), vector)
+        (want,) = torch.autograd.grad(call(vector[None]).sum(), vector)
+        assert torch.equal(grad, want)
+
+
+def test_calls_on_two_streams_and_threads_at_once(fo):
+    """Split products, whose workspaces are their stream's."""
+    import threading
+
+    x = [torch.randn(64, 4096, device="cuda").bfloat16() for _ in range(4)]
+    w = torch.randn(128, 4096, device="cuda").bfloat16() * 0.02
+    int4 = fo.quantize_int4(w)
+    want = [(fo.gated_linear(t, w), fo.int4_linear(t, *int4)) for t in x]
+    streams, got = [torch.cuda.Stream() for _ in x], [[] for _ in x]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(20):
+                got[i] = [fo.gated_linear(x[i], w), fo.int4_linear(x[i], *int4)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(x))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for mine, yours in zip(got, want) for p, q in zip(mine, yours))
+
+
 def test_command():
     run = subprocess.run([sys.executable, str(PATH), "--tokens", "3", "--width", "256", "--hidden", "384"],
                          capture_output=True, text=True, timeout=100)

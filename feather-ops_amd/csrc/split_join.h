@@ -28,21 +28,45 @@ __device__ __forceinline__ bool join_splits(const P& p, f32x4 (&acc)[RM][RN], in
     before = __builtin_amdgcn_readfirstlane(before);
     asm volatile("" ::: "memory");   // the reads below come after it
     if (before + 1 != static_cast<uint32_t>(p.splits)) return false;
+    constexpr int kFragments = RM * RN;
+    constexpr int kBatch = kFragments % 16 == 0 ? 16 : kFragments;
+    const auto load = [&](f32x4 (&part)[kBatch], int s, int f0) {
+#pragma unroll
+        for (int f = 0; f < kBatch; ++f)
+            part[f] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, place(s) + (f0 + f) * kWave * 16u, 0, kDeviceScope));
+        __builtin_amdgcn_sched_barrier(0);
+    };
     // As many loads in flight as there are registers for. (Left to itself the compiler waits for each: 1000 x 27648 x 5120 in 256 x
-    // 256 tiles and three K ranges took 266 us.)
-    constexpr int kBatch = RM * RN % 16 == 0 ? 16 : RM * RN;
-    for (int s = 0; s < p.splits; ++s) {
+    // 256 tiles and three K ranges took 266 us, with 16 together 257.) Where a SIMD has one wave there is room for two batches: one
+    // is loaded while the other is added.
+    const auto add = [&](const f32x4 (&part)[kBatch], int s, int f0) {
 #pragma unroll
-        for (int f0 = 0; f0 < RM * RN; f0 += kBatch) {
-            f32x4 part[kBatch];
+        for (int f = 0; f < kBatch; ++f) {
+            f32x4& sum = acc[(f0 + f) / RN][(f0 + f) % RN];
+            sum = s == 0 ? part[f] : sum + part[f];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (kFragments == 4 * kBatch) {
+        f32x4 even[kBatch], odd[kBatch];
+        load(even, 0, 0);
+        for (int s = 0; s < p.splits; ++s) {
+            load(odd, s, kBatch);
+            add(even, s, 0);
+            load(even, s, 2 * kBatch);
+            add(odd, s, kBatch);
+            load(odd, s, 3 * kBatch);
+            add(even, s, 2 * kBatch);
+            load(even, s + 1 < p.splits ? s + 1 : s, 0);   // (the last one for nothing)
+            add(odd, s, 3 * kBatch);
+        }
+    } else {
+        for (int s = 0; s < p.splits; ++s) {
 #pragma unroll
-            for (int f = 0; f < kBatch; ++f)
-                part[f] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, place(s) + (f0 + f) * kWave * 16u, 0, kDeviceScope));
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int f = 0; f < kBatch; ++f) {
-                f32x4& sum = acc[(f0 + f) / RN][(f0 + f) % RN];
-                sum = s == 0 ? part[f] : sum + part[f];
+            for (int f0 = 0; f0 < kFragments; f0 += kBatch) {
+                f32x4 part[kBatch];
+                load(part, s, f0);
+                add(part, s, f0);
             }
         }
     }

@@ -74,10 +74,10 @@ int feather_block_scaled_mm_launches(int64_t M, int64_t N, int64_t K, int64_t ou
 bool feather_copy_rows(const void* from, int64_t ld_from, void* to, int64_t ld_to, int64_t rows, int64_t cols, hipStream_t stream);
 
 /*
- * The same of feather_product and feather_gated_linear (gated, N = F) or, with int4, of feather_int4_linear: kernels of
- * linear_launch.h's LinearKernel, columns of a gated block counted twice.
+ * The same of feather_product and feather_gated_linear (gated, N = F) or, with int4, of feather_int4_linear (fine: groups of 32, or
+ * of 64 in bf16, with zero points): kernels of linear_launch.h's LinearKernel, columns of a gated block counted twice.
  */
-int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, bool int4, int64_t out[16]);
+int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, bool int4, bool fine, int64_t out[16]);
 
 }  // extern "C"
 

@@ -27,10 +27,12 @@ void plain(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
 template <int kGroups, bool kZeros>
 void gated(const Int4Params& p, const LinearPlan& plan, hipStream_t stream) {
     constexpr Form kForm = Form::kGated;
+    if constexpr (!kZeros || kGroups == 1 || (kGroups == 2 && !kBf16)) {   // others have no plan of 16 waves
+        if (plan.kernel == kFew16_2_16_1) return few<FewRows<1, 2, 16, 1>, kGroups, kZeros, kForm>(p, plan, stream);
+        if (plan.kernel == kFew32_2_4_4) return few<FewRows<2, 2, 4, 4>, kGroups, kZeros, kForm>(p, plan, stream);
+    }
     if (plan.kernel == kFew16_2_4_2) few<FewRows<1, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
     else if (plan.kernel == kFew16_2_8_1) few<FewRows<1, 2, 8, 1>, kGroups, kZeros, kForm>(p, plan, stream);
-    else if (plan.kernel == kFew16_2_16_1) few<FewRows<1, 2, 16, 1>, kGroups, kZeros, kForm>(p, plan, stream);
-    else if (plan.kernel == kFew32_2_4_4) few<FewRows<2, 2, 4, 4>, kGroups, kZeros, kForm>(p, plan, stream);
     else if (plan.kernel == kFew32_2_4_2) few<FewRows<2, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
     else few<FewRows<4, 2, 4, 2>, kGroups, kZeros, kForm>(p, plan, stream);
 }

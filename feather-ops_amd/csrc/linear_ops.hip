@@ -49,9 +49,17 @@ constexpr TileCost kInt4Tiles[] = {
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8};
 constexpr float kLaunchCost = 2.0f;   // us from the end of one launch to the next one's work
 
-enum class Kind { kPlain, kGated, kInt4, kInt4Gated };
+enum class Kind { kPlain, kGated, kInt4, kInt4Gated, kInt4GatedFine };
 
-constexpr bool is_int4(Kind kind) { return kind == Kind::kInt4 || kind == Kind::kInt4Gated; }
+constexpr bool is_int4(Kind kind) { return kind >= Kind::kInt4; }
+constexpr bool is_gated(Kind kind) { return kind != Kind::kPlain && kind != Kind::kInt4; }
+
+Kind int4_kind(bool gated, bool fine) { return !gated ? Kind::kInt4 : fine ? Kind::kInt4GatedFine : Kind::kInt4Gated; }
+
+// Scales and zero points of many groups take registers that a gated kernel of 16 waves has not got: 24 rows of 5120 -> 13824 in
+// groups of 32 with zero points 88 us by 2_4_4 and 54 by 2_4_2, of 64 in bf16 50 and 43 (fp16 34 and 40); 1 row of 16384 -> 2048,
+// groups of 32, 2_16_1 49, 2_8_1 33.
+bool is_fine(int group, bool zeros, int type) { return zeros && (group == 32 || (group == 64 && type == FEATHER_BF16)); }
 
 const TileCost* tiles_begin(bool int4) { return int4 ? std::begin(kInt4Tiles) : std::begin(kTiles); }
 const TileCost* tiles_end(bool int4) { return int4 ? std::end(kInt4Tiles) : std::end(kTiles); }
@@ -105,16 +113,16 @@ LinearPlan few_plan(LinearKernel kernel, int rm, int rn, int wk, int wn, int64_t
 //   8192 2_8_1 19.1, 2_4_2 20.4; 2048 x 16384 2_16_1 15.7, 2_8_1 19.8.
 //   24 rows: 13824 x 5120 1_4_4 17.9, 2_4_4/2 19.3, 2_4_2 19.4; 5120 x 13824 1_4_4/2 22.2, /4 25.4, 1_8_2 26.1. Gated: 13824 x 5120
 //   2_4_4 31.3, 4_4_2 31.9, 2_4_2 37.2; 4096 x 4096 2_4_2/2 11.4, 2_4_4/2 15.1.
-LinearPlan int4_plan(int64_t M, int64_t N, int64_t K, bool gated) {
+LinearPlan int4_plan(int64_t M, int64_t N, int64_t K, bool gated, bool fine) {
     if (M > 32) return few_plan(kFew64_2_4_2, 4, 2, 4, 2, N, K, gated, 8);
     if (M > 16) {
         if (!gated) return few_plan(kFew32_1_4_4, 2, 1, 4, 4, N, K, gated, 8);
-        if (N > 64 * 160) return few_plan(kFew32_2_4_4, 2, 2, 4, 4, N, K, gated, 8);
+        if (N > 64 * 160 && !fine) return few_plan(kFew32_2_4_4, 2, 2, 4, 4, N, K, gated, 8);
         return few_plan(kFew32_2_4_2, 2, 2, 4, 2, N, K, gated, 8);
     }
     if (gated) {
         if (N > 8192) return few_plan(kFew16_2_4_2, 1, 2, 4, 2, N, K, gated, 16);
-        if (N > 2048 || K <= 8192) return few_plan(kFew16_2_8_1, 1, 2, 8, 1, N, K, gated, 32);
+        if (N > 2048 || K <= 8192 || fine) return few_plan(kFew16_2_8_1, 1, 2, 8, 1, N, K, gated, 32);
         return few_plan(kFew16_2_16_1, 1, 2, 16, 1, N, K, gated, 64);
     }
     if (N > 8192) return few_plan(kFew16_2_8_1, 1, 2, 8, 1, N, K, gated, 32);
@@ -155,8 +163,9 @@ constexpr FewCost kGatedFew[] = {{16, 5.3f, 0.0011f, 2.4e6f}, {32, 9.5f, 0.00075
 // One launch for a part. Few rows of a gated block or of 4-bit weights, all of the columns, go to a kernel of their own.
 LinearPlan whole_plan(Kind kind, int64_t M, int64_t N, int64_t K, bool all_columns) {
     if (kind == Kind::kPlain || !all_columns || M > kFewRows) return tile_plan(M, N, K, is_int4(kind));
-    const bool gated = kind != Kind::kInt4;
-    LinearPlan plan = is_int4(kind) ? int4_plan(M, gated ? N / 2 : N, K, gated) : gated_few_plan(M, N / 2, K);
+    const bool gated = is_gated(kind);
+    LinearPlan plan = is_int4(kind) ? int4_plan(M, gated ? N / 2 : N, K, gated, kind == Kind::kInt4GatedFine)
+                                    : gated_few_plan(M, N / 2, K);
     const FewCost* cost = is_int4(kind) ? kInt4Few : kGatedFew;
     while (M > cost->rows) ++cost;
     const float weights = static_cast<float>(N) * static_cast<float>(K);
@@ -217,8 +226,7 @@ const Parts& parts_of(Kind kind, int64_t M, int64_t N, int64_t K) {
                       static_cast<uint64_t>(K) * 0x165667b19e3779f9u + (static_cast<uint64_t>(kind) << 36);
     Entry& e = table[(hash >> 32) % kEntries];
     if (e.M != M || e.N != N || e.K != K || e.kind != kind || e.parts.count == 0) {
-        const bool gated = kind == Kind::kGated || kind == Kind::kInt4Gated;
-        e = Entry{kind, M, N, K, cut(kind, 0, 0, M, gated ? 2 * ceil_div(N, 16) * 16 : N, K, true, 2)};
+        e = Entry{kind, M, N, K, cut(kind, 0, 0, M, is_gated(kind) ? 2 * ceil_div(N, 16) * 16 : N, K, true, 2)};
     }
     return e.parts;
 }
@@ -247,7 +255,7 @@ bool launchable(const Parts& parts) {
 // The launches of a product, one after the other.
 template <typename P, typename Launch>
 void launch(const P& whole, const Parts& parts, Kind kind, Launch&& go) {
-    const bool gated = kind == Kind::kGated || kind == Kind::kInt4Gated;
+    const bool gated = is_gated(kind);
     for (int i = 0; i < parts.count; ++i) {
         const Part& part = parts.part[i];
         P p = whole;
@@ -509,9 +517,9 @@ extern "C" bool feather_product(const void* a, int64_t lda, bool a_across, const
     return true;
 }
 
-extern "C" int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, bool int4, int64_t out[16]) {
+extern "C" int feather_linear_launches(int64_t M, int64_t N, int64_t K, bool gated, bool int4, bool fine, int64_t out[16]) {
     if (!sizes_ok(M, gated ? 2 * N : N, K)) return 0;
-    const Parts& parts = parts_of(int4 ? (gated ? Kind::kInt4Gated : Kind::kInt4) : gated ? Kind::kGated : Kind::kPlain, M, N, K);
+    const Parts& parts = parts_of(int4 ? int4_kind(gated, fine) : gated ? Kind::kGated : Kind::kPlain, M, N, K);
     for (int i = 0; i < parts.count; ++i) {
         const Part& part = parts.part[i];
         const int64_t launch[4] = {part.plan.kernel, part.plan.splits, part.M, part.N};
@@ -535,7 +543,9 @@ bool int4_ok(const uint8_t* codes, int64_t ld_codes, const void* scale, int64_t 
 }  // namespace
 
 extern "C" int64_t feather_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated) {
-    return sizes_ok(M, gated ? 2 * N : N, K) ? workspace_of(parts_of(gated ? Kind::kInt4Gated : Kind::kInt4, M, N, K)) : -1;
+    if (!sizes_ok(M, gated ? 2 * N : N, K)) return -1;
+    const int64_t need = workspace_of(parts_of(int4_kind(gated, false), M, N, K));
+    return std::max(need, workspace_of(parts_of(int4_kind(gated, true), M, N, K)));
 }
 
 extern "C" bool feather_int4_linear_direct(const uint8_t* codes, int64_t ld_codes, int64_t M, int64_t N, int64_t K, bool gated) {
@@ -545,7 +555,7 @@ extern "C" bool feather_int4_linear_direct(const uint8_t* codes, int64_t ld_code
     // Dequantized, codes are read and values written (us at 4.4 TB/s). Of 84 shapes, 65 to 4096 rows, this picks the slower way by more
     // than 4% for four, 10% at most.
     const float before = 2.0f * kLaunchCost + static_cast<float>(rows) * static_cast<float>(K) * (2.5f / 4.4e6f);
-    const float direct = parts_of(gated ? Kind::kInt4Gated : Kind::kInt4, M, N, K).cost;
+    const float direct = parts_of(int4_kind(gated, false), M, N, K).cost;
     return direct <= before + parts_of(gated ? Kind::kGated : Kind::kPlain, M, N, K).cost;
 }
 
@@ -559,7 +569,7 @@ extern "C" bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* c
         !int4_ok(codes, ld_codes, scale, ld_scale, zero, ld_zero, group, type, rows, K) ||
         (M > kFewRows && (!on_16(codes) || ld_codes % 16 != 0)))
         return false;
-    const Kind kind = gated ? Kind::kInt4Gated : Kind::kInt4;
+    const Kind kind = int4_kind(gated, is_fine(group, zero != nullptr, type));
     const Parts& parts = parts_of(kind, M, N, K);
     const int64_t need = workspace_of(parts);
     if (!launchable(parts) || !workspace_ok(workspace, workspace_bytes, need)) return false;

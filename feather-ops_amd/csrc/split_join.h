@@ -32,8 +32,10 @@ __device__ __forceinline__ bool join_splits(const P& p, f32x4 (&acc)[RM][RN], in
     constexpr int kBatch = kFragments % 16 == 0 ? 16 : kFragments;
     const auto load = [&](f32x4 (&part)[kBatch], int s, int f0) {
 #pragma unroll
-        for (int f = 0; f < kBatch; ++f)
-            part[f] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, place(s) + (f0 + f) * kWave * 16u, 0, kDeviceScope));
+        for (int f = 0; f < kBatch; ++f) {
+            const uint32_t at = place(s) + (f0 + f) * kWave * 16u;
+            part[f] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(parts, at, 0, kDeviceScope));
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
     // As many loads in flight as there are registers for. (Left to itself the compiler waits for each: 1000 x 27648 x 5120 in 256 x

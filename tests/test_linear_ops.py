@@ -52,11 +52,11 @@ def lib():
 def launches(lib):
     call = lib.feather_linear_launches
     call.restype = INT
-    call.argtypes = [I64] * 3 + [BOOL] * 2 + [ctypes.POINTER(I64)]
+    call.argtypes = [I64] * 3 + [BOOL] * 3 + [ctypes.POINTER(I64)]
 
-    def of(m, n, k, gated=False, int4=False):
+    def of(m, n, k, gated=False, int4=False, fine=False):
         out = (I64 * 16)()
-        return [tuple(out[4 * i:4 * i + 4]) for i in range(call(m, n, k, gated, int4, out))]
+        return [tuple(out[4 * i:4 * i + 4]) for i in range(call(m, n, k, gated, int4, fine, out))]
 
     return of
 
@@ -91,6 +91,17 @@ def test_shapes_go_to_their_kernels(launches, kind):
 def test_every_kernel_is_reached():
     reached = {launch for listed in (PRODUCT, GATED, INT4, INT4_GATED) for shape in listed.values() for launch in shape}
     assert reached == {(kernel, split) for kernel in KERNELS for split in (False, True)} - {(kernel, True) for kernel in NEVER_SPLIT}
+
+
+def test_fine_groups_with_zero_points_take_fewer_waves(launches, lib):
+    """Their workspace is asked for without knowing the groups: it is enough for both."""
+    for shape in INT4_GATED:
+        coarse, fine = launches(*shape, True, True), launches(*shape, True, True, True)
+        for (kernel, _, *size), (other, splits, *same) in zip(coarse, fine):
+            assert KERNELS[other] not in ("few 16 2/16/1", "few 32 2/4/4") and size == same
+            assert kernel == other or KERNELS[kernel] in ("few 16 2/16/1", "few 32 2/4/4")
+            assert splits == 1 or lib.feather_int4_linear_workspace_bytes(*shape, True) > 0
+        assert launches(*shape, False, True) == launches(*shape, False, True, True)
 
 
 def test_which_codes_are_dequantized(lib):

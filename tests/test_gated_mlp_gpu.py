@@ -286,3 +286,27 @@ def test_codes_past_4_gib(fo, m):
     value, slope = ref.activation(gate, "silu")
     off = (slope.abs() + 2 * d_gate) * d_gate * up.abs() + value.abs() * d_up + d_gate * d_up + ref.ACT * (value * up).abs()
     ref.check(half[:, [0, n // 2 - 1]], value * up, off)
+
+
+@pytest.mark.parametrize("m", [1, 24, 50, 80])
+def test_weights_past_4_gib(fo, m):
+    """Read along their rows by the kernels for few rows and by tiles, and across them by dx."""
+    k, f, chunks = 16384, 70000, 4
+    g = torch.Generator("cuda").manual_seed(0)
+    w = torch.empty((2 * f, k), dtype=torch.bfloat16, device="cuda")
+    for part in w.chunk(8):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda") * k**-0.5)
+    assert w.numel() * 2 > 1 << 32
+    x = torch.randn((m, k), generator=g, device="cuda").bfloat16().requires_grad_()
+    y = fo.gated_linear(x, w)
+    cols = torch.tensor([0, 1, f // 2, f - 33, f - 1], device="cuda")
+    ref.check(y[:, cols], *ref.gated(x.detach(), torch.cat((w[cols], w[f + cols])), None, "silu"))
+    if m < 80:
+        return
+    gy = torch.randn((m, f), generator=g, device="cuda").bfloat16()
+    (gx,) = torch.autograd.grad(y, x, gy)
+    want, bound = 0, 0
+    for at in torch.arange(f, device="cuda").chunk(chunks):   # in parts, for the 64-bit weight's sake
+        part = ref.gated_gradients(x.detach(), torch.cat((w[at], w[f + at])), None, "silu", gy[:, at])[0]
+        want, bound = want + part[0], bound + part[1]
+    ref.check(gx, want, chunks * bound)   # a sum over all of them is off by at most as many times its parts' bounds

@@ -45,13 +45,13 @@ __device__ __forceinline__ void store4(const LinearParams& p, int m, int n, f32x
     }
 }
 
-// A row's sums to outputs: gate and up of columns n .. n + 3, or (plain) the sums themselves.
+// A row's sums, in units of `unit`, to outputs: gate and up of columns n .. n + 3, or (plain) the sums themselves.
 template <Form kForm, bool kBf16>
-__device__ __forceinline__ void store_sums(const LinearParams& p, int m, int n, f32x4 sum, f32x4 up) {
+__device__ __forceinline__ void store_sums(const LinearParams& p, int m, int n, f32x4 sum, f32x4 up, float unit) {
     if (m >= p.M || n >= p.N) return;
-    sum += bias4<kBf16>(p.bias, n, p.N);
+    sum = sum * unit + bias4<kBf16>(p.bias, n, p.N);
     if constexpr (kForm != Form::kPlain) {
-        up += bias4<kBf16>(p.bias, int64_t{p.N} + n, int64_t{2} * p.N);
+        up = up * unit + bias4<kBf16>(p.bias, int64_t{p.N} + n, int64_t{2} * p.N);
         if constexpr (kForm == Form::kGatedKeep) {
             float* const row = p.h + static_cast<int64_t>(m) * p.ldh + n;   // both halves padded to 8 columns
             store_any(row, sum);
@@ -64,10 +64,15 @@ __device__ __forceinline__ void store_sums(const LinearParams& p, int m, int n, 
     store4<kBf16>(p, m, n, sum);
 }
 
+// Waves of a SIMD that a kernel's registers have to leave room for. (Left alone, those of two groups with zero points take 130: one
+// row of 5120 -> 13824 in bf16 19.8 us, with 5 of them spilled 18.1.)
+template <typename T, int kGroups, bool kZeros>
+constexpr int kFewWaves = T::RM == 1 && T::kThreads == 512 && kZeros && kGroups == 2 ? 4 : T::kThreads / 256;
+
 // kGroups: a step's groups of 4-bit codes (4, 2 or 1 of 32, 64 or 128), or 0: 16-bit weights. kZeros: the codes have zero points
 // of their own.
 template <typename T, int kGroups, bool kZeros, Form kForm, bool kBf16>
-__global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::conditional_t<kGroups != 0, Int4Params, LinearParams> p) {
+__global__ __launch_bounds__(T::kThreads, (kFewWaves<T, kGroups, kZeros>)) void few_rows_kernel(const std::conditional_t<kGroups != 0, Int4Params, LinearParams> p) {
     constexpr bool kInt4 = kGroups != 0;
     constexpr int RM = T::RM, RN = T::RN, WK = T::WK, WN = T::WN;
     constexpr bool kGated = kForm != Form::kPlain;
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::condit
             const int s = kRun ? at % 4 : at / 4 % 4;
             const int c = kRun ? at / 4 % 4 : at % 4;
             u32x4 v = piece[i];
-            if constexpr (kInt4) v = __builtin_bit_cast(u32x4, order8(v));
+            if constexpr (kInt4) v = __builtin_bit_cast(u32x4, order8<kBf16>(v));
             if (row < p.M) *reinterpret_cast<u32x4*>(to + at / 16 * T::kStepBytes + (s * T::kRows + row) * 64 + c * 16) = v;
         }
     };
@@ -141,9 +146,7 @@ __global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::condit
                               make_rsrc(weight + (kGated ? p.N + static_cast<int64_t>(n0) : n0) * pitch, records)};
     const uint32_t w_off = static_cast<uint32_t>(r16) * static_cast<uint32_t>(pitch) + 16u * g;
 
-    // 4-bit: scales (and bf16's zero points) of the 4 columns of each fragment that the lane's sums belong to; fp16's zero points of
-    // the row whose codes it holds.
-    constexpr bool kRowZeros = kZeros && !kBf16;
+    // 4-bit: scales of the 4 columns of each fragment that the lane's sums belong to; zero points of the row whose codes it holds.
     [[maybe_unused]] ScaleAt at[RN];
     [[maybe_unused]] uint32_t zero_at[RN];
     [[maybe_unused]] int groups = 1;
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::condit
             const int total = up ? 2 * p.N : p.N;
             const int n = (up ? p.N : 0) + n0 + row_of(j);
             at[j] = scale_at(n + 4 * g, total);
-            zero_at[j] = kRowZeros ? static_cast<uint32_t>(n + r16 < total ? n + r16 : total - 1) : at[j].from;
+            if constexpr (kZeros) zero_at[j] = static_cast<uint32_t>(n + r16 < total ? n + r16 : total - 1);
         }
         groups = (p.K + p.group - 1) / p.group;
     }
@@ -191,8 +194,7 @@ __global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::condit
 #pragma unroll
                 for (int j = 0; j < RN; ++j) {
                     f.scale[j][c] = load_any<u32x2>(p.scale + group * p.ld_scale + at[j].from);
-                    if constexpr (kRowZeros) f.zero[j][c] = (p.zero + group * p.ld_zero)[zero_at[j]];
-                    else if constexpr (kZeros) f.zero[j][c] = load_any<uint32_t>(p.zero + group * p.ld_zero + zero_at[j]);
+                    if constexpr (kZeros) f.zero[j][c] = (p.zero + group * p.ld_zero)[zero_at[j]];
                 }
             }
         }
@@ -216,45 +218,28 @@ __global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::condit
 #pragma unroll
             for (int c = 0; c < kGroups; ++c) {
                 half8 x[RM][kPer];
-                f32x4 sums[RM];   // bf16: -136 times the sum of x, where the codes' sums start, or (zero points) that sum
 #pragma unroll
-                for (int i = 0; i < RM; ++i) {
-                    sums[i] = none;
+                for (int i = 0; i < RM; ++i)
 #pragma unroll
-                    for (int s = 0; s < kPer; ++s) {
-                        x[i][s] = __builtin_bit_cast(half8, read_rows(turn, c * kPer + s, i));
-                        if constexpr (kBf16) sums[i] = mfma16<true>(constant8<!kZeros>(), x[i][s], sums[i]);
-                    }
-                }
+                    for (int s = 0; s < kPer; ++s) x[i][s] = __builtin_bit_cast(half8, read_rows(turn, c * kPer + s, i));
                 f32x4 t[RM][RN];
 #pragma unroll
                 for (int j = 0; j < RN; ++j) {
-                    if constexpr (kRowZeros) decode.set_zero(f.zero[j][c]);
+                    if constexpr (kZeros) decode.set_zero(f.zero[j][c]);
 #pragma unroll
                     for (int s = 0; s < kPer; ++s) {
-                        const half8 code = decode(w[j][c * kPer + s]);
+                        const half8 code = decode.template values<kZeros>(w[j][c * kPer + s]);
 #pragma unroll
-                        for (int i = 0; i < RM; ++i)
-                            t[i][j] = mfma16<kBf16>(code, x[i][s], s > 0 ? t[i][j] : kBf16 && !kZeros ? sums[i] : none);
+                        for (int i = 0; i < RM; ++i) t[i][j] = mfma16<kBf16>(code, x[i][s], s > 0 ? t[i][j] : none);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < RN; ++j) {
                     const f32x4 scale = scales4<kBf16>(f.scale[j][c], at[j].shift);
-                    f32x4 off = none;
-                    if constexpr (kZeros && kBf16) {
-                        off = zeros4(f.zero[j][c], at[j].shift);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) off[e] = -128.0f - off[e];
-                    }
 #pragma unroll
                     for (int i = 0; i < RM; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float v = t[i][j][e];
-                            if constexpr (kZeros && kBf16) v = __builtin_fmaf(off[e], sums[i][e], v);
-                            acc[i][j][e] = __builtin_fmaf(v, scale[e], acc[i][j][e]);
-                        }
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[i][j][e], scale[e], acc[i][j][e]);
                 }
             }
         } else {
@@ -313,7 +298,7 @@ __global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::condit
         }
         if (p.splits > 1 && !join_splits<kUnits * WN>(p, sum, static_cast<int>(blockIdx.x), split, unit, lane)) continue;
         store_sums<kForm, kBf16>(p, f0 / RN * 16 + r16, static_cast<int>(blockIdx.x) * (kWaveCols * WN) + wn * kWaveCols + row_of(f0 % RN) + 4 * g,
-                                 sum[0][0], sum[0][kPair - 1]);
+                                 sum[0][0], sum[0][kPair - 1], kInt4 ? Decode<kBf16>::kUnit : 1.0f);
     }
 }
 

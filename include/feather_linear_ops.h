@@ -75,8 +75,7 @@ int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
 /*
  * y = x W^T + bias (gated false), or act(x Wg^T + bg) * (x Wu^T + bu) with W's first N rows the gates' and N more the ups'
  * (gated true: W, scale, zero and bias have 2 N rows), rounded once. x [M, K], padded to K % 8 == 0 with zeros. Up to 64 rows
- * codes are taken as they are, each group's sum times its scale in fp32 (in bf16 of codes + 128: NaN from values of x above 1e34). For
- * more rows a weight is rounded to `type` first, 15
+ * codes are taken as they are, each group's sum times its scale in fp32. For more rows a weight is rounded to `type` first, 15
  * times a scale is within the type's range, and the codes' rows start on 16-byte boundaries.
  */
 bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64_t ld_codes, const void* scale,

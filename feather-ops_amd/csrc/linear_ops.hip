@@ -180,6 +180,8 @@ Parts cut(Kind kind, int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, bo
     const LinearPlan whole = whole_plan(kind, M, N, K, all_columns);
     Parts best{{{m0, n0, M, N, whole}}, 1, whole.cost};
     if (depth == 0 || whole.cost < 20.0f) return best;
+    // Columns of 4-bit weights would go to tiles, which round them and want codes on 16-byte boundaries: not for few rows.
+    if (is_int4(kind) && all_columns && M <= kFewRows) return best;
     const auto attempt = [&](bool rows, int64_t at) {
         const int64_t total = rows ? M : N;
         if (at <= 0 || at >= total) return;

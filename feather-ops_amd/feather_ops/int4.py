@@ -134,7 +134,8 @@ def int4_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero:
                 bias: torch.Tensor | None = None) -> torch.Tensor:
     """`x @ W^T + bias` with a 4-bit weight W `[N, K]`: x `[..., K]`, the result `[..., N]`, both bfloat16 or float16; bias `[N]`.
 
-    Up to 64 rows take the codes as they are, each group's sum times its scale in fp32; more take W rounded to x's dtype. The
+    Up to 64 rows take the codes as they are, each group's sum times its scale in fp32. Of more rows most take W rounded to x's dtype
+    (15 times a scale has to be within its range), and some, such as a batch's last ones, the codes: by the sizes alone. The
     result is rounded once. Differentiable once, in reverse mode, in x and bias (the weight is frozen): dx = dy @ W with W rounded
     to x's dtype. Scales in another dtype than x's, scales and zero points that are not stored group by group, codes whose rows do
     not start on 4-byte boundaries, and rows of x off 16-byte boundaries or of no multiple of 8 values are copied on every call.

@@ -75,8 +75,9 @@ int64_t feather_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
 /*
  * y = x W^T + bias (gated false), or act(x Wg^T + bg) * (x Wu^T + bu) with W's first N rows the gates' and N more the ups'
  * (gated true: W, scale, zero and bias have 2 N rows), rounded once. x [M, K], padded to K % 8 == 0 with zeros. Up to 64 rows
- * codes are taken as they are, each group's sum times its scale in fp32. For more rows a weight is rounded to `type` first, 15
- * times a scale is within the type's range, and the codes' rows start on 16-byte boundaries.
+ * codes are taken as they are, each group's sum times its scale in fp32. Of more rows each is computed so or, most of them, with the
+ * weight rounded to `type` first; which ones depends on the sizes alone. For more than 64 rows 15 times a scale is within the type's
+ * range, and the codes' rows start on 16-byte boundaries.
  */
 bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64_t ld_codes, const void* scale,
                          int64_t ld_scale, const uint8_t* zero, int64_t ld_zero, int group, const void* bias, int type, bool gated,
@@ -85,7 +86,7 @@ bool feather_int4_linear(const void* x, int64_t ldx, const uint8_t* codes, int64
 int64_t feather_int4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated);
 
 /* Whether feather_int4_linear takes M rows of these codes and is at least as fast as feather_int4_dequantize and a product in 16
- * bits, whose results are the same but for the order of their sums. True up to 64 rows. */
+ * bits, where every row has the rounded weight. True up to 64 rows. */
 bool feather_int4_linear_direct(const uint8_t* codes, int64_t ld_codes, int64_t M, int64_t N, int64_t K, bool gated);
 
 /* w [N, K] of `type` from 4-bit weights, each value rounded once; ldw a multiple of 8, columns from K to the next multiple of 8

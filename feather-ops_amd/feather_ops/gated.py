@@ -117,7 +117,7 @@ def _gated_linear_auto_backward(grad: torch.Tensor, x: torch.Tensor, weight: tor
     grad_x, grad_weight, grad_bias = ops.gated_backward.default(as_rows(grad), kept, rows, padded, act, need_x, need_weight,
                                                                 need_bias, workspace)
     if need_x:
-        grad_x = grad_x[:, :k].reshape(x.shape)
+        grad_x = grad_x[:, :k].contiguous().reshape(x.shape)
     if need_weight:
         grad_weight = grad_weight[:, :k].contiguous()
     return grad_x, grad_weight, grad_bias

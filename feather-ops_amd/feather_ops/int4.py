@@ -262,7 +262,7 @@ def _linear_auto_context(ctx, inputs, output) -> None:
 def _linear_auto_backward(ctx, grad: torch.Tensor) -> tuple:
     need_x, _, _, _, need_bias = ctx.needs_input_grad
     dx = _int4_linear_auto_backward(grad, *ctx.saved_tensors, ctx.k) if need_x else None
-    return dx, None, None, None, grad.float().sum(tuple(range(grad.dim() - 1))).to(grad.dtype) if need_bias else None
+    return dx, None, None, None, grad.reshape(-1, grad.shape[-1]).float().sum(0).to(grad.dtype) if need_bias else None
 
 
 _int4_linear_auto.register_autograd(_linear_auto_backward, setup_context=_linear_auto_context)

@@ -45,13 +45,23 @@ def operand(x: torch.Tensor) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(M: int, F: int, K: int, trains: bool) -> int:
-    """For the block, and for the products of its gradients."""
+def _workspace_bytes(M: int, F: int, K: int, need_x: bool, need_weight: bool) -> int:
+    """For the block, and for the products of the gradients that are needed."""
     lib = _lib.c_library()
-    need = lib.feather_gated_linear_workspace_bytes(M, F, K)
-    if trains:
-        need = max(need, lib.feather_product_workspace_bytes(M, K, 2 * F), lib.feather_product_workspace_bytes(2 * F, K, M))
-    return max(0, need)
+    need = [lib.feather_gated_linear_workspace_bytes(M, F, K)]
+    if need_x:
+        need.append(lib.feather_product_workspace_bytes(M, K, 2 * F))
+    if need_weight:
+        need.append(lib.feather_product_workspace_bytes(2 * F, K, M))
+    if min(need) < 0:
+        raise ValueError(f"sizes are out of range: x [{M}, {K}], weight [{2 * F}, {K}]")
+    return max(need)
+
+
+def check_depth(of: str, depth: int, what: str) -> None:
+    """A gradient's sum is no longer than a product's."""
+    if depth > _FAR:
+        raise ValueError(f"the gradient of {of} is a sum over {what}, at most {_FAR} of them, got {depth}")
 
 
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -62,7 +72,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
 
     Differentiable once, in reverse mode, in x, weight and bias; for that both sums are kept in fp32 (8 F bytes a row), and their
     gradients rounded to x's dtype. Rows of x and weight that do not start on 16-byte boundaries, or whose length is no multiple
-    of 8, are copied on every call. K is at most 2**21."""
+    of 8, are copied on every call. K is at most 2**21, and so are 2 F where x takes a gradient and x's rows where the weight does."""
     act = activation_number(activation)
     if x.dtype not in HALVES or weight.dtype != x.dtype:
         raise ValueError(f"x and weight must both be bfloat16 or both float16, got {x.dtype} and {weight.dtype}")
@@ -75,15 +85,21 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if x.numel() == 0 or weight.numel() == 0:
         gate, up = nn.functional.linear(x, weight, bias).chunk(2, -1)
         return activate(gate, act) * up
+    if torch.is_grad_enabled():
+        if x.requires_grad:
+            check_depth("x", weight.shape[0], "the weight's rows")
+        if weight.requires_grad:
+            check_depth("the weight", x.numel() // x.shape[-1], "the rows of x")
     if torch.compiler.is_compiling():
         return _gated_linear_auto(x, weight, bias, act)
     return _gated(x, weight, bias, act)
 
 
 def _gated(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, act: int) -> torch.Tensor:
-    trains = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    records = torch.is_grad_enabled()
     rows, weight = operand(as_rows(x)), operand(as_rows(weight))
-    need = _workspace_bytes(int(rows.shape[0]), int(weight.shape[0]) // 2, int(rows.shape[1]), trains)
+    need = _workspace_bytes(int(rows.shape[0]), int(weight.shape[0]) // 2, int(rows.shape[1]), records and rows.requires_grad,
+                            records and weight.requires_grad)
     y = torch.ops.feather_ops.gated_linear.default(rows, weight, bias, act, _workspace(rows, need) if need else None)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
@@ -111,7 +127,7 @@ def _gated_linear_auto_backward(grad: torch.Tensor, x: torch.Tensor, weight: tor
     ops = torch.ops.feather_ops
     k = x.shape[-1]
     rows, padded = operand(as_rows(x)), operand(as_rows(weight))
-    need = _workspace_bytes(rows.shape[0], weight.shape[0] // 2, rows.shape[1], True)
+    need = _workspace_bytes(rows.shape[0], weight.shape[0] // 2, rows.shape[1], need_x, need_weight)
     workspace = _workspace(rows, need) if need else None
     kept = ops.gated_forward.default(rows, padded, bias, act, True, workspace)[1]
     grad_x, grad_weight, grad_bias = ops.gated_backward.default(as_rows(grad), kept, rows, padded, act, need_x, need_weight,

@@ -19,7 +19,7 @@ from torch import nn
 from . import _lib
 from .block_scaled import _plain, _workspace, as_rows
 from .gate import silu_mul
-from .gated import HALVES, _workspace_bytes as _gated_workspace_bytes, activate, activation_number, operand
+from .gated import HALVES, _workspace_bytes as _gated_workspace_bytes, activate, activation_number, check_depth, operand
 from .modules import relabel_modules
 
 GROUPS = (32, 64, 128)
@@ -111,10 +111,14 @@ def dequantize_int4(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor
 def _workspace_bytes(M: int, rows: int, K: int, gated: bool, trains: bool) -> int:
     lib = _lib.c_library()
     n, k8 = rows // 2 if gated else rows, -(-K // 8) * 8
-    need = lib.feather_int4_linear_workspace_bytes(M, n, K, gated)
+    need = [lib.feather_int4_linear_workspace_bytes(M, n, K, gated)]
     if M > 64:   # some go through the product in 16 bits, by their sizes and the codes' alignment
-        need = max(need, _gated_workspace_bytes(M, n, k8, False) if gated else lib.feather_product_workspace_bytes(M, n, k8))
-    return max(0, need, lib.feather_product_workspace_bytes(M, K, rows) if trains else 0)
+        need.append(_gated_workspace_bytes(M, n, k8, False, False) if gated else lib.feather_product_workspace_bytes(M, n, k8))
+    if trains:
+        need.append(lib.feather_product_workspace_bytes(M, K, rows))
+    if min(need) < 0:
+        raise ValueError(f"sizes are out of range: x [{M}, {K}], weight [{rows}, {K}]")
+    return max(need)
 
 
 def _prepared(x: torch.Tensor, codes: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor | None:
@@ -139,12 +143,14 @@ def int4_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero:
     result is rounded once. Differentiable once, in reverse mode, in x and bias (the weight is frozen): dx = dy @ W with W rounded
     to x's dtype. Scales in another dtype than x's, scales and zero points that are not stored group by group, codes whose rows do
     not start on 4-byte boundaries, and rows of x off 16-byte boundaries or of no multiple of 8 values are copied on every call.
-    K is at most 2**21."""
+    K is at most 2**21, and so is N where x takes a gradient."""
     bias = _prepared(x, codes, bias)
     k = x.shape[-1]
     _check(codes, scale, zero, k)
     if x.numel() == 0 or codes.numel() == 0:
         return nn.functional.linear(x, x.new_zeros((codes.shape[0], k)), bias)
+    if torch.is_grad_enabled() and x.requires_grad:
+        check_depth("x", codes.shape[0], "the weight's rows")
     if torch.compiler.is_compiling():
         return _int4_linear_auto(x, codes, scale, zero, bias)
     return _linear(x, codes, scale, zero, bias)
@@ -152,7 +158,7 @@ def int4_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero:
 
 def _linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
             bias: torch.Tensor | None) -> torch.Tensor:
-    trains = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))
+    trains = torch.is_grad_enabled() and x.requires_grad
     k = x.shape[-1]
     rows = operand(as_rows(x))
     codes, scale, zero = _laid_out(codes, scale, zero, x.dtype)

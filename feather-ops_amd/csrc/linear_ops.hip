@@ -370,7 +370,7 @@ __device__ __forceinline__ void backward_rows(const BackwardParams& p, int at, i
             store_piece<kType, false>(out, at, valid, gate);
             store_piece<kType, false>(out + p.cols, at, valid, up);
             if (last)
-                for (int c = 2 * p.cols; c < ((2 * p.cols + 7) & ~7); ++c) out[c] = 0;
+                for (int c = 2 * p.cols; c < 2 * half; ++c) out[c] = 0;
         }
     }
     if (p.sums) {
@@ -474,7 +474,7 @@ extern "C" bool feather_gated_backward(const void* grad_y, int64_t ld_grad_y, co
     const int64_t F8 = (F + 7) / 8 * 8;
     if (M < 1 || M > kMaxSize || F < 1 || F > kMaxSize / 8 || !half_type(type) || activation < 0 || activation > 2 ||
         !matrix_ok(grad_y, ld_grad_y, M, F) || !aligned_to_type(grad_y, type) || !kept || !on_16(kept) || ld_kept % 4 != 0 ||
-        ld_kept < 2 * F8 || !grad || !on_16(grad) || ld_grad % 8 != 0 || ld_grad < 2 * F)
+        ld_kept < 2 * F8 || !grad || !on_16(grad) || ld_grad % 8 != 0 || ld_grad < 2 * F8)
         return false;
     const int group = rows_of(M, sums != nullptr);
     constexpr int64_t kMost = 65535;   // groups of rows of a launch

@@ -40,8 +40,7 @@ class GatedMLP(nn.Module):
         """(the layer's output, the residual stream h) for x and residual `[tokens, width]`."""
         y, h = fo.rms_norm(x, self.norm, residual, self.eps)
         if self.int4:
-            layer = self.gate_up
-            y = fo.int4_gated_linear(y, layer.weight_int4, layer.weight_scale, layer.weight_zero, activation=self.activation)
+            y = fo.int4_gated_linear(y, *self.gate_up.quantized_weight(), activation=self.activation)
         else:
             y = fo.gated_linear(y, self.gate_up.weight, activation=self.activation)
         return self.down(y), h

@@ -17,7 +17,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .block_scaled import _plain, _workspace, as_rows
+from .block_scaled import _UNKNOWN, _Source, _plain, _state_of, _workspace, as_rows
 from .gate import silu_mul
 from .gated import HALVES, _workspace_bytes as _gated_workspace_bytes, activate, activation_number, check_depth, operand
 from .modules import relabel_modules
@@ -144,6 +144,13 @@ def int4_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero:
     to x's dtype. Scales in another dtype than x's, scales and zero points that are not stored group by group, codes whose rows do
     not start on 4-byte boundaries, and rows of x off 16-byte boundaries or of no multiple of 8 values are copied on every call.
     K is at most 2**21, and so is N where x takes a gradient."""
+    return _checked_linear(x, codes, scale, zero, bias, None, _UNKNOWN)
+
+
+def _checked_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, bias: torch.Tensor | None,
+                    weight: torch.Tensor | None, source: tuple[int, int]) -> torch.Tensor:
+    """int4_linear; weight and source: what the codes were taken of, and its state then (_Source), for a traced program's passes to
+    see for themselves."""
     bias = _prepared(x, codes, bias)
     k = x.shape[-1]
     _check(codes, scale, zero, k)
@@ -152,7 +159,7 @@ def int4_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero:
     if torch.is_grad_enabled() and x.requires_grad:
         check_depth("x", codes.shape[0], "the weight's rows")
     if torch.compiler.is_compiling():
-        return _int4_linear_auto(x, codes, scale, zero, bias)
+        return _int4_linear_auto(x, codes, scale, zero, bias, weight, *source)
     return _linear(x, codes, scale, zero, bias)
 
 
@@ -199,20 +206,108 @@ def _gated(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torc
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 
 
-class Int4Linear:
-    """Mixin for `nn.Linear` (via `relabel_modules`): `forward` is `int4_linear` with the weight as it was when `quantize_weight_`
-    was called, 16-bit in and out. It is kept in three non-persistent buffers, `weight_int4`, `weight_scale` and `weight_zero`;
-    parameters and `state_dict` stay as they were. The weight is frozen; gradients reach the input and the bias, so the layer can
-    sit under trainable adapters."""
+# A state that no weight has: codes of another one.
+_STALE = (-1, -1)
 
-    def quantize_weight_(self, group: int = 128, zeros: bool = False) -> None:
-        codes, scale, zero = quantize_int4(self.weight, group, zeros=zeros)
-        self.register_buffer("weight_int4", codes, persistent=False)
-        self.register_buffer("weight_scale", scale, persistent=False)
-        self.register_buffer("weight_zero", zero, persistent=False)
+
+class Int4Linear:
+    """Mixin for `nn.Linear` (via `relabel_modules`): `forward` is `int4_linear`, 16-bit in and out. The weight is frozen; gradients
+    reach the input and the bias, so the layer can sit under trainable adapters.
+
+    The weight is quantized by `quantize_weight_` (which `to_int4_linear` calls) into three non-persistent buffers, `weight_int4`,
+    `weight_scale` and `weight_zero`. A pass that finds the weight changed (`load_state_dict`, another parameter in its place, another
+    type) quantizes it into them again, so a captured graph follows when the layer is next called or `quantize_weight_` is; what a layer
+    that is itself being captured or traced finds changed is quantized in that pass alone. Only writes through `weight.data`, which
+    torch does not count, and those to a weight made in inference mode need a call of `quantize_weight_`. A weight that was let go
+    (None, or of another shape) or moved to another device leaves the codes as they are. Parameters and `state_dict` stay as they
+    were."""
+
+    def quantize_weight_(self, group: int | None = None, zeros: bool | None = None) -> None:
+        """Quantize the weight as it is now, in groups of `group` columns, with zero points or without (None: as the layer has them, at
+        first 128 and without)."""
+        before = self.__dict__.get("_int4_format", (128, False, None))
+        group = before[0] if group is None else group
+        zeros = before[1] if zeros is None else zeros
+        dtype = self.weight.dtype if self.weight.dtype in HALVES else before[2]   # fp32: in the type that it had
+        fresh = quantize_int4(self.weight if dtype is None else self.weight.to(dtype), group, zeros=zeros)
+        kept = [self._buffers.get(name) for name in _BUFFERS]
+        if all((old is None) == (new is None) and (old is None or _can_hold(old, new)) for old, new in zip(kept, fresh)):
+            for old, new in zip(kept, fresh):   # in place, for graphs that read them
+                if old is not None:
+                    old.copy_(new)
+        else:
+            for name, new in zip(_BUFFERS, fresh):
+                self.register_buffer(name, new, persistent=False)
+        self._int4_format = (group, zeros, dtype)
+        self._codes_of = _Source(self.weight)
+
+    def register_parameter(self, name: str, param: nn.Parameter | None) -> None:
+        super().register_parameter(name, param)
+        if name == "weight":   # another one: what its codes were of is let go
+            self._codes_of = _Source(None)
+
+    def _apply(self, fn: Callable[[torch.Tensor], torch.Tensor], recurse: bool = True) -> nn.Module:
+        """To another device or type (`to`, `half`, ...), which the weight takes. Codes, scales and zero points move with it to a
+        device, and are taken of the weight as it is then on the GPU."""
+        kept = [(name, self._buffers.pop(name)) for name in _BUFFERS if name in self._buffers]
+        super()._apply(fn, recurse)
+        if kept:
+            device = fn(kept[0][1]).device
+            for name, buffer in kept:
+                if buffer is not None and buffer.device != device:
+                    buffer = torch.empty_like(buffer, device=device) if buffer.is_meta else buffer.to(device)
+                self.register_buffer(name, buffer, persistent=False)
+            if self.weight is not None and not self._is_current(self.weight):
+                self._codes_of = _Source(None)   # a later weight may lie where this one did
+                if self._takes(self.weight) and self.weight.is_cuda:
+                    self.quantize_weight_()
+        return self
+
+    def _takes(self, weight: torch.Tensor | None) -> bool:
+        """Whether codes are to follow a weight: one of their shape and on their device."""
+        codes = self._buffers["weight_int4"]
+        return (weight is not None and weight.dim() == 2 and weight.shape[0] == codes.shape[0]
+                and (weight.shape[1] + 1) // 2 == codes.shape[1] and weight.device == codes.device)
+
+    def _is_current(self, weight: torch.Tensor) -> bool:
+        source = self.__dict__.get("_codes_of")
+        return source is not None and source.weight is weight and source.state == _state_of(weight)
+
+    def quantized_weight(self) -> Int4Weight:
+        """The codes, scales and zero points, brought up to date. In a program that torch.compile traces they are taken as they are: the
+        layer's own node looks at them."""
+        weight, kept = self.weight, tuple(self._buffers[name] for name in _BUFFERS)
+        if torch.compiler.is_compiling() or not self._takes(weight) or self._is_current(weight):
+            return kept
+        if (not isinstance(weight, nn.Parameter) or torch._C._len_torch_dispatch_stack()
+                or (weight.is_cuda and torch.cuda.is_current_stream_capturing())):
+            return _requantized(weight, *kept)
+        self.quantize_weight_()
+        return tuple(self._buffers[name] for name in _BUFFERS)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return int4_linear(x, self.weight_int4, self.weight_scale, self.weight_zero, self.bias)
+        weight, state = self.weight, _UNKNOWN
+        codes, scale, zero = self.quantized_weight()
+        if torch.compiler.is_compiling() and self._takes(weight):
+            source = getattr(self, "_codes_of", None)
+            known = source is not None and source.weight is not None and isinstance(weight, nn.Parameter)
+            state = source.state if known else _STALE
+        return _checked_linear(x, codes, scale, zero, self.bias, None if state == _UNKNOWN else _plain(weight), state)
+
+
+_BUFFERS = ("weight_int4", "weight_scale", "weight_zero")
+
+
+def _can_hold(kept: torch.Tensor, new: torch.Tensor) -> bool:
+    return (kept.dtype == new.dtype and kept.shape == new.shape and kept.stride() == new.stride() and kept.device == new.device
+            and (torch.is_inference_mode_enabled() or not kept.is_inference()))
+
+
+def _requantized(weight: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None) -> Int4Weight:
+    """A weight in 4 bits as another one is."""
+    if weight.dtype not in HALVES:
+        weight = weight.to(scale.dtype)
+    return quantize_int4(weight, _group_of(weight.shape[1], scale.shape[1]), zeros=zero is not None)
 
 
 def to_int4_linear(root: nn.Module, group: int = 128, zeros: bool = False,
@@ -232,21 +327,31 @@ def to_int4_linear(root: nn.Module, group: int = 128, zeros: bool = False,
 # ---- one node each under torch.compile ----
 
 
+def _codes_now(weight: torch.Tensor | None, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, address: int,
+               version: int) -> Int4Weight:
+    """Codes if the weight is as it was when they were taken of it, as far as that is known, and else its own."""
+    if weight is None or (address, version) in (_UNKNOWN, _state_of(weight)):
+        return codes, scale, zero
+    return _requantized(weight, codes, scale, zero)
+
+
 @torch.library.custom_op("feather_ops::int4_linear_auto", mutates_args=())
 def _int4_linear_auto(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
-                      bias: torch.Tensor | None) -> torch.Tensor:
+                      bias: torch.Tensor | None, weight: torch.Tensor | None = None, address: int = 0,
+                      version: int = -1) -> torch.Tensor:
     """int4_linear as one opaque op."""
-    return _linear(x, codes, scale, zero, bias)
+    return _linear(x, *_codes_now(weight, codes, scale, zero, address, version), bias)
 
 
 @_int4_linear_auto.register_fake
-def _(x, codes, scale, zero, bias):
+def _(x, codes, scale, zero, bias, weight=None, address=0, version=-1):
     return x.new_empty((*x.shape[:-1], codes.shape[0]))
 
 
 @torch.library.custom_op("feather_ops::int4_linear_auto_backward", mutates_args=())
 def _int4_linear_auto_backward(grad: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
-                               k: int) -> torch.Tensor:
+                               k: int, weight: torch.Tensor | None = None, address: int = 0, version: int = -1) -> torch.Tensor:
+    codes, scale, zero = _codes_now(weight, codes, scale, zero, address, version)
     rows = operand(as_rows(grad))
     codes, scale, zero = _laid_out(codes, scale, zero, grad.dtype)
     need = max(0, _lib.c_library().feather_product_workspace_bytes(rows.shape[0], k, codes.shape[0]))
@@ -255,20 +360,25 @@ def _int4_linear_auto_backward(grad: torch.Tensor, codes: torch.Tensor, scale: t
 
 
 @_int4_linear_auto_backward.register_fake
-def _(grad, codes, scale, zero, k):
+def _(grad, codes, scale, zero, k, weight=None, address=0, version=-1):
     return grad.new_empty((*grad.shape[:-1], k))
 
 
 def _linear_auto_context(ctx, inputs, output) -> None:
-    x, codes, scale, zero, _ = inputs
-    ctx.save_for_backward(codes, scale, zero)
+    x, codes, scale, zero, _, weight, *ctx.source = inputs
+    ctx.save_for_backward(codes, scale, zero, weight)
     ctx.k = x.shape[-1]
 
 
 def _linear_auto_backward(ctx, grad: torch.Tensor) -> tuple:
-    need_x, _, _, _, need_bias = ctx.needs_input_grad
-    dx = _int4_linear_auto_backward(grad, *ctx.saved_tensors, ctx.k) if need_x else None
-    return dx, None, None, None, grad.reshape(-1, grad.shape[-1]).float().sum(0).to(grad.dtype) if need_bias else None
+    need_x, need_bias = ctx.needs_input_grad[0], ctx.needs_input_grad[4]
+    dx = db = None
+    if need_x:
+        codes, scale, zero, weight = ctx.saved_tensors
+        dx = _int4_linear_auto_backward(grad, codes, scale, zero, ctx.k, weight, *ctx.source)
+    if need_bias:
+        db = grad.reshape(-1, grad.shape[-1]).float().sum(0).to(grad.dtype)
+    return dx, None, None, None, db, None, None, None
 
 
 _int4_linear_auto.register_autograd(_linear_auto_backward, setup_context=_linear_auto_context)

@@ -52,10 +52,13 @@ def _group_of(k: int, groups: int) -> int:
 
 
 def _grouped(t: torch.Tensor) -> torch.Tensor:
-    """[N, groups] stored group by group, 4 values to a group at least (copied where it is not)."""
+    """[N, groups] stored group by group, with memory for 4 values to a group at least (copied where it is not)."""
     n, groups = t.shape
-    if (n <= 1 or t.stride(0) == 1) and (max(n, t.stride(1)) if groups <= 1 else t.stride(1)) >= max(n, 4):
-        return t
+    step = max(n, t.stride(1)) if groups <= 1 else t.stride(1)
+    if (n <= 1 or t.stride(0) == 1) and step >= max(n, 4):
+        end = t.storage_offset() + (groups - 1) * t.stride(1) + 4
+        if n >= 4 or end * t.element_size() <= t.untyped_storage().nbytes():
+            return t
     out = t.new_empty((groups, -(-n // 4) * 4))[:, :n].t()
     return out.copy_(t)
 

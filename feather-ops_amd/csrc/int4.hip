@@ -55,7 +55,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const WeightParams p
     if (p.zero) {
         low = across<kLanes>(low, false);
         high = across<kLanes>(high, true);
-        scale = (high - low) / 15.0f;
+        const float range = high - low;
+        scale = range < __builtin_huge_valf() ? range / 15.0f : high / 15.0f - low / 15.0f;   // past fp32's range
     } else {
         scale = __builtin_bit_cast(float, most) / 7.0f;
     }

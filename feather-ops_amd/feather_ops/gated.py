@@ -85,7 +85,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if x.numel() == 0 or weight.numel() == 0:
         gate, up = nn.functional.linear(x, weight, bias).chunk(2, -1)
         return activate(gate, act) * up
-    if torch.is_grad_enabled():
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         if x.requires_grad:
             check_depth("x", weight.shape[0], "the weight's rows")
         if weight.requires_grad:
@@ -96,10 +96,11 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
 
 
 def _gated(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, act: int) -> torch.Tensor:
-    records = torch.is_grad_enabled()
     rows, weight = operand(as_rows(x)), operand(as_rows(weight))
-    need = _workspace_bytes(int(rows.shape[0]), int(weight.shape[0]) // 2, int(rows.shape[1]), records and rows.requires_grad,
-                            records and weight.requires_grad)
+    need_x, need_weight = rows.requires_grad, weight.requires_grad
+    if not torch.is_grad_enabled():
+        need_x = need_weight = False
+    need = _workspace_bytes(int(rows.shape[0]), int(weight.shape[0]) // 2, int(rows.shape[1]), need_x, need_weight)
     y = torch.ops.feather_ops.gated_linear.default(rows, weight, bias, act, _workspace(rows, need) if need else None)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
 

@@ -44,6 +44,7 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, zeros: bool = False
     return codes[:, : -(-k // 2)], scale[:, :n].t(), zero[:, :n].t() if zeros else None
 
 
+@functools.lru_cache(maxsize=4096)
 def _group_of(k: int, groups: int) -> int:
     for group in GROUPS:
         if -(-k // group) == groups:
@@ -54,10 +55,10 @@ def _group_of(k: int, groups: int) -> int:
 def _grouped(t: torch.Tensor) -> torch.Tensor:
     """[N, groups] stored group by group, with memory for 4 values to a group at least (copied where it is not)."""
     n, groups = t.shape
-    step = max(n, t.stride(1)) if groups <= 1 else t.stride(1)
-    if (n <= 1 or t.stride(0) == 1) and step >= max(n, 4):
-        end = t.storage_offset() + (groups - 1) * t.stride(1) + 4
-        if n >= 4 or end * t.element_size() <= t.untyped_storage().nbytes():
+    first, step = t.stride()
+    if (n <= 1 or first == 1) and (max(n, step) if groups <= 1 else step) >= max(n, 4):
+        end = (groups - 1) * step + 4
+        if n >= 4 or (t.storage_offset() + end) * t.element_size() <= t.untyped_storage().nbytes():
             return t
     out = t.new_empty((groups, -(-n // 4) * 4))[:, :n].t()
     return out.copy_(t)
@@ -77,16 +78,17 @@ def _whole_bytes(codes: torch.Tensor) -> torch.Tensor:
 
 
 def _check(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, k: int) -> None:
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] != -(-k // 2):
-        raise ValueError(f"codes must be uint8 [N, {-(-k // 2)}], two columns to a byte, got {tuple(codes.shape)} {codes.dtype}")
-    if scale.dim() != 2 or scale.shape[0] != codes.shape[0] or not scale.dtype.is_floating_point:
-        raise ValueError(f"scale must be [{codes.shape[0]}, groups], got {tuple(scale.shape)} {scale.dtype}")
-    _group_of(k, scale.shape[1])
+    size, groups = codes.shape, scale.shape
+    if codes.dtype != torch.uint8 or len(size) != 2 or size[1] != -(-k // 2):
+        raise ValueError(f"codes must be uint8 [N, {-(-k // 2)}], two columns to a byte, got {tuple(size)} {codes.dtype}")
+    if len(groups) != 2 or groups[0] != size[0] or not scale.dtype.is_floating_point:
+        raise ValueError(f"scale must be [{size[0]}, groups], got {tuple(groups)} {scale.dtype}")
+    _group_of(int(k), int(groups[1]))   # int: the plan of a traced call fixes its sizes
     if scale.requires_grad:
         raise ValueError("a quantized weight takes no gradients")
     if zero is not None:
-        if zero.dtype != torch.uint8 or zero.shape != scale.shape:
-            raise ValueError(f"zero must be uint8 {tuple(scale.shape)}, got {tuple(zero.shape)} {zero.dtype}")
+        if zero.dtype != torch.uint8 or zero.shape != groups:
+            raise ValueError(f"zero must be uint8 {tuple(groups)}, got {tuple(zero.shape)} {zero.dtype}")
 
 
 def _laid_out(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, dtype: torch.dtype) -> Int4Weight:
@@ -159,7 +161,7 @@ def _checked_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, z
     _check(codes, scale, zero, k)
     if x.numel() == 0 or codes.numel() == 0:
         return nn.functional.linear(x, x.new_zeros((codes.shape[0], k)), bias)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         check_depth("x", codes.shape[0], "the weight's rows")
     if torch.compiler.is_compiling():
         return _int4_linear_auto(x, codes, scale, zero, bias, weight, *source)
@@ -168,7 +170,7 @@ def _checked_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, z
 
 def _linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None,
             bias: torch.Tensor | None) -> torch.Tensor:
-    trains = torch.is_grad_enabled() and x.requires_grad
+    trains = x.requires_grad and torch.is_grad_enabled()
     k = x.shape[-1]
     rows = operand(as_rows(x))
     codes, scale, zero = _laid_out(codes, scale, zero, x.dtype)
@@ -272,15 +274,16 @@ class Int4Linear:
         return (weight is not None and weight.dim() == 2 and weight.shape[0] == codes.shape[0]
                 and (weight.shape[1] + 1) // 2 == codes.shape[1] and weight.device == codes.device)
 
-    def _is_current(self, weight: torch.Tensor) -> bool:
+    def _is_current(self, weight: torch.Tensor | None) -> bool:
         source = self.__dict__.get("_codes_of")
-        return source is not None and source.weight is weight and source.state == _state_of(weight)
+        return source is not None and weight is not None and source.weight is weight and source.state == _state_of(weight)
 
     def quantized_weight(self) -> Int4Weight:
         """The codes, scales and zero points, brought up to date. In a program that torch.compile traces they are taken as they are: the
         layer's own node looks at them."""
-        weight, kept = self.weight, tuple(self._buffers[name] for name in _BUFFERS)
-        if torch.compiler.is_compiling() or not self._takes(weight) or self._is_current(weight):
+        weight, buffers = self.weight, self._buffers
+        kept = buffers["weight_int4"], buffers["weight_scale"], buffers["weight_zero"]
+        if torch.compiler.is_compiling() or self._is_current(weight) or not self._takes(weight):
             return kept
         if (not isinstance(weight, nn.Parameter) or torch._C._len_torch_dispatch_stack()
                 or (weight.is_cuda and torch.cuda.is_current_stream_capturing())):
@@ -289,13 +292,12 @@ class Int4Linear:
         return tuple(self._buffers[name] for name in _BUFFERS)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        weight, state = self.weight, _UNKNOWN
         codes, scale, zero = self.quantized_weight()
-        if torch.compiler.is_compiling() and self._takes(weight):
-            source = getattr(self, "_codes_of", None)
-            known = source is not None and source.weight is not None and isinstance(weight, nn.Parameter)
-            state = source.state if known else _STALE
-        return _checked_linear(x, codes, scale, zero, self.bias, None if state == _UNKNOWN else _plain(weight), state)
+        if not torch.compiler.is_compiling() or not self._takes(self.weight):
+            return int4_linear(x, codes, scale, zero, self.bias)
+        weight, source = self.weight, getattr(self, "_codes_of", None)
+        known = source is not None and source.weight is not None and isinstance(weight, nn.Parameter)
+        return _checked_linear(x, codes, scale, zero, self.bias, _plain(weight), source.state if known else _STALE)
 
 
 _BUFFERS = ("weight_int4", "weight_scale", "weight_zero")

@@ -1,6 +1,6 @@
 // The kernel for few rows, with 16-bit or 4-bit weights. The weight is read once, straight into registers, and that is what
 // bounds it; the rows of x, which every workgroup reads, go through LDS. One row of 4096 -> 14336 gated takes 44 us in 16 bits (5.3
-// TB/s) and 16.0 with 4-bit weights (3.7; the loads alone 14.5), 24 rows of 5120 -> 13824 57 and 32.5 (5.0 and 2.3; the loads alone
+// TB/s) and with 4-bit weights 16.4 in fp16 and 16.8 in bf16 (3.7; the loads alone 14.5), 24 rows of 5120 -> 13824 57 and 32.5 (5.0 and 2.3; the loads alone
 // 25: codes become 16 bits between them).
 //
 // A workgroup's waves are WK parts of K by WN parts of its columns. An iteration takes WK steps of 128 k's, one to each part: its
@@ -64,15 +64,10 @@ __device__ __forceinline__ void store_sums(const LinearParams& p, int m, int n, 
     store4<kBf16>(p, m, n, sum);
 }
 
-// Waves of a SIMD that a kernel's registers have to leave room for. (Left alone, those of two groups with zero points take 130: one
-// row of 5120 -> 13824 in bf16 19.8 us, with 5 of them spilled 18.1.)
-template <typename T, int kGroups, bool kZeros>
-constexpr int kFewWaves = T::RM == 1 && T::kThreads == 512 && kZeros && kGroups == 2 ? 4 : T::kThreads / 256;
-
 // kGroups: a step's groups of 4-bit codes (4, 2 or 1 of 32, 64 or 128), or 0: 16-bit weights. kZeros: the codes have zero points
 // of their own.
 template <typename T, int kGroups, bool kZeros, Form kForm, bool kBf16>
-__global__ __launch_bounds__(T::kThreads, (kFewWaves<T, kGroups, kZeros>)) void few_rows_kernel(const std::conditional_t<kGroups != 0, Int4Params, LinearParams> p) {
+__global__ __launch_bounds__(T::kThreads) void few_rows_kernel(const std::conditional_t<kGroups != 0, Int4Params, LinearParams> p) {
     constexpr bool kInt4 = kGroups != 0;
     constexpr int RM = T::RM, RN = T::RN, WK = T::WK, WN = T::WN;
     constexpr bool kGated = kForm != Form::kPlain;

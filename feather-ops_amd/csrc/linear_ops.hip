@@ -57,8 +57,8 @@ constexpr bool is_gated(Kind kind) { return kind != Kind::kPlain && kind != Kind
 Kind int4_kind(bool gated, bool fine) { return !gated ? Kind::kInt4 : fine ? Kind::kInt4GatedFine : Kind::kInt4Gated; }
 
 // Scales and zero points of many groups take registers that a gated kernel of 16 waves has not got: 24 rows of 5120 -> 13824 in
-// groups of 32 with zero points 88 us by 2_4_4 and 54 by 2_4_2, of 64 in bf16 50 and 43 (fp16 34 and 40); 1 row of 16384 -> 2048,
-// groups of 32, 2_16_1 49, 2_8_1 33.
+// groups of 32 with zero points 88 us by 2_4_4 and 54 by 2_4_2 (50 since bf16 keeps no sums of x), of 64 in bf16 50 and 43 (fp16 34 and
+// 40); 1 row of 16384 -> 2048, groups of 32, 2_16_1 49, 2_8_1 33.
 bool is_fine(int group, bool zeros, int type) { return zeros && (group == 32 || (group == 64 && type == FEATHER_BF16)); }
 
 const TileCost* tiles_begin(bool int4) { return int4 ? std::begin(kInt4Tiles) : std::begin(kTiles); }
@@ -314,6 +314,9 @@ void use_workspace(LinearParams& p, void* workspace) {
 // ---- the gated block's elementwise backward ----
 //
 //   grad_gate = dy up act'(gate)     grad_up = dy act(gate)
+//
+// They are rounded to 16 bits as operands of the products that follow, which is what the matrix units take: the gradients of x and the
+// weight are off by 2.35e-3 of their norm in bf16, of which their own rounding is 1.66e-3.
 //
 // A lane takes 8 columns of both halves of a few rows, whose loads are all in flight. Memory bounds it: 4096 x 12288 169 us, 4.2
 // TB/s (8 rows a lane, four by four, 172; 16 178). The bias's sums are kept over more rows, 16 of them (180 us and 20 MB of sums;

@@ -38,7 +38,8 @@ __device__ __forceinline__ bool join_splits(const P& p, f32x4 (&acc)[RM][RN], in
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    // As many loads in flight as there are registers for. (Left to itself the compiler waits for each: 1000 x 27648 x 5120 in 256 x
+    // As many loads in flight as there are registers for. (The block-scaled products, 71 split shapes of 1 to 4096 rows, take as long as
+    // with a loop over the parts alone: 1.000 of its time in the mean, 0.986 to 1.015.) (Left to itself the compiler waits for each: 1000 x 27648 x 5120 in 256 x
     // 256 tiles and three K ranges took 266 us, with 16 together 257.) Where a SIMD has one wave there is room for two batches: one
     // is loaded while the other is added.
     const auto add = [&](const f32x4 (&part)[kBatch], int s, int f0) {

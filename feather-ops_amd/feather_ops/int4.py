@@ -182,7 +182,8 @@ def _linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: tor
 def int4_gated_linear(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None,
                       bias: torch.Tensor | None = None, activation: str = "silu") -> torch.Tensor:
     """`gated_linear` with a 4-bit weight of 2 F rows, the gates' first: x `[..., K]`, the result `[..., F]`, in one launch up to 64
-    rows. Where x or bias takes gradients it is `int4_linear` and the activation of its outputs, in x's dtype."""
+    rows. Where x or bias takes gradients it is `int4_linear` and the activation of its outputs, in x's dtype: both sums are rounded
+    before the activation, so a pass that records gradients and one that does not differ by that."""
     act = activation_number(activation)
     bias = _prepared(x, codes, bias)
     if codes.dim() != 2 or codes.shape[0] % 2:

@@ -67,6 +67,19 @@ def test_largest_inputs(fo, m, group, zeros):
 
 
 @pytest.mark.parametrize("group,zeros", GROUPS)
+@pytest.mark.parametrize("exponent", [-118, -124])
+@pytest.mark.parametrize("m", ROWS)
+def test_smallest_inputs(fo, m, exponent, group, zeros):
+    """bfloat16's least values: no product of one with a code is lost where results have a place for it."""
+    dtype, k = torch.bfloat16, 300
+    weight = _weight(40, k, group, zeros, dtype, 1.0)
+    x = (torch.randn(m, k, device="cuda") * 2.0**exponent).to(dtype)
+    want, bound = ref.int4(x, *weight, None)
+    # terms are multiples of fp32's least value, 2^-149, in the sums' unit of 2048: each may be off by half of one
+    ref.check(fo.int4_linear(x, *weight), want, bound + k * 2.0**-150 * 2048)
+
+
+@pytest.mark.parametrize("group,zeros", GROUPS)
 @pytest.mark.parametrize("dtype", ref.HALVES)
 @pytest.mark.parametrize("m", ROWS)
 def test_sums_that_fp32_holds_are_exact(fo, m, dtype, group, zeros):
